@@ -1,0 +1,444 @@
+"""Paged key / value cache: step plans, page writes and attention over pages against plain 64-bit forms.
+
+Tolerance of attention.  With ``A = sum_j p_j |v_j|`` (p normalised): the probabilities are rounded to bf16 before they meet
+the values (half a step, 2^-8 of each: at most 2^-8 A in the sum), the result is rounded once (2^-8 |o|); scores are fp32
+sums of at most 256 products and of the probabilities' exponent, whose error moves a probability by less than 2^-12 for the
+scores of these tests (|s| < 64: 256 * 2^-24 * 64 = 2^-10 in the worst case of one-sided rounding, a sixteenth of that in
+any order a kernel sums in).  Together 2^-8 |o| + (2^-8 + 2^-12) A."""
+
+import math
+
+import pytest
+import torch
+
+from torchtitan_b200.ops import ext, paged, reference as ref
+
+DEVICES = [pytest.param("cpu"), pytest.param("cuda", marks=pytest.mark.gpu)]
+
+
+def _i32(x, device):
+    return torch.tensor(x, dtype=torch.int32, device=device)
+
+
+class _Step:
+    """A step over groups of sequences: ``groups = [(prefix tokens, [(cached behind the prefix, new rows), ...]), ...]``.
+    Page contents that no sequence owns are NaN, so that nothing outside a sequence can go unnoticed."""
+
+    def __init__(self, groups, *, hq, hkv, D, ps, device, pad=0, seed=0, extra_cols=0, interleaved_pools=False, dtype=torch.bfloat16):
+        g = torch.Generator().manual_seed(seed)
+        self.hq, self.hkv, self.D, self.ps = hq, hkv, D, ps
+        self.cached, self.new, start, prefix, own = [], [], [0], [], []
+        for p, members in groups:
+            for c, n in members:
+                self.cached.append(p + c)
+                self.new.append(n)
+                own.append(len(start) - 1)
+            start.append(len(self.cached))
+            prefix.append(p)
+        B = len(self.cached)
+        total = [c + n for c, n in zip(self.cached, self.new)]
+        W = max([1] + [-(-t // ps) for t in total]) + extra_cols
+        S = B + 3
+        slots = torch.randperm(S, generator=g)[:B].tolist()
+        n_pages = sum(-(-t // ps) for t in total) + 4
+        order = torch.randperm(n_pages, generator=g).tolist()
+        table = torch.full((S, W), -7, dtype=torch.int32)
+        self.pages_of = []
+        for b in range(B):
+            first = start[own[b]]
+            common = prefix[own[b]] // ps if b != first else 0
+            mine = self.pages_of[first][:common] if common else []
+            while len(mine) < -(-total[b] // ps):
+                mine = mine + [order.pop()]
+            self.pages_of.append(mine)
+            table[slots[b], :len(mine)] = torch.tensor(mine, dtype=torch.int32)
+        R = sum(self.new) + pad
+        kv = torch.full((2, n_pages, hkv, ps, D), float("nan"))
+        for b in range(B):
+            for j in range(-(-total[b] // ps)):
+                n = min(ps, total[b] - j * ps)
+                fresh = torch.isnan(kv[:, self.pages_of[b][j], :, :n, :1])
+                kv[:, self.pages_of[b][j], :, :n] = torch.where(fresh, torch.randn(2, hkv, n, D, generator=g), kv[:, self.pages_of[b][j], :, :n])
+        kv = kv.to(dtype)
+        if interleaved_pools:                      # keys and values of a page side by side: strided pools
+            pool = kv.transpose(0, 1).contiguous().to(device)
+            self.kp, self.vp = pool[:, 0], pool[:, 1]
+        else:
+            self.kp, self.vp = kv[0].contiguous().to(device), kv[1].contiguous().to(device)
+        self.q = torch.randn(R, hq, D, generator=g).to(dtype).to(device)
+        self.sink = torch.randn(hq, generator=g).to(device)
+        self.table, self.slots, self.n_pages, self.R, self.device = table.to(device), slots, n_pages, R, device
+        self.start, self.prefix = start, prefix
+        self.scale = 1 / math.sqrt(D)
+
+    def plan(self, windows=(0,), grouped=True, **kw):
+        d = self.device
+        held = _i32([len(p) for p in self.pages_of], d)
+        g = dict(group_start=_i32(self.start, d), group_prefix=_i32(self.prefix, d)) if grouped else {}
+        return paged.page_plan(_i32(self.cached, d), _i32(self.new, d), self.table, _i32(self.slots, d), _i32([], d), self.ps, self.R,
+                               num_pages=self.n_pages, mapped=held, n_heads=self.hq, n_kv_heads=self.hkv, windows=windows, **g, **kw)
+
+    def oracle(self, window=0, sinks=None):
+        """(o, sum_j p_j |v_j|) in 64 bits."""
+        out = torch.zeros(self.q.shape, dtype=torch.float64)
+        size = torch.zeros_like(out)
+        kp, vp, q, r = self.kp.cpu().double(), self.vp.cpu().double(), self.q.cpu().double(), 0
+        G = self.hq // self.hkv
+        for b in range(len(self.new)):
+            for i in range(self.new[b]):
+                pos = self.cached[b] + i
+                lo = max(0, pos - window + 1) if window else 0
+                j = torch.arange(lo, pos + 1)
+                page = torch.tensor(self.pages_of[b])[j // self.ps]
+                k, v = kp[page, :, j % self.ps], vp[page, :, j % self.ps]
+                s = torch.einsum("hgd,jhd->hgj", q[r].view(self.hkv, G, self.D), k) * self.scale
+                if sinks is not None:
+                    s = torch.cat([s, sinks.cpu().double().view(self.hkv, G, 1)], -1)
+                p = torch.softmax(s, -1)[..., :len(j)]
+                out[r] = torch.einsum("hgj,jhd->hgd", p, v).reshape(self.hq, self.D)
+                size[r] = torch.einsum("hgj,jhd->hgd", p, v.abs()).reshape(self.hq, self.D)
+                r += 1
+        return out, size
+
+    def check(self, got, window=0, sinks=None):
+        want, size = self.oracle(window, sinks)
+        n = sum(self.new)
+        err = (got[:n].cpu().double() - want[:n]).abs()
+        tol = 2 ** -8 * want[:n].abs() + (2 ** -8 + 2 ** -12) * size[:n]
+        assert (err <= tol).all(), (float((err - tol).max()), float(err.max()))
+
+
+# ------------------------------------------------------------------------------------------------------------------ plans
+def _plan_oracle(cached, new, table, slots, pages, mapped, ps, R):
+    """Token by token."""
+    table = table.clone()
+    it = iter(pages)
+    starts, pos, slot = [0], [], []
+    for c, n, s, m in zip(cached, new, slots, mapped):
+        for col in range(m, -(-(c + n) // ps)):
+            table[s, col] = next(it)
+        for j in range(c, c + n):
+            pos.append(j)
+            slot.append(int(table[s, j // ps]) * ps + j % ps)
+        starts.append(starts[-1] + n)
+    pad = R - len(pos)
+    return table, starts, pos + [0] * pad, slot + [-1] * pad
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("B,ps,top,most,pad", [(1, 16, 1, 1, 0), (1, 64, 500, 1, 3), (7, 16, 100, 40, 0), (300, 32, 2000, 3, 1), (64, 256, 90, 700, 5)])
+def test_plan(device, B, ps, top, most, pad):
+    g = torch.Generator().manual_seed(B)
+    cached = torch.randint(0, top, (B,), generator=g).tolist()
+    new = torch.randint(0, most + 1, (B,), generator=g).tolist()
+    new[0] = max(new[0], 1)
+    cached[0] = cached[0] // ps * ps                                   # a length that ends with its page
+    W = max(-(-(c + n) // ps) for c, n in zip(cached, new)) + 1
+    slots = torch.randperm(B + 4, generator=g)[:B].tolist()
+    held = [-(-c // ps) for c in cached]
+    mapped = list(held)
+    mapped[-1] = 0                                                     # a new sequence whose prefix pages come along
+    n_pages = sum(held) + sum(-(-(c + n) // ps) - m for c, n, m in zip(cached, new, mapped)) + 2
+    order = torch.randperm(n_pages, generator=g).tolist()
+    table = torch.full((B + 4, W), -9, dtype=torch.int32)
+    for s, h in zip(slots[:-1], held[:-1]):
+        table[s, :h] = torch.tensor([order.pop() for _ in range(h)], dtype=torch.int32)
+    need = sum(max(0, -(-(c + n) // ps) - m) for c, n, m in zip(cached, new, mapped))
+    pages = [order.pop() for _ in range(need)]
+    R = sum(new) + pad
+    want = _plan_oracle(cached, new, table, slots, pages, mapped, ps, R)
+    t = table.to(device)
+    p = paged.page_plan(_i32(cached, device), _i32(new, device), t, _i32(slots, device), _i32(pages, device), ps, R,
+                        num_pages=n_pages, mapped=_i32(mapped, device))
+    assert torch.equal(t.cpu(), want[0])
+    assert p.row_start.tolist() == want[1] and p.positions.tolist() == want[2] and p.slot_map.tolist() == want[3]
+    if device == "cuda":
+        assert ext.require().status(True) == 0
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_plan_without_sequences_or_rows(device):
+    table = torch.full((2, 3), 5, dtype=torch.int32, device=device)
+    e = _i32([], device)
+    p = paged.page_plan(e, e, table, e, e, 16, 4, num_pages=9)
+    assert p.row_start.tolist() == [0] and p.slot_map.tolist() == [-1] * 4 and p.positions.tolist() == [0] * 4
+    p = paged.page_plan(_i32([20], device), _i32([0], device), table, _i32([1], device), e, 16, 0, num_pages=9)
+    assert p.row_start.tolist() == [0, 0] and p.slot_map.numel() == 0
+    assert (table == 5).all()
+
+
+def test_plan_refusals_on_the_cpu():
+    table = torch.zeros(2, 3, dtype=torch.int32)
+    call = lambda c, n, s, pages, R=8, **kw: paged.page_plan(_i32(c, "cpu"), _i32(n, "cpu"), table, _i32(s, "cpu"), _i32(pages, "cpu"),
+                                                             kw.get("ps", 16), R, num_pages=4)
+    with pytest.raises(ValueError, match="page_size"):
+        call([0], [1], [0], [0], ps=24)
+    with pytest.raises(ValueError, match="block table"):
+        call([0], [1], [2], [0])
+    with pytest.raises(ValueError, match="block table"):
+        call([47], [2], [0], [0])
+    with pytest.raises(ValueError, match="too few pages"):
+        call([0], [1], [0], [])
+    with pytest.raises(ValueError, match="outside the pool"):
+        call([0], [1], [0], [4])
+    with pytest.raises(ValueError, match="same slot"):
+        call([0, 0], [1, 1], [0, 0], [0, 1])
+    with pytest.raises(ValueError, match="total_rows"):
+        call([0], [9], [0], [0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cached,new,slots,pages,R,ps", [
+    ([0], [1], [2], [0], 8, 16), ([0], [1], [-1], [0], 8, 16), ([47], [2], [0], [0], 8, 16), ([0], [1], [0], [], 8, 16),
+    ([0], [1], [0], [4], 8, 16), ([0], [1], [0], [-2], 8, 16), ([0, 0], [1, 1], [0, 0], [0, 1], 8, 16), ([0], [9], [0], [0], 8, 16),
+    ([-3], [1], [0], [0], 8, 16), ([2 ** 31 - 1], [1], [0], [0], 8, 16), ([0], [2 ** 31 - 1], [0], [0], 8, 16), ([0], [-1], [0], [0], 8, 16)])
+def test_bad_device_data_sets_the_status_and_stays_inside(cached, new, slots, pages, R, ps):
+    """What the CPU form refuses is flagged on the device: bad rows get slot -1 (or are left out), nothing outside the table is
+    written, and attention and writes on such a plan return."""
+    ops = ext.require()
+    ops.status(True)
+    guard = torch.full((6, 3), -5, dtype=torch.int32, device="cuda")
+    table = guard[2:4]
+    p = paged.page_plan(_i32(cached, "cuda"), _i32(new, "cuda"), table, _i32(slots, "cuda"), _i32(pages, "cuda"), ps, R, num_pages=4,
+                        n_heads=8, n_kv_heads=2)
+    assert ops.status(True) & 16
+    assert (guard[:2] == -5).all() and (guard[4:] == -5).all()
+    assert ((p.slot_map >= -1) & (p.slot_map < 4 * ps)).all() and int(p.row_start[-1]) <= R
+    kp, vp = (torch.zeros(4, 2, ps, 64, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    x = torch.ones(R, 2, 64, device="cuda", dtype=torch.bfloat16)
+    paged.write_kv(x, x, kp, vp, p.slot_map)
+    paged.attention(torch.ones(R, 8, 64, device="cuda", dtype=torch.bfloat16), kp, vp, p, 0.1)
+    torch.cuda.synchronize()
+    ops.status(True)
+
+
+# ----------------------------------------------------------------------------------------------------------------- writes
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("T,hkv,D,ps,dtype", [(1, 1, 64, 16, torch.bfloat16), (37, 3, 128, 32, torch.float32), (500, 8, 256, 64, torch.bfloat16),
+                                              (5, 2, 8, 16, torch.bfloat16)])
+def test_write(device, T, hkv, D, ps, dtype):
+    g = torch.Generator().manual_seed(T)
+    n_pages = T // ps + 5
+    pool = torch.randn(n_pages, 2, hkv, ps, D, generator=g).to(dtype).to(device)
+    kp, vp = pool[:, 0], pool[:, 1]                                    # strided pools
+    packed = torch.randn(T, 4 * hkv, D, generator=g).to(dtype).to(device)
+    k, v = packed[:, hkv:2 * hkv], packed[:, 3 * hkv:]                 # strided rows
+    slot = torch.randperm(n_pages * ps, generator=g)[:T]
+    slot[T // 2] = -1 if T > 1 else slot[0]
+    want_k, want_v = kp.clone(), vp.clone()
+    for t, s in enumerate(slot.tolist()):
+        if s >= 0:
+            want_k[s // ps, :, s % ps], want_v[s // ps, :, s % ps] = k[t], v[t]
+    paged.write_kv(k, v, kp, vp, slot.to(device))
+    assert torch.equal(kp, want_k) and torch.equal(vp, want_v)
+    before = pool.clone()
+    paged.write_kv(k[:0], v[:0], kp, vp, slot[:0].to(device))          # no rows
+    assert torch.equal(pool, before)
+    odd = torch.zeros(k.numel() + 1, dtype=dtype, device=device)[1:].view(T, hkv, D)       # vectors not on 16 bytes
+    odd.copy_(v)
+    paged.write_kv(odd, odd, kp, vp, slot.to(device))
+    live = slot.to(device) >= 0
+    assert torch.equal(kp.transpose(1, 2).reshape(-1, hkv, D)[slot.to(device)[live]], v[live])
+
+
+@pytest.mark.gpu
+def test_write_past_32_bit_offsets_and_out_of_range_slots():
+    n_pages, ps = 20000, 64
+    kp = torch.zeros(n_pages, 8, ps, 256, device="cuda", dtype=torch.bfloat16)             # 2.6e9 elements
+    x = torch.randn(3, 8, 256, device="cuda").to(torch.bfloat16)
+    slots = torch.tensor([n_pages * ps - 1, 0, 17000 * ps + 5], device="cuda")
+    paged.write_kv(x, x, kp, kp, slots)
+    flat = kp.transpose(1, 2)
+    for i, s in enumerate(slots.tolist()):
+        assert torch.equal(flat[s // ps, s % ps], x[i])
+    ops = ext.require()
+    assert ops.status(True) == 0
+    paged.write_kv(x, x, kp, kp, torch.tensor([n_pages * ps, -4, 2 ** 40], device="cuda"))
+    assert ops.status(True) & 16
+
+
+def test_write_refusals():
+    kp = torch.zeros(2, 2, 16, 64)
+    with pytest.raises((RuntimeError, IndexError, ValueError)):
+        paged.write_kv(torch.zeros(3, 1, 64), torch.zeros(3, 1, 32), kp, kp, torch.zeros(3, dtype=torch.int64))
+
+
+# -------------------------------------------------------------------------------------------------------------- attention
+_SHAPES = [
+    # groups, hq, hkv, D, ps, window
+    ([(0, [(0, 1)])], 4, 4, 64, 16, 0),                                            # one token, nothing cached
+    ([(0, [(5, 1), (64, 1), (63, 1), (0, 1), (200, 1)])], 8, 2, 128, 16, 0),       # a group without a prefix
+    ([(0, [(300, 1)]), (0, [(17, 1)]), (0, [(0, 3)]), (0, [(31, 0)]), (0, [(33, 2)])], 8, 1, 128, 32, 0),
+    ([(0, [(1000, 1)])], 28, 4, 128, 64, 0),                                       # seven query heads per key head
+    ([(0, [(130, 20)]), (0, [(0, 70)])], 16, 4, 128, 64, 0),                       # many rows a sequence
+    ([(128, [(0, 1), (7, 1), (70, 1)]), (0, [(9, 1)]), (64, [(1, 2), (0, 1)])], 8, 2, 128, 64, 0),
+    ([(256, [(i, 1) for i in range(20)])], 32, 4, 128, 16, 0),                     # many rows behind one prefix
+    ([(192, [(3, 1), (50, 2), (0, 1)]), (0, [(400, 3)])], 8, 2, 64, 64, 100),      # a window that ends inside the prefix
+    ([(0, [(90, 5)]), (0, [(500, 1)])], 64, 8, 64, 16, 33),
+    ([(64, [(20, 1), (3, 1)]), (0, [(40, 4)])], 16, 4, 256, 32, 0),
+    ([(0, [(77, 1)])], 40, 1, 64, 256, 7),
+    ([(512, [(10, 9), (0, 30), (100, 1)])], 8, 2, 128, 128, 0),
+]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("shape", range(len(_SHAPES)))
+@pytest.mark.parametrize("sinks", [False, True])
+def test_attention(device, shape, sinks):
+    groups, hq, hkv, D, ps, window = _SHAPES[shape]
+    s = _Step(groups, hq=hq, hkv=hkv, D=D, ps=ps, device=device, pad=2 if shape % 2 else 0, seed=shape, extra_cols=shape % 3,
+              interleaved_pools=shape % 2 == 0)
+    sink = s.sink if sinks else None
+    for grouped in (True, False):
+        got = paged.attention(s.q, s.kp, s.vp, s.plan((window,), grouped), s.scale, window=window, sinks=sink)
+        s.check(got, window, sink)
+        assert not got[sum(s.new):].any()                                           # rows behind the last sequence
+    if device == "cuda":
+        assert ext.require().status(True) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("groups,hq,hkv,D,ps,window", [
+    ([(0, [(20000, 1)])], 8, 2, 128, 64, 0),                                        # one long sequence: its axis is split
+    ([(0, [(c, 1)]) for c in (3000, 1, 77, 2048, 640, 12, 4000)], 32, 8, 128, 64, 0),
+    ([(2048, [(c, 1) for c in range(0, 320, 8)]), (1024, [(5, 1)] * 3), (0, [(999, 1)])], 16, 4, 128, 64, 0),
+    ([(4096, [(c, 2) for c in range(33)])], 16, 2, 64, 32, 0),
+    ([(3000 // 16 * 16, [(c, 1) for c in range(12)])], 16, 2, 256, 16, 500),
+    ([(0, [(1000, 500)])], 8, 2, 128, 64, 0),                                       # a chunk of a prompt
+    ([(0, [(6000, 1), (100, 1)])], 32, 1, 64, 128, 1024),
+])
+def test_attention_long(groups, hq, hkv, D, ps, window):
+    s = _Step(groups, hq=hq, hkv=hkv, D=D, ps=ps, device="cuda", seed=3)
+    got = paged.attention(s.q, s.kp, s.vp, s.plan((window,)), s.scale, window=window)
+    s.check(got, window)
+    again = paged.attention(s.q, s.kp, s.vp, s.plan((window,)), s.scale, window=window)
+    assert torch.equal(got, again)                                                  # the order of the sums is fixed
+
+
+@pytest.mark.gpu
+def test_attention_writes_into_out_and_leaves_the_padding_alone():
+    s = _Step([(64, [(5, 1), (9, 1)]), (0, [(30, 2)])], hq=8, hkv=2, D=128, ps=16, device="cuda", pad=3)
+    out = torch.full(s.q.shape, 7.0, dtype=s.q.dtype, device="cuda")
+    got = paged.attention(s.q, s.kp, s.vp, s.plan(), s.scale, out=out)
+    assert got is out and (out[-3:] == 7).all()
+    s.check(out)
+    want = out.clone()
+    wide = torch.zeros(s.R, 20, 128, dtype=s.q.dtype, device="cuda")                # queries as a slice of a packed projection
+    wide[:, :8] = s.q
+    assert torch.equal(paged.attention(wide[:, :8], s.kp, s.vp, s.plan(), s.scale, out=out)[:-3], want[:-3])
+    odd = torch.zeros(s.q.numel() + 1, dtype=s.q.dtype, device="cuda")[1:].view(s.q.shape)
+    odd.copy_(s.q)
+    assert torch.equal(paged.attention(odd, s.kp, s.vp, s.plan(), s.scale, out=out)[:-3], want[:-3])
+
+
+@pytest.mark.gpu
+def test_attention_with_extreme_scores_and_infinite_keys_outside():
+    """Scores of +-3e4 (one key takes everything), equal scores, and a sequence whose neighbour's pages hold infinities."""
+    s = _Step([(0, [(100, 1)]), (0, [(50, 1)])], hq=4, hkv=2, D=64, ps=16, device="cuda")
+    s.kp[s.pages_of[0][0], 0, 3] = 300.0
+    s.q[0] = 1.0
+    s.q[1] = 0.0                                                                    # all scores equal
+    want, size = s.oracle()
+    got = paged.attention(s.q, s.kp, s.vp, s.plan(), s.scale)
+    assert ((got.cpu().double() - want).abs() <= 2 ** -8 * want.abs() + (2 ** -8 + 2 ** -12) * size).all()
+    s.kp[s.pages_of[0][1]] = float("inf")
+    other = paged.attention(s.q, s.kp, s.vp, s.plan(), s.scale)
+    assert torch.equal(other[1], got[1])
+
+
+@pytest.mark.gpu
+def test_attention_past_32_bit_offsets():
+    ps, D, hkv = 64, 128, 8
+    n_pages = 36000                                                                  # 2.4e9 elements a pool
+    kp, vp = (torch.zeros(n_pages, hkv, ps, D, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    ids = [35999, 3, 35998]
+    g = torch.Generator("cuda").manual_seed(0)
+    for i in ids:
+        kp[i] = torch.randn(hkv, ps, D, device="cuda", generator=g).to(kp.dtype)
+        vp[i] = torch.randn(hkv, ps, D, device="cuda", generator=g).to(kp.dtype)
+    q = torch.randn(1, 8, D, device="cuda", generator=g).to(kp.dtype)
+    table = _i32([ids], "cuda")
+    plan = lambda t, n: paged.page_plan(_i32([149], "cuda"), _i32([1], "cuda"), t, _i32([0], "cuda"), _i32([], "cuda"), ps, 1,
+                                        num_pages=n, mapped=_i32([3], "cuda"), n_heads=8, n_kv_heads=hkv)
+    a = paged.attention(q, kp, vp, plan(table, n_pages), 0.1)
+    b = paged.attention(q, kp[ids].contiguous(), vp[ids].contiguous(), plan(_i32([[0, 1, 2]], "cuda"), 3), 0.1)
+    assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_attention_refusals(device):
+    s = _Step([(0, [(5, 1)])], hq=4, hkv=2, D=64, ps=16, device=device)
+    plan = s.plan()
+    with pytest.raises(ValueError, match="query rows"):
+        paged.attention(s.q.repeat(2, 1, 1), s.kp, s.vp, plan, 1.0)
+    with pytest.raises(ValueError, match="pools"):
+        paged.attention(s.q, s.kp[:-1], s.vp[:-1], plan, 1.0)
+    with pytest.raises(ValueError, match="pools"):
+        paged.attention(s.q, s.kp, s.vp[..., :32], plan, 1.0)
+    with pytest.raises(ValueError, match="queries"):
+        paged.attention(s.q[:, :3], s.kp, s.vp, plan, 1.0)
+
+
+@pytest.mark.gpu
+def test_other_types_take_the_counted_plain_form():
+    from torchtitan_b200.ops import functional as OF
+
+    s = _Step([(0, [(20, 1)])], hq=4, hkv=2, D=64, ps=16, device="cuda", dtype=torch.float32)
+    n0 = OF.settings.library_fallbacks
+    got = paged.attention(s.q, s.kp, s.vp, s.plan(), s.scale)
+    assert OF.settings.library_fallbacks == n0 + 1
+    want, size = s.oracle()
+    assert ((got.cpu().double() - want).abs() <= 2 ** -12 * (size + want.abs())).all()
+
+
+@pytest.mark.gpu
+def test_a_captured_step_replays_on_other_lengths_and_pages():
+    """Plan, write and attention in one graph: the lengths and tables are device data, so a replay follows them."""
+    dev, ps, hq, hkv, D, B, W, n_pages = "cuda", 16, 8, 2, 128, 3, 20, 70
+    kp, vp = (torch.zeros(n_pages, hkv, ps, D, device=dev, dtype=torch.bfloat16) for _ in range(2))
+    cached, new, slots = _i32([0, 0, 0], dev), _i32([1, 1, 1], dev), _i32([0, 1, 2], dev)
+    table = torch.arange(B * W, device=dev, dtype=torch.int32).view(B, W).contiguous()
+    mapped = _i32([W] * B, dev)
+    none = _i32([], dev)
+    q = torch.zeros(4, hq, D, device=dev, dtype=torch.bfloat16)
+    k, v = (torch.zeros(4, hkv, D, device=dev, dtype=torch.bfloat16) for _ in range(2))
+
+    def step():
+        p = paged.page_plan(cached, new, table, slots, none, ps, 4, num_pages=n_pages, mapped=mapped, n_heads=hq, n_kv_heads=hkv)
+        paged.write_kv(k, v, kp, vp, p.slot_map)
+        return paged.attention(q, kp, vp, p, 0.1)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for _ in range(2):                                 # two graphs of the same step, replayed in turn
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            o = step()
+        graphs.append((g, o))
+    rnd = torch.Generator(dev).manual_seed(1)
+    for i, lens in enumerate([(5, 100, 0), (300, 1, 64), (17, 200, 31), (3, 4, 5)]):
+        for t in (q, k, v, kp, vp):
+            t.copy_(torch.randn(t.shape, device=dev, generator=rnd).to(t.dtype))
+        cached.copy_(_i32(lens, dev))
+        new.copy_(_i32([1, 2, 1] if i % 2 else [1, 1, 1], dev))
+        g, o = graphs[i % 2]
+        g.replay()
+        got = o.clone()
+        assert torch.equal(got, step())
+
+
+@pytest.mark.gpu
+def test_a_side_stream_gives_the_same_result():
+    s = _Step([(64, [(5, 1), (9, 1)]), (0, [(700, 2)])], hq=8, hkv=2, D=128, ps=16, device="cuda")
+    want = paged.attention(s.q, s.kp, s.vp, s.plan(), s.scale)
+    outs, streams = [], [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for st in streams:                                  # two calls at once
+        with torch.cuda.stream(st):
+            outs.append(paged.attention(s.q, s.kp, s.vp, s.plan(), s.scale))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs)

@@ -18,6 +18,23 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> mla_assemble_bwd(const at::Tensor
 at::Tensor conv_silu_fwd(const at::Tensor& x, const at::Tensor& w, const c10::optional<at::Tensor>& pos);
 std::tuple<at::Tensor, at::Tensor> conv_silu_bwd(const at::Tensor& x, const at::Tensor& w,
                                                  const c10::optional<at::Tensor>& pos, const at::Tensor& dy);
+std::tuple<at::Tensor, at::Tensor> qk_norm_rope_fwd(const at::Tensor& x, int64_t hq, int64_t hkv, const c10::optional<at::Tensor>& qw,
+                                                    const c10::optional<at::Tensor>& kw, const c10::optional<at::Tensor>& table,
+                                                    const c10::optional<at::Tensor>& positions, const c10::optional<at::Tensor>& axes,
+                                                    bool interleaved, double eps, double gain, double q_scale);
+std::tuple<at::Tensor, at::Tensor> qk_norm_rope_bwd(const at::Tensor& dq, const at::Tensor& dk, const c10::optional<at::Tensor>& dv,
+                                                    const at::Tensor& x, int64_t hq, int64_t hkv, const c10::optional<at::Tensor>& qw,
+                                                    const c10::optional<at::Tensor>& kw, const c10::optional<at::Tensor>& table,
+                                                    const c10::optional<at::Tensor>& positions, const c10::optional<at::Tensor>& axes,
+                                                    bool interleaved, double eps, double gain, double q_scale);
+std::tuple<at::Tensor, at::Tensor, at::Tensor> page_plan(const at::Tensor& cached, const at::Tensor& new_rows, at::Tensor block_table,
+                                                         const at::Tensor& slots, const at::Tensor& pages,
+                                                         const c10::optional<at::Tensor>& mapped, int64_t page_size,
+                                                         int64_t total_rows, int64_t num_pages);
+void paged_write(const at::Tensor& k, const at::Tensor& v, at::Tensor k_pages, at::Tensor v_pages, const at::Tensor& slot_map);
+void paged_attention_simple(const at::Tensor& q, const at::Tensor& k_pages, const at::Tensor& v_pages, const at::Tensor& block_table,
+                            const at::Tensor& slots, const at::Tensor& cached, const at::Tensor& row_start, double scale, int64_t window,
+                            const c10::optional<at::Tensor>& sinks, at::Tensor out, bool zero_tail);
 int64_t status(bool clear);
 at::Tensor cross_entropy_(at::Tensor logits, const at::Tensor& labels, const at::Tensor& scale);
 void adamw_(at::Tensor master, const at::Tensor& grad, at::Tensor exp_avg, at::Tensor exp_avg_sq,
@@ -108,6 +125,16 @@ TORCH_LIBRARY(tb200, m) {
         &tb200::mla_assemble_bwd);
   m.def("conv_silu_fwd(Tensor x, Tensor w, Tensor? pos) -> Tensor", &tb200::conv_silu_fwd);
   m.def("conv_silu_bwd(Tensor x, Tensor w, Tensor? pos, Tensor dy) -> (Tensor, Tensor)", &tb200::conv_silu_bwd);
+  m.def("qk_norm_rope_fwd(Tensor x, int hq, int hkv, Tensor? qw, Tensor? kw, Tensor? table, Tensor? positions, Tensor? axes, "
+        "bool interleaved, float eps, float gain, float q_scale) -> (Tensor, Tensor)", &tb200::qk_norm_rope_fwd);
+  m.def("qk_norm_rope_bwd(Tensor dq, Tensor dk, Tensor? dv, Tensor x, int hq, int hkv, Tensor? qw, Tensor? kw, Tensor? table, "
+        "Tensor? positions, Tensor? axes, bool interleaved, float eps, float gain, float q_scale) -> (Tensor, Tensor)",
+        &tb200::qk_norm_rope_bwd);
+  m.def("page_plan(Tensor cached, Tensor new_rows, Tensor(a!) block_table, Tensor slots, Tensor pages, Tensor? mapped, int page_size, "
+        "int total_rows, int num_pages) -> (Tensor, Tensor, Tensor)", &tb200::page_plan);
+  m.def("paged_write(Tensor k, Tensor v, Tensor(a!) k_pages, Tensor(b!) v_pages, Tensor slot_map) -> ()", &tb200::paged_write);
+  m.def("paged_attention_simple(Tensor q, Tensor k_pages, Tensor v_pages, Tensor block_table, Tensor slots, Tensor cached, "
+        "Tensor row_start, float scale, int window, Tensor? sinks, Tensor(a!) out, bool zero_tail) -> ()", &tb200::paged_attention_simple);
   m.def("status(bool clear) -> int", &tb200::status);
   m.def("cross_entropy_(Tensor(a!) logits, Tensor labels, Tensor scale) -> Tensor", &tb200::cross_entropy_);
   m.def("adamw_(Tensor(a!) master, Tensor grad, Tensor(b!) exp_avg, Tensor(c!) exp_avg_sq, Tensor(d!)? lowp, "

@@ -15,6 +15,7 @@ enum StatusBits : int {
   kStatusRopePositionOutOfRange = 1 << 0,
   kStatusLabelOutOfRange = 1 << 1,
   kStatusWaitTimedOut = 1 << 2,
+  kStatusPagePlanInvalid = 1 << 4,  // a page table, slot or page id outside its range, or too few pages or columns
 };
 
 struct __align__(16) bf16x8 {

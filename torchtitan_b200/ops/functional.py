@@ -34,7 +34,7 @@ import torch.nn.functional as F
 from . import ext, reference as ref
 
 __all__ = [
-    "settings", "rms_norm", "linear", "norm_linear", "swiglu", "swiglu_linear", "rope_qk_", "rope",
+    "settings", "rms_norm", "linear", "norm_linear", "swiglu", "swiglu_linear", "rope_qk_", "rope", "qk_norm_rope",
     "attention", "attention_packed", "linear_cross_entropy", "cross_entropy_sum", "gemm_nt", "gemm_nn", "gemm_tn", "embedding",
 ]
 
@@ -492,6 +492,76 @@ def rope_qk_(qkv: torch.Tensor, table: torch.Tensor, positions: torch.Tensor, in
              head_dim: int):
     """In-place RoPE on the q and k heads of a packed projection output ``[T, (Hq+2Hkv)*D]``."""
     return _RopeQKInplaceFn.apply(qkv, table, positions, interleaved, n_rot_heads, head_dim)
+
+
+# =====================================================================
+# Per-head norms of queries and keys + RoPE
+# =====================================================================
+def _heads_ok(t: torch.Tensor) -> torch.Tensor:
+    """``t[T, H, D]`` with adjacent heads and 16-byte aligned rows, copied only when it is not."""
+    if t.stride(2) == 1 and (t.stride(1) == t.shape[2] or t.shape[1] == 1) and t.stride(0) % 8 == 0 and t.data_ptr() % 16 == 0:
+        return t.as_strided(t.shape, (t.stride(0), t.shape[2], 1))
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+class _QKNormRopeFn(torch.autograd.Function):
+    """Keeps the projection output only: the backward reads it in any case and recomputes each head's rsqrt."""
+
+    @staticmethod
+    def forward(ctx, qkv, q_weight, k_weight, table, positions, axes, meta):
+        hq, hkv = meta[0], meta[1]
+        x = qkv
+        if _cuda(qkv):
+            _count()
+            x = _heads_ok(qkv)
+            q, k = ext.require().qk_norm_rope_fwd(x, hq, hkv, q_weight, k_weight, table, positions, axes, *meta[2:])
+        else:
+            q, k = ref.qk_norm_rope_fwd(x, hq, hkv, q_weight, k_weight, table, positions, axes, *meta[2:])
+        ctx.save_for_backward(x, q_weight, k_weight, table, positions, axes)
+        ctx.meta = meta
+        return q, k, qkv[:, hq + hkv:]
+
+    @staticmethod
+    def backward(ctx, dq, dk, dv):
+        x, q_weight, k_weight, table, positions, axes = ctx.saved_tensors
+        hq, hkv = ctx.meta[:2]
+        if _cuda(x):
+            _count(1 if q_weight is None and k_weight is None else 2)
+            dx, dw = ext.require().qk_norm_rope_bwd(_heads_ok(dq), _heads_ok(dk), _heads_ok(dv), x, hq, hkv, q_weight, k_weight, table,
+                                                    positions, axes, *ctx.meta[2:])
+        else:
+            dx, dw = ref.qk_norm_rope_bwd(dq, dk, dv, x, hq, hkv, q_weight, k_weight, table, positions, axes, *ctx.meta[2:])
+        dws = [_deliver_wgrad(w, dw[i]) if w is not None and ctx.needs_input_grad[1 + i] else None
+               for i, w in enumerate((q_weight, k_weight))]
+        return dx, dws[0], dws[1], None, None, None, None
+
+
+def qk_norm_rope(qkv: torch.Tensor, n_heads: int, n_kv_heads: int, q_weight: torch.Tensor | None, k_weight: torch.Tensor | None,
+                 table: torch.Tensor | None, positions: torch.Tensor | None, interleaved: bool, *, eps: float = 1e-6,
+                 gain_center: float = 0.0, q_scale: float = 1.0, axes: torch.Tensor | None = None):
+    """RMSNorm of every query and key head and the rotary embedding in one pass over a packed projection output.
+
+    ``qkv [T, Hq + 2 Hkv, D]`` -> ``(q [T, Hq, D], k [T, Hkv, D], v)`` with ``v`` a view of ``qkv``: each head vector is
+    scaled by its ``rsqrt(mean(x^2) + eps)`` and by ``weight + gain_center`` (nothing when the weight is None), queries
+    also by ``q_scale``, and its first ``table.shape[1]`` elements are rotated (``table = None``: no rotation).
+    ``positions [T]`` int64 index the fp32 ``table`` (``cos | sin``); with several position axes ``positions`` is
+    ``[axes, T]`` and ``axes [rot / 2]`` (int32) names the axis that each frequency follows.  The result is rounded
+    once.  bf16 or fp32, head dimensions up to 256 in multiples of 8, rotary widths in multiples of 16 (8 when
+    ``interleaved``)."""
+    if qkv.dim() != 3 or qkv.shape[1] != n_heads + 2 * n_kv_heads:
+        raise ValueError(f"qk_norm_rope: expected [T, {n_heads} + 2 * {n_kv_heads}, D], got {tuple(qkv.shape)}")
+    if table is not None:
+        want = (qkv.shape[0],) if axes is None else (positions.shape[0], qkv.shape[0])
+        if tuple(positions.shape) != want:
+            raise ValueError(f"qk_norm_rope: positions {tuple(positions.shape)} do not fit {qkv.shape[0]} tokens"
+                             + ("" if axes is None else " on several axes"))
+        if table.shape[1] > qkv.shape[2] or table.shape[1] % (8 if interleaved else 16):
+            raise ValueError(f"qk_norm_rope: rotary width {table.shape[1]} for head dimension {qkv.shape[2]}")
+        positions = positions.long().contiguous()
+    else:
+        positions = axes = None
+    meta = (int(n_heads), int(n_kv_heads), bool(interleaved), float(eps), float(gain_center), float(q_scale))
+    return _QKNormRopeFn.apply(qkv, q_weight, k_weight, table, positions, axes, meta)
 
 
 # =====================================================================

@@ -1,0 +1,116 @@
+"""Paged key / value cache: the plan of a step, the write of its new rows, and attention over the pages.
+
+A layer's cache is a pair of pools ``k_pages, v_pages [num_pages, Hkv, page_size, D]``; the pages of a sequence are listed
+in its row (*slot*) of ``block_table [slots, columns]``.  A step feeds a flat stream of new rows: ``new[b]`` rows of the
+sequence in slot ``slots[b]``, which has ``cached[b]`` tokens in its pages already.  ``page_plan`` extends the table rows
+by the pages handed out and computes, on the device, where every row goes; ``write_kv`` stores the rows' keys and values;
+``attention`` lets every row attend to its sequence's tokens up to and including itself.
+
+Sequences that share a prefix (their tables begin with the same pages) may be passed as groups of neighbours: the prefix
+is then attended to once for all rows of the group and merged with what follows it.
+
+Lengths and tables live on the device and are checked there: an entry that is out of range is skipped (its row gets slot
+-1) and bit 16 of ``torch.ops.tb200.status`` is set.  On CPU tensors the plain forms of ``ops/reference.py`` run, which
+raise instead.
+"""
+
+from __future__ import annotations
+
+from dataclasses import dataclass
+
+import torch
+
+from . import ext, reference as ref
+from .functional import _count, _library_fallback
+
+__all__ = ["PagePlan", "page_plan", "write_kv", "attention", "supported"]
+
+PAGE_SIZES = (16, 32, 64, 128, 256)
+HEAD_DIMS = (64, 128, 256)
+
+
+@dataclass(eq=False)
+class PagePlan:
+    """Where the rows of one step go; made once per step and used by every layer."""
+
+    row_start: torch.Tensor      # [B + 1] int32: first row of each sequence in the flat stream
+    positions: torch.Tensor      # [R] int64: position of each row in its sequence (0 behind the last sequence)
+    slot_map: torch.Tensor       # [R] int64: page * page_size + offset of each row, -1 = nowhere
+    cached: torch.Tensor
+    slots: torch.Tensor
+    block_table: torch.Tensor
+    page_size: int
+    num_pages: int
+    total_rows: int
+
+
+def supported(q: torch.Tensor, k_pages: torch.Tensor) -> bool:
+    """Shapes of the attention kernels: bf16, head dimension 64, 128 or 256."""
+    return q.is_cuda and q.dtype == torch.bfloat16 and k_pages.dtype == torch.bfloat16 and q.shape[-1] in HEAD_DIMS
+
+
+def page_plan(cached: torch.Tensor, new: torch.Tensor, block_table: torch.Tensor, slots: torch.Tensor, pages: torch.Tensor,
+              page_size: int, total_rows: int, *, num_pages: int, mapped: torch.Tensor | None = None,
+              group_start: torch.Tensor | None = None, group_prefix: torch.Tensor | None = None, n_heads: int | None = None,
+              n_kv_heads: int | None = None, windows: tuple[int, ...] = (0,), max_rows: int | None = None) -> PagePlan:
+    """Plan of one step over ``B = len(slots)`` sequences (all index tensors int32 on one device).
+
+    ``pages`` are the ids handed out, in the order of the sequences: sequence ``b`` takes as many as it needs for
+    ``cached[b] + new[b]`` tokens beyond the ``mapped[b]`` columns of its table row that are filled already (default:
+    those that hold its cached tokens).  ``total_rows`` is the length of the flat stream, at least ``sum(new)``."""
+    if page_size not in PAGE_SIZES:
+        raise ValueError(f"page_plan: page_size must be one of {PAGE_SIZES}, got {page_size}")
+    args = (cached, new, block_table, slots, pages, mapped, int(page_size), int(total_rows), int(num_pages))
+    if block_table.is_cuda:
+        _count()
+        row_start, positions, slot_map = ext.require().page_plan(*args)
+    else:
+        row_start, positions, slot_map = ref.page_plan(*args)
+    return PagePlan(row_start, positions, slot_map, cached, slots, block_table, int(page_size), int(num_pages), int(total_rows))
+
+
+def _vectors(t: torch.Tensor) -> torch.Tensor:
+    """``t`` itself when its last dimension is contiguous and every vector starts on 16 bytes, else a copy."""
+    e = t.element_size()
+    if t.stride(-1) == 1 and all((s * e) % 16 == 0 for s in t.stride()[:-1]) and t.data_ptr() % 16 == 0:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def write_kv(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, slot_map: torch.Tensor) -> None:
+    """Store ``k, v [R, Hkv, D]`` at their slots of the pools; rows with slot -1 are left out."""
+    if k_pages.is_cuda:
+        _count()
+        ext.require().paged_write(_vectors(k), _vectors(v), k_pages, v_pages, slot_map)
+    else:
+        ref.paged_write(k, v, k_pages, v_pages, slot_map)
+
+
+def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, plan: PagePlan, scale: float, *, window: int = 0,
+              sinks: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """``q [R, Hq, D]`` -> ``[R, Hq, D]``: row ``r`` at position ``p`` of its sequence attends to the tokens
+    ``max(0, p - window + 1) .. p`` (``window = 0``: all up to ``p``).  ``sinks [Hq]``: one logit per head in the softmax
+    denominator.  Rows behind the last sequence are zero, or left as they are when ``out`` is given."""
+    if q.shape[0] != plan.total_rows:
+        raise ValueError(f"paged attention: {q.shape[0]} query rows, the plan has {plan.total_rows}")
+    if tuple(k_pages.shape) != tuple(v_pages.shape) or k_pages.shape[0] != plan.num_pages or k_pages.shape[2] != plan.page_size:
+        raise ValueError(f"paged attention: pools {tuple(k_pages.shape)} / {tuple(v_pages.shape)} do not fit a plan of "
+                         f"{plan.num_pages} pages of {plan.page_size}")
+    if q.shape[1] % k_pages.shape[1] or q.shape[2] != k_pages.shape[3]:
+        raise ValueError(f"paged attention: queries {tuple(q.shape)} against pools {tuple(k_pages.shape)}")
+    if not supported(q, k_pages):
+        if q.is_cuda:
+            _library_fallback(f"paged attention on {q.dtype} with head dimension {q.shape[-1]}")
+        o = ref.paged_attention(q, k_pages, v_pages, plan.block_table, plan.slots, plan.cached, plan.row_start, float(scale),
+                                int(window), sinks)
+        if out is None:
+            return o
+        n = int(plan.row_start[-1])
+        out[:n] = o[:n]
+        return out
+    _count()
+    dst = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
+    ext.require().paged_attention_simple(_vectors(q), k_pages, v_pages, plan.block_table, plan.slots, plan.cached, plan.row_start,
+                                         float(scale), int(window), None if sinks is None else sinks.float().contiguous(), dst,
+                                         out is None)
+    return dst

@@ -111,6 +111,123 @@ def rope_apply(x: torch.Tensor, table: torch.Tensor, positions: torch.Tensor, in
     return out.to(x.dtype)
 
 
+# ------------------------------------------------- per-head norms of queries and keys + RoPE
+def _rope_rows(table: torch.Tensor, positions: torch.Tensor, axes: torch.Tensor | None):
+    """``(cos, sin) [T, 1, rot / 2]``; with ``axes`` frequency f follows ``positions[axes[f]]``."""
+    half = table.shape[1] // 2
+    if axes is None:
+        cs = table[positions.long()]
+        return cs[:, None, :half], cs[:, None, half:]
+    f = torch.arange(half, device=table.device)
+    at = positions.long()[axes.long()].t()
+    return table[at, f][:, None], table[at, f + half][:, None]
+
+
+def _rotate(xf: torch.Tensor, cos, sin, interleaved: bool) -> torch.Tensor:
+    half = cos.shape[-1]
+    xr, rest = xf[..., :2 * half], xf[..., 2 * half:]
+    if interleaved:
+        a, b = xr[..., 0::2], xr[..., 1::2]
+        y = torch.stack([a * cos - b * sin, a * sin + b * cos], dim=-1).flatten(-2)
+    else:
+        a, b = xr[..., :half], xr[..., half:]
+        y = torch.cat([a * cos - b * sin, b * cos + a * sin], dim=-1)
+    return torch.cat([y, rest], dim=-1) if rest.shape[-1] else y
+
+
+def qk_norm_rope_fwd(x, hq, hkv, qw, kw, table, positions, axes, interleaved, eps, gain, q_scale):
+    """``x [T, Hq + 2 Hkv, D]`` -> normalised, rotated ``q [T, Hq, D]``, ``k [T, Hkv, D]`` (rounded once)."""
+    out = []
+    for xs, w, scale in ((x[:, :hq], qw, q_scale), (x[:, hq:hq + hkv], kw, 1.0)):
+        n = xs.float()
+        n = n * torch.rsqrt(n.pow(2).mean(-1, keepdim=True) + eps)
+        n = n * scale if w is None else n * ((w.float() + gain) * scale)
+        if table is not None:
+            n = _rotate(n, *_rope_rows(table, positions, axes), interleaved)
+        out.append(n.to(x.dtype).contiguous())
+    return out[0], out[1]
+
+
+def qk_norm_rope_bwd(dq, dk, dv, x, hq, hkv, qw, kw, table, positions, axes, interleaved, eps, gain, q_scale):
+    """``(dx of x's shape, dw [2, D] fp32)``; ``dv = None`` is zero."""
+    dx = torch.zeros_like(x, memory_format=torch.contiguous_format)
+    dw = torch.zeros(2 if (qw is not None or kw is not None) else 0, x.shape[2], dtype=torch.float32, device=x.device)
+    for i, (h0, h1, d, w, scale) in enumerate(((0, hq, dq, qw, q_scale), (hq, hq + hkv, dk, kw, 1.0))):
+        xf, dn = x[:, h0:h1].float(), d.float()
+        if table is not None:
+            cos, sin = _rope_rows(table, positions, axes)
+            dn = _rotate(dn, cos, -sin, interleaved)
+        r = torch.rsqrt(xf.pow(2).mean(-1, keepdim=True) + eps)
+        xh = xf * r
+        if dw.shape[0]:
+            dw[i] = (dn * xh).sum((0, 1)) * scale
+        g = dn * scale if w is None else dn * ((w.float() + gain) * scale)
+        dx[:, h0:h1] = (r * (g - xh * (g * xh).mean(-1, keepdim=True))).to(x.dtype)
+    if dv is not None:
+        dx[:, hq + hkv:] = dv
+    return dx, dw
+
+
+# -------------------------------------------------------------- paged key / value cache
+def page_plan(cached, new, block_table, slots, pages, mapped, page_size: int, total_rows: int, num_pages: int):
+    """Extends the sequences' rows of ``block_table`` (in place) by ``pages`` and returns ``(row_start [B + 1] int32,
+    positions [R] int64, slot_map [R] int64)``.  Lists of a CPU run are small: plain loops, every index checked."""
+    cached, new, slots, pages = (t.tolist() for t in (cached, new, slots, pages))
+    held = [-(-c // page_size) for c in cached] if mapped is None else mapped.tolist()
+    S, W = block_table.shape
+    if len(set(slots)) != len(slots):
+        raise ValueError("page_plan: the same slot twice")
+    row_start, positions, slot_map, at = [0], [], [], 0
+    for c, n, s, have in zip(cached, new, slots, held):
+        end = -(-(c + n) // page_size)
+        if c < 0 or n < 0 or not 0 <= s < S or end > W:
+            raise ValueError(f"page_plan: sequence of {c} + {n} tokens in slot {s} does not fit a {S} x {W} block table")
+        take = pages[at:at + max(0, end - have)]
+        if len(take) < end - have or any(not 0 <= i < num_pages for i in take):
+            raise ValueError("page_plan: too few pages, or a page outside the pool")
+        block_table[s, have:have + len(take)] = torch.tensor(take, dtype=block_table.dtype)
+        at += len(take)
+        row = block_table[s].tolist()
+        for j in range(c, c + n):
+            positions.append(j)
+            slot_map.append(row[j // page_size] * page_size + j % page_size)
+        row_start.append(row_start[-1] + n)
+    if row_start[-1] > total_rows:
+        raise ValueError(f"page_plan: {row_start[-1]} new rows, but total_rows is {total_rows}")
+    pad = total_rows - row_start[-1]
+    dev = block_table.device
+    return (torch.tensor(row_start, dtype=torch.int32, device=dev), torch.tensor(positions + [0] * pad, dtype=torch.int64, device=dev),
+            torch.tensor(slot_map + [-1] * pad, dtype=torch.int64, device=dev))
+
+
+def paged_write(k, v, k_pages, v_pages, slot_map) -> None:
+    live = slot_map >= 0
+    ps = k_pages.shape[2]
+    page, off = slot_map[live] // ps, slot_map[live] % ps
+    k_pages[page, :, off] = k[live]
+    v_pages[page, :, off] = v[live]
+
+
+def paged_attention(q, k_pages, v_pages, block_table, slots, cached, row_start, scale: float, window: int, sinks):
+    """Per sequence: gather its pages and attend densely (fp32).  Rows behind the last sequence are zero."""
+    out = torch.zeros(q.shape, dtype=q.dtype, device=q.device)
+    Hq, D = q.shape[1:]
+    Hkv, ps = k_pages.shape[1:3]
+    rs = row_start.tolist()
+    for b, (s, c) in enumerate(zip(slots.tolist(), cached.tolist())):
+        r0, r1 = rs[b], rs[b + 1]
+        if r1 == r0:
+            continue
+        L = c + r1 - r0
+        ids = block_table[s, :-(-L // ps)].long()
+        k, v = (p[ids].transpose(0, 1).reshape(Hkv, -1, D)[:, :L].transpose(0, 1) for p in (k_pages, v_pages))
+        o, lse = block_attention_fwd(q[r0:r1], k, v, scale, True, c, None, window)
+        if sinks is not None:
+            o = (o.float() * torch.sigmoid(lse - sinks.float()[:, None]).t()[..., None]).to(q.dtype)
+        out[r0:r1] = o
+    return out
+
+
 # ----------------------------------------------------------------- SwiGLU
 def swiglu_fwd(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
     return (F.silu(gate.float()) * up.float()).to(gate.dtype)
