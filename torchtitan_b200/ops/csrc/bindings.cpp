@@ -32,9 +32,12 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> page_plan(const at::Tensor& cache
                                                          const c10::optional<at::Tensor>& mapped, int64_t page_size,
                                                          int64_t total_rows, int64_t num_pages);
 void paged_write(const at::Tensor& k, const at::Tensor& v, at::Tensor k_pages, at::Tensor v_pages, const at::Tensor& slot_map);
-void paged_attention_simple(const at::Tensor& q, const at::Tensor& k_pages, const at::Tensor& v_pages, const at::Tensor& block_table,
-                            const at::Tensor& slots, const at::Tensor& cached, const at::Tensor& row_start, double scale, int64_t window,
-                            const c10::optional<at::Tensor>& sinks, at::Tensor out, bool zero_tail);
+at::Tensor paged_work(const at::Tensor& cached, const at::Tensor& row_start, const at::Tensor& slots, const c10::optional<at::Tensor>& group_start,
+                      const c10::optional<at::Tensor>& group_prefix, int64_t table_cols, int64_t page_size,
+                      int64_t total_rows, int64_t hq, int64_t hkv, int64_t window);
+void paged_attention(const at::Tensor& q, const at::Tensor& k_pages, const at::Tensor& v_pages, const at::Tensor& table,
+                     const at::Tensor& cached, const at::Tensor& row_start, const at::Tensor& work, int64_t groups, double scale,
+                     int64_t window, const c10::optional<at::Tensor>& sinks, at::Tensor out, bool zero_tail);
 int64_t status(bool clear);
 at::Tensor cross_entropy_(at::Tensor logits, const at::Tensor& labels, const at::Tensor& scale);
 void adamw_(at::Tensor master, const at::Tensor& grad, at::Tensor exp_avg, at::Tensor exp_avg_sq,
@@ -133,8 +136,10 @@ TORCH_LIBRARY(tb200, m) {
   m.def("page_plan(Tensor cached, Tensor new_rows, Tensor(a!) block_table, Tensor slots, Tensor pages, Tensor? mapped, int page_size, "
         "int total_rows, int num_pages) -> (Tensor, Tensor, Tensor)", &tb200::page_plan);
   m.def("paged_write(Tensor k, Tensor v, Tensor(a!) k_pages, Tensor(b!) v_pages, Tensor slot_map) -> ()", &tb200::paged_write);
-  m.def("paged_attention_simple(Tensor q, Tensor k_pages, Tensor v_pages, Tensor block_table, Tensor slots, Tensor cached, "
-        "Tensor row_start, float scale, int window, Tensor? sinks, Tensor(a!) out, bool zero_tail) -> ()", &tb200::paged_attention_simple);
+  m.def("paged_work(Tensor cached, Tensor row_start, Tensor slots, Tensor? group_start, Tensor? group_prefix, int table_cols, "
+        "int page_size, int total_rows, int hq, int hkv, int window) -> Tensor", &tb200::paged_work);
+  m.def("paged_attention(Tensor q, Tensor k_pages, Tensor v_pages, Tensor table, Tensor cached, Tensor row_start, Tensor work, "
+        "int groups, float scale, int window, Tensor? sinks, Tensor(a!) out, bool zero_tail) -> ()", &tb200::paged_attention);
   m.def("status(bool clear) -> int", &tb200::status);
   m.def("cross_entropy_(Tensor(a!) logits, Tensor labels, Tensor scale) -> Tensor", &tb200::cross_entropy_);
   m.def("adamw_(Tensor(a!) master, Tensor grad, Tensor(b!) exp_avg, Tensor(c!) exp_avg_sq, Tensor(d!)? lowp, "

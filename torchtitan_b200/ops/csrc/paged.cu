@@ -7,8 +7,10 @@
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <cuda.h>
 
 #include "common.cuh"
+#include "tc.cuh"
 
 namespace tb200 {
 int* status_word_ptr();
@@ -20,6 +22,7 @@ constexpr int kMaxSlots = 65536;        // rows of the block table: one bit each
 constexpr int kMaxCols = 1 << 20;       // columns of the block table and rows of a step: a block's scan stays inside 32 bits
 constexpr int kMaxRows = 1 << 22;
 constexpr int kMaxLength = 1 << 30;     // tokens of one sequence
+constexpr int kMinTiles = 2;            // a CTA's stretch is at least this long: shorter ones cost more to join than they save
 
 // Inclusive scan over the block; `part` needs 33 entries.
 __device__ __forceinline__ int block_scan(int v, int* part, int& total) {
@@ -184,76 +187,633 @@ __global__ void __launch_bounds__(256) write_kernel(const WriteParams p) {
 }
 
 // ------------------------------------------------------------------------------------------------------------- attention
-struct SimpleParams {
-  const __nv_bfloat16* q;
-  int64_t q_row, q_head;
-  const __nv_bfloat16 *kp, *vp;
-  int64_t kp_page, kp_head, kp_slot, vp_page, vp_head, vp_slot;   // in elements
-  const int *table, *slots, *cached, *row_start;
-  const float* sinks;
-  __nv_bfloat16* out;                     // [R, Hq, D]
-  int B, S, W, R, Hq, Hkv, D, ps, num_pages, window;
-  float scale;
-  bool zero_tail;
+// Work.  A *source* is a set of neighbouring rows that all look at one key range of one table row: the rows of a sequence
+// on what follows its group's prefix, or all rows of a group on the prefix.  Its (row, query head of one key head) pairs
+// are cut into *units* of kUnitRows; a unit's keys are cut into tiles.  The tiles of all units and key heads form one line
+// that is cut into equal stretches, one per CTA, whatever the lengths are: a CTA works through the *pieces* of units that
+// fall into its stretch.  A piece that covers its unit is finished where it is; the others leave (max, sum, unnormalised
+// fp32 output) behind, at most two per CTA (the first and the last of a stretch), which the combine kernel joins in the
+// order of the line, so results do not depend on scheduling.  A group's two sources are joined there as well.
+constexpr int kUnitRows = 16;                    // pairs of a unit: one m16 tile
+constexpr int kTile = 64;                        // keys per tile
+
+struct Unit {
+  int row0, pairs, pair0, slot;                  // first row and pair count of the source, first pair of the unit, table row
+  int key_lo, key_hi, base, direct;              // keys [lo, hi); position of the source's first row, or -1 for a prefix; alone
+};
+
+// Layout of the int32 work buffer (one per window), from the sizes that the host knows.
+struct WorkLayout {
+  int64_t seq_group, src_unit, tiles, units, size;   // header: [0] units, [1] tiles (of one key head)
+  __host__ __device__ WorkLayout(int64_t B, int64_t NG, int64_t max_units) {
+    seq_group = 4;
+    src_unit = seq_group + B;
+    tiles = (src_unit + B + NG + 3) / 4 * 4;
+    units = (tiles + max_units + 1 + 3) / 4 * 4;
+    size = units + 8 * max_units;
+  }
+};
+
+struct WorkParams {
+  const int *cached, *row_start, *slots, *group_start, *group_prefix;
+  int B, NG, W, ps, G, window, max_units;
+  int* work;
   int* status;
 };
 
-// One block of four warps per (row, query head); a warp takes every fourth key, its lanes hold D / 32 elements each.
-__global__ void __launch_bounds__(128) simple_kernel(const SimpleParams p) {
-  __shared__ float sm_m[4], sm_l[4], sm_o[4][256];
-  const int r = blockIdx.x / p.Hq, h = blockIdx.x % p.Hq;
+__global__ void __launch_bounds__(1024) work_kernel(const WorkParams p) {
+  extern __shared__ int sm[];
+  const int n_src = p.B + p.NG;
+  int* unit_start = sm;                          // [n_src + 1]
+  int* prefix = sm + n_src + 1;                  // [NG] tokens of the group's prefix, as used
+  int* leader = prefix + p.NG;                   // [NG] first sequence with rows
+  __shared__ int part[33];
+  const WorkLayout lay(p.B, p.NG, p.max_units);
+  int* seq_group = p.work + lay.seq_group;
+  int* src_unit = p.work + lay.src_unit;
+  int* tiles = p.work + lay.tiles;
+  Unit* units = reinterpret_cast<Unit*>(p.work + lay.units);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int per = p.D / 32;
-  __nv_bfloat16* out = p.out + ((int64_t)r * p.Hq + h) * p.D;
+  bool bad = false;
+  for (int b = threadIdx.x; b < p.B; b += blockDim.x) seq_group[b] = -1;
+  __syncthreads();
+  // groups: one warp each.  The prefix ends at the shortest member, and a group with one live sequence shares nothing.
+  for (int g = warp; g < p.NG; g += blockDim.x / 32) {
+    const int a = min(max(p.group_start[g], 0), p.B), e = min(max(p.group_start[g + 1], a), p.B);
+    bad |= a != p.group_start[g] || e != p.group_start[g + 1];
+    int live = 0, shortest = INT_MAX, first = INT_MAX;
+    for (int b = a + lane; b < e; b += 32) {
+      if (p.row_start[b + 1] == p.row_start[b]) continue;
+      ++live;
+      shortest = min(shortest, p.cached[b]);
+      first = min(first, b);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      live += __shfl_xor_sync(0xffffffffu, live, o);
+      shortest = min(shortest, __shfl_xor_sync(0xffffffffu, shortest, o));
+      first = min(first, __shfl_xor_sync(0xffffffffu, first, o));
+    }
+    const int use = live > 1 ? max(0, min(p.group_prefix[g], shortest)) : 0;
+    if (lane == 0) { prefix[g] = use; leader[g] = first; }
+    if (use > 0)
+      for (int b = a + lane; b < e; b += 32) seq_group[b] = g;
+  }
+  __syncthreads();
+  auto source_rows = [&](int s, int& r0, int& r1) {
+    if (s < p.B) {
+      r0 = p.row_start[s];
+      r1 = p.row_start[s + 1];
+    } else {
+      const int g = s - p.B;
+      r0 = r1 = 0;
+      if (prefix[g] > 0) {
+        r0 = p.row_start[min(max(p.group_start[g], 0), p.B)];
+        r1 = p.row_start[min(max(p.group_start[g + 1], 0), p.B)];
+      }
+    }
+  };
+  int n_units = 0;
+  for (int s0 = 0; s0 < n_src; s0 += blockDim.x) {
+    const int s = s0 + threadIdx.x;
+    int n = 0;
+    if (s < n_src) {
+      int r0, r1;
+      source_rows(s, r0, r1);
+      n = (int)(((int64_t)(r1 - r0) * p.G + kUnitRows - 1) / kUnitRows);
+    }
+    int total;
+    const int e = block_scan(n, part, total);
+    if (s < n_src) {
+      unit_start[s] = n_units + e - n;
+      src_unit[s] = n > 0 ? n_units + e - n : -1;
+    }
+    n_units += total;
+  }
+  if (threadIdx.x == 0) unit_start[n_src] = n_units;
+  if (n_units > p.max_units) {                   // overlapping groups: device data that is flagged
+    bad = true;
+    n_units = p.max_units;
+  }
+  __syncthreads();
+  int n_tiles = 0;
+  for (int u0 = 0; u0 < n_units; u0 += blockDim.x) {
+    const int u = u0 + threadIdx.x;
+    int n = 0;
+    if (u < n_units) {
+      const int s = find_segment(unit_start, n_src, u);
+      int r0, r1;
+      source_rows(s, r0, r1);
+      Unit w;
+      w.row0 = r0;
+      w.pairs = (r1 - r0) * p.G;
+      w.pair0 = (u - unit_start[s]) * kUnitRows;
+      const int last = min(w.pair0 + kUnitRows, w.pairs) - 1;
+      const int64_t room = (int64_t)p.W * p.ps;
+      if (s < p.B) {
+        const int g = seq_group[s], c = p.cached[s];
+        w.slot = p.slots[s];
+        w.base = c;
+        w.direct = g < 0;
+        w.key_lo = g < 0 ? 0 : prefix[g];
+        if (p.window > 0) w.key_lo = max(w.key_lo, c + w.pair0 / p.G - p.window + 1);
+        w.key_hi = (int)min((int64_t)c + last / p.G + 1, room);
+      } else {
+        const int g = s - p.B;
+        w.slot = p.slots[min(leader[g], p.B - 1)];
+        w.base = -1;
+        w.direct = 0;
+        // the smallest position of the group's rows bounds the window of all of them
+        int from = 0;
+        if (p.window > 0) {
+          from = INT_MAX;
+          const int a = min(max(p.group_start[g], 0), p.B), e = min(max(p.group_start[g + 1], a), p.B);
+          for (int b = a; b < e; ++b)
+            if (p.row_start[b + 1] > p.row_start[b]) from = min(from, p.cached[b]);
+          from = max(0, from - p.window + 1);
+        }
+        w.key_lo = from;
+        w.key_hi = (int)min((int64_t)prefix[g], room);
+      }
+      n = w.key_hi > w.key_lo ? (w.key_hi - 1) / kTile - w.key_lo / kTile + 1 : 0;
+      units[u] = w;
+    }
+    int total;
+    const int e = block_scan(n, part, total);
+    if (u < n_units) tiles[u] = n_tiles + e - n;
+    n_tiles += total;
+  }
+  if (threadIdx.x == 0) {
+    tiles[n_units] = n_tiles;
+    p.work[0] = n_units;
+    p.work[1] = n_tiles;
+  }
+  if (bad) atomicOr(p.status, kStatusPagePlanInvalid);
+}
+
+struct AttnParams {
+  const __nv_bfloat16* q;
+  int64_t q_row, q_head;
+  __nv_bfloat16* out;                            // [R, Hq, D]
+  const float* sinks;                            // [Hq] or null
+  const int *table, *cached, *row_start, *work;
+  int B, NG, S, W, R, Hq, Hkv, G, ps, num_pages, window, max_units, ctas;
+  float scale_log2;
+  bool zero_tail;
+  float *part_o, *part_ml;                       // [ctas, 2, kUnitRows, D], [ctas, 2, kUnitRows, 2]: pieces
+  float *row_o, *row_ml;                         // [2, R, Hq, D], [2, R, Hq, 2]: whole units of groups (own keys, prefix)
+  int* status;
+};
+
+template <int D>
+struct Cfg {
+  static constexpr int kStages = D == 64 ? 4 : D == 128 ? 3 : 2;
+  static constexpr int kCtasPerSm = D == 256 ? 1 : 2;
+  static constexpr uint32_t kHalfBytes = kTile * D * 2;          // keys (or values) of a tile
+  static constexpr uint32_t kStageBytes = 2 * kHalfBytes;
+  static constexpr uint32_t kExchange = 2 * kUnitRows * D * 4;   // two fp32 output tiles
+  static constexpr uint32_t kSmem = kStages * kStageBytes + kExchange + 4 * kUnitRows * 2 * 4 + 16 * kStages + 16;
+};
+
+__device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack2bf(float lo, float hi) {
+  __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&h);
+}
+__device__ __forceinline__ void consumer_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+// The same, true for all when any thread brings true.
+__device__ __forceinline__ bool consumer_any(bool v) {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred a, b;\n\tsetp.ne.u32 a, %1, 0;\n\tbar.red.or.pred b, 1, 128, a;\n\tselp.u32 %0, 1, 0, b;\n\t}"
+               : "=r"(r) : "r"((uint32_t)v) : "memory");
+  return r != 0;
+}
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2, int c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+      ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
+}
+
+// Tiles of a CTA's stretch.
+__device__ __forceinline__ int64_t stretch(const int* work, int Hkv, int ctas) {
+  return max((int64_t)kMinTiles, ((int64_t)work[1] * Hkv + ctas - 1) / ctas);
+}
+
+// A CTA's walk over its stretch of the line.
+struct Walk {
+  const int* tiles;
+  const Unit* units;
+  int n_units, Hkv;
+  int64_t at, end;
+  int u, head, first, count;                     // current piece: unit, key head, first tile of the unit, tiles
+  int unit_tiles;
+
+  __device__ __forceinline__ Walk(const int* work, const WorkLayout& lay, int Hkv_, int cta, int ctas) : Hkv(Hkv_) {
+    tiles = work + lay.tiles;
+    units = reinterpret_cast<const Unit*>(work + lay.units);
+    n_units = work[0];
+    const int64_t line = (int64_t)work[1] * Hkv, per = stretch(work, Hkv, ctas);
+    at = min(line, cta * per);
+    end = min(line, at + per);
+    u = at < end ? find_segment(tiles, n_units, (int)(at / Hkv)) : 0;
+  }
+  __device__ __forceinline__ bool next() {
+    if (at >= end) return false;
+    while ((int64_t)tiles[u + 1] * Hkv <= at) ++u;
+    unit_tiles = tiles[u + 1] - tiles[u];
+    const int64_t in = at - (int64_t)tiles[u] * Hkv;
+    head = (int)(in / unit_tiles);
+    first = (int)(in % unit_tiles);
+    count = (int)min((int64_t)(unit_tiles - first), end - at);
+    at += count;
+    return true;
+  }
+};
+
+// Few rows (a unit of 16 pairs), bound by the bytes of the keys and values: 16 rows of tensor work per key are far below
+// what mma.sync sustains, so the design is about keeping TMA loads in flight.  One producer warp streams 64-key tiles of K
+// and V (128-byte swizzled boxes, one per page and 64 columns) through a ring; each of four consumer warps takes 16 keys of
+// every tile and keeps its own running maximum, sum and output in registers, so no warp waits for another inside a piece.
+// The four are joined at the end of a piece.
+template <int D>
+__global__ void __launch_bounds__(160, Cfg<D>::kCtasPerSm)
+attn_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const AttnParams p) {
+  using C = Cfg<D>;
+  using namespace tc;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const uint32_t base = smem_u32(smem);
+  float* exch = reinterpret_cast<float*>(smem + C::kStages * C::kStageBytes);
+  float* ml = exch + C::kExchange / 4;                                   // [4][kUnitRows][2]
+  const uint32_t bars = base + C::kStages * C::kStageBytes + C::kExchange + 4 * kUnitRows * 2 * 4;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + (bars - base) + 16 * C::kStages);
+  auto full = [&](int s) { return bars + 16u * s; };
+  auto empty = [&](int s) { return bars + 16u * s + 8u; };
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(full(s), 1);
+      mbar_init(empty(s), 4);
+    }
+    *abort_flag = 0;
+    mbar_fence_init();
+  }
+  __syncthreads();
+  const WorkLayout lay(p.B, p.NG, p.max_units);
+  Walk walk(p.work, lay, p.Hkv, blockIdx.x, p.ctas);
+  int it = 0;
+
+  if (warp == 4) {
+    // ---------------------------------------------------------------------------------------------------- producer
+    const int box = min(p.ps, kTile), subs = kTile / box;
+    const int loads = 2 * (D / 64) * subs;       // at most 2 * 4 * 4 = 32: one lane each
+    const int kv = lane / ((D / 64) * subs), col = (lane / subs) % (D / 64), sub = lane % subs;
+    const CUtensorMap* map = kv ? &tmap_v : &tmap_k;
+    bool ok = true;
+    while (ok && walk.next()) {
+      const Unit u = walk.units[walk.u];
+      const int* row = p.table + (int64_t)u.slot * p.W;
+      const int t0 = u.key_lo / kTile + walk.first;
+      auto entry = [&](int t) {                  // page of this lane's box of tile t, -1 when no key of it is needed
+        const int64_t key = (int64_t)t * kTile + sub * box;
+        return lane < loads && key < u.key_hi ? row[key / p.ps] : INT_MIN;
+      };
+      int page = entry(t0);
+      for (int i = 0; i < walk.count; ++i, ++it) {
+        const int st = it % C::kStages;
+        const int t = t0 + i;
+        const int after = i + 1 < walk.count ? entry(t + 1) : INT_MIN;
+        if (!mbar_wait(empty(st), ((it / C::kStages) & 1) ^ 1, abort_flag)) { ok = false; break; }
+        const int need = __popc(__ballot_sync(0xffffffffu, page != INT_MIN));
+        if (lane == 0) mbar_expect_tx(full(st), need * box * 128);
+        __syncwarp();
+        if (page != INT_MIN) {
+          if (page < 0 || page >= p.num_pages) {  // out of range: the load fills zeros
+            atomicOr(p.status, kStatusPagePlanInvalid);
+            page = p.num_pages;
+          }
+          const int key = t * kTile + sub * box;
+          tma_load_4d(base + st * C::kStageBytes + kv * C::kHalfBytes + col * (kTile * 128) + sub * box * 128, map, full(st),
+                      col * 64, key % p.ps, walk.head, page);
+        }
+        page = after;
+      }
+    }
+  } else {
+    // ---------------------------------------------------------------------------------------------------- consumers
+    const int quad = lane & 3, r_lo = lane >> 2;                         // this thread's rows: r_lo and r_lo + 8
+    bool ok = true;
+    while (ok && walk.next()) {
+      const Unit u = walk.units[walk.u];
+      // rows: queries as A fragments, visible key range
+      uint32_t qf[D / 16][4];
+      int lo[2], hi[2];
+      int lo_min = INT_MAX, lo_max = 0, hi_min = INT_MAX, hi_max = -1;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int pr = u.pair0 + r_lo + 8 * j;
+        const bool live = pr < u.pairs;
+        const int i = live ? pr / p.G : 0;
+        const __nv_bfloat16* qr = p.q + (int64_t)(u.row0 + i) * p.q_row + (int64_t)(walk.head * p.G + (live ? pr % p.G : 0)) * p.q_head + quad * 2;
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          qf[k][j] = live ? *reinterpret_cast<const uint32_t*>(qr + k * 16) : 0u;
+          qf[k][2 + j] = live ? *reinterpret_cast<const uint32_t*>(qr + k * 16 + 8) : 0u;
+        }
+        lo[j] = u.key_lo;
+        hi[j] = u.key_hi - 1;
+        if (live) {
+          if (u.base >= 0) {
+            hi[j] = min(hi[j], u.base + i);
+            if (p.window > 0) lo[j] = max(lo[j], u.base + i - p.window + 1);
+          } else if (p.window > 0) {
+            const int b = find_segment(p.row_start, p.B, u.row0 + i);
+            lo[j] = max(lo[j], p.cached[b] + u.row0 + i - p.row_start[b] - p.window + 1);
+          }
+          lo_min = min(lo_min, lo[j]);
+          lo_max = max(lo_max, lo[j]);
+          hi_min = min(hi_min, hi[j]);
+          hi_max = max(hi_max, hi[j]);
+        }
+      }
+      lo_min = __reduce_min_sync(0xffffffffu, lo_min);
+      lo_max = __reduce_max_sync(0xffffffffu, lo_max);
+      hi_min = __reduce_min_sync(0xffffffffu, hi_min);
+      hi_max = __reduce_max_sync(0xffffffffu, hi_max);
+      float o[D / 8][4];
+#pragma unroll
+      for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
+      float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+
+      const int t0 = u.key_lo / kTile + walk.first;
+      for (int i = 0; i < walk.count; ++i, ++it) {
+        const int st = it % C::kStages;
+        if (!mbar_wait(full(st), (it / C::kStages) & 1, abort_flag)) { ok = false; break; }
+        const uint32_t ks = base + st * C::kStageBytes, vs = ks + C::kHalfBytes;
+        const int k0 = (t0 + i) * kTile + warp * 16;                     // this warp's first key
+        const int kr = warp * 16;
+        if (k0 <= hi_max && k0 + 15 >= lo_min) {
+          // S = Q K^T
+          float s[2][4];
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
+          {
+            const int key = kr + ((lane >> 4) << 3) + (lane & 7);
+            const uint32_t rowa = ks + key * 128;
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k) {
+              const int chunk = (k & 3) * 2 + ((lane >> 3) & 1);
+              uint32_t b[4];
+              ldmatrix4(rowa + (k >> 2) * (kTile * 128) + ((chunk ^ (key & 7)) << 4), b);
+              mma16816(s[0], qf[k], b[0], b[1]);
+              mma16816(s[1], qf[k], b[2], b[3]);
+            }
+          }
+          const bool edge = k0 + 15 > hi_min || k0 < lo_max;
+          if (edge) {
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int key = k0 + n * 8 + quad * 2 + (e & 1);
+                if (key < lo[e >> 1] || key > hi[e >> 1]) s[n][e] = -INFINITY;
+              }
+            // values outside every row's range may be anything, and a zero weight does not silence an infinity
+            if (k0 + 15 > hi_max || k0 < lo_min) {
+              for (int c = lane; c < 16 * (D / 8); c += 32) {
+                const int key = c / (D / 8), ch = c % (D / 8);
+                if (k0 + key > hi_max || k0 + key < lo_min)
+                  asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(vs + (ch >> 3) * (kTile * 128) + (kr + key) * 128 +
+                               (((ch & 7) ^ ((kr + key) & 7)) << 4)), "r"(0) : "memory");
+              }
+              fence_proxy_async_smem();
+              __syncwarp();
+            }
+          }
+          // running maximum: raised only when it grew by more than 2^8, P = exp2(S scale - m) stays in bf16's range
+          float mt[2];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            mt[j] = fmaxf(fmaxf(s[0][2 * j], s[0][2 * j + 1]), fmaxf(s[1][2 * j], s[1][2 * j + 1]));
+            mt[j] = fmaxf(mt[j], __shfl_xor_sync(0xffffffffu, mt[j], 1));
+            mt[j] = fmaxf(mt[j], __shfl_xor_sync(0xffffffffu, mt[j], 2)) * p.scale_log2;
+          }
+          if (__any_sync(0xffffffffu, mt[0] > m[0] + 8.f || mt[1] > m[1] + 8.f)) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const float mn = fmaxf(m[j], mt[j]);
+              const float a = m[j] == -INFINITY ? 0.f : exp2f(m[j] - mn);
+              m[j] = mn;
+              l[j] *= a;
+#pragma unroll
+              for (int n = 0; n < D / 8; ++n) {
+                o[n][2 * j] *= a;
+                o[n][2 * j + 1] *= a;
+              }
+            }
+          }
+          uint32_t pf[4];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float neg = m[j] == -INFINITY ? 0.f : -m[j];
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+              const float a = exp2f(fmaf(s[n][2 * j], p.scale_log2, neg)), b = exp2f(fmaf(s[n][2 * j + 1], p.scale_log2, neg));
+              l[j] += a + b;
+              pf[2 * n + j] = pack2bf(a, b);
+            }
+          }
+          // O += P V
+          {
+            const int key = kr + (((lane >> 3) & 1) << 3) + (lane & 7);
+            const uint32_t rowa = vs + key * 128;
+#pragma unroll
+            for (int n = 0; n < D / 16; ++n) {
+              const int chunk = (n & 3) * 2 + (lane >> 4);
+              uint32_t b[4];
+              ldmatrix4_t(rowa + (n >> 2) * (kTile * 128) + ((chunk ^ (key & 7)) << 4), b);
+              mma16816(o[2 * n], pf, b[0], b[1]);
+              mma16816(o[2 * n + 1], pf, b[2], b[3]);
+            }
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(empty(st));
+      }
+      // ---- join the four warps
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        l[j] += __shfl_xor_sync(0xffffffffu, l[j], 1);
+        l[j] += __shfl_xor_sync(0xffffffffu, l[j], 2);
+        if (quad == 0) {
+          ml[(warp * kUnitRows + r_lo + 8 * j) * 2] = m[j];
+          ml[(warp * kUnitRows + r_lo + 8 * j) * 2 + 1] = l[j];
+        }
+      }
+      if (consumer_any(!ok)) break;              // a wait ran out: all four leave together
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float mm = -INFINITY;
+        for (int w = 0; w < 4; ++w) mm = fmaxf(mm, ml[(w * kUnitRows + r_lo + 8 * j) * 2]);
+        const float f = m[j] == -INFINITY ? 0.f : exp2f(m[j] - mm);
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n) {
+          o[n][2 * j] *= f;
+          o[n][2 * j + 1] *= f;
+        }
+      }
+      // an fp32 tile in shared memory: column blocks of eight are spread over the banks by the row
+      auto slot = [&](int which, int row, int c) { return exch + which * (kUnitRows * D) + row * D + (c ^ ((row & 7) << 3)); };
+      auto put = [&](int which) {
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            *reinterpret_cast<float2*>(slot(which, r_lo + 8 * j, n * 8 + quad * 2)) = make_float2(o[n][2 * j], o[n][2 * j + 1]);
+      };
+      auto add = [&](int which) {
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float2 v = *reinterpret_cast<const float2*>(slot(which, r_lo + 8 * j, n * 8 + quad * 2));
+            o[n][2 * j] += v.x;
+            o[n][2 * j + 1] += v.y;
+          }
+      };
+      if (warp & 1) put(warp >> 1);
+      consumer_sync();
+      if (!(warp & 1)) add(warp >> 1);
+      if (warp == 2) put(1);
+      consumer_sync();
+      if (warp == 0) {
+        add(1);
+        put(0);
+      }
+      consumer_sync();
+      const bool whole = walk.count == walk.unit_tiles;
+      const int which = walk.first > 0 ? 0 : 1;
+      const int64_t cta = blockIdx.x;
+      for (int c = threadIdx.x; c < kUnitRows * (D / 4); c += 128) {
+        const int row = c / (D / 4), d = (c % (D / 4)) * 4;
+        const int pr = u.pair0 + row;
+        if (pr >= u.pairs) continue;
+        const float4 v = *reinterpret_cast<const float4*>(slot(0, row, d));
+        float mm = -INFINITY, ll = 0.f;
+        for (int w = 0; w < 4; ++w) mm = fmaxf(mm, ml[(w * kUnitRows + row) * 2]);
+        for (int w = 0; w < 4; ++w) {
+          const float mw = ml[(w * kUnitRows + row) * 2];
+          ll += mw == -INFINITY ? 0.f : exp2f(mw - mm) * ml[(w * kUnitRows + row) * 2 + 1];
+        }
+        const int64_t rh = (int64_t)(u.row0 + pr / p.G) * p.Hq + walk.head * p.G + pr % p.G;
+        if (whole && u.direct) {
+          float den = ll;
+          float f = 1.f;
+          if (p.sinks != nullptr) {
+            const float sk = p.sinks[rh % p.Hq] * 1.4426950408889634f, top = fmaxf(sk, mm);
+            f = mm == -INFINITY ? 0.f : exp2f(mm - top);
+            den = ll * f + exp2f(sk - top);
+          }
+          f = den > 0.f ? f / den : 0.f;
+          *reinterpret_cast<uint2*>(p.out + rh * D + d) = make_uint2(pack2bf(v.x * f, v.y * f), pack2bf(v.z * f, v.w * f));
+        } else if (whole) {
+          const int64_t at = (int64_t)(u.base < 0) * p.R * p.Hq + rh;
+          *reinterpret_cast<float4*>(p.row_o + at * D + d) = v;
+          if (d == 0) *reinterpret_cast<float2*>(p.row_ml + at * 2) = make_float2(mm, ll);
+        } else {
+          const int64_t at = (cta * 2 + which) * kUnitRows + row;
+          *reinterpret_cast<float4*>(p.part_o + at * D + d) = v;
+          if (d == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(mm, ll);
+        }
+      }
+      consumer_sync();
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x == 0 && *abort_flag) atomicOr(p.status, kStatusWaitTimedOut);
+}
+
+// One warp per (row, query head): joins the pieces of its units; rows that were finished by one piece are left alone.
+template <int D>
+__global__ void __launch_bounds__(256) combine_kernel(const AttnParams p) {
+  constexpr int N = D / 32;
+  const int lane = threadIdx.x & 31;
+  const int64_t rh = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (rh >= (int64_t)p.R * p.Hq) return;
+  const int r = (int)(rh / p.Hq), h = (int)(rh % p.Hq);
+  __nv_bfloat16* out = p.out + rh * D + lane * N;
+  auto store = [&](const float (&o)[N], float f) {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) *reinterpret_cast<uint32_t*>(out + i) = pack2bf(o[i] * f, o[i + 1] * f);
+  };
+  float o[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) o[i] = 0.f;
   if (r >= p.row_start[p.B]) {
-    if (p.zero_tail)
-      for (int d = threadIdx.x; d < p.D; d += 128) out[d] = __float2bfloat16_rn(0.f);
+    if (p.zero_tail) store(o, 0.f);
     return;
   }
+  const WorkLayout lay(p.B, p.NG, p.max_units);
   const int b = find_segment(p.row_start, p.B, r);
-  const int slot = p.slots[b];
-  const int pos = p.cached[b] + r - p.row_start[b];
-  const int kv = h / (p.Hq / p.Hkv);
-  float q[8], o[8];
-  for (int i = 0; i < 8; ++i) {
-    o[i] = 0.f;
-    q[i] = i < per ? __bfloat162float(p.q[r * p.q_row + h * p.q_head + lane * per + i]) : 0.f;
-  }
+  const int g = p.work[lay.seq_group + b];
+  const int* tiles = p.work + lay.tiles;
+  const Unit* units = reinterpret_cast<const Unit*>(p.work + lay.units);
+  const int n_units = p.work[0];
+  const int64_t per = stretch(p.work, p.Hkv, p.ctas);
+  const int kvh = h / p.G;
   float m = -INFINITY, l = 0.f;
-  const int64_t last = min((int64_t)pos, (int64_t)p.W * p.ps - 1);
-  for (int64_t j = (p.window > 0 ? max(0, pos - p.window + 1) : 0) + warp; j <= last; j += 4) {
-    const int page = p.table[(int64_t)slot * p.W + j / p.ps];
-    if (page < 0 || page >= p.num_pages) {
-      atomicOr(p.status, kStatusPagePlanInvalid);
-      continue;
-    }
-    const __nv_bfloat16* k = p.kp + page * p.kp_page + kv * p.kp_head + (j % p.ps) * p.kp_slot + lane * per;
-    const __nv_bfloat16* v = p.vp + page * p.vp_page + kv * p.vp_head + (j % p.ps) * p.vp_slot + lane * per;
-    float s = 0.f;
-    for (int i = 0; i < per; ++i) s += q[i] * __bfloat162float(k[i]);
-    s = warp_sum(s) * p.scale;
-    const float mn = fmaxf(m, s);
-    const float a = m == -INFINITY ? 0.f : expf(m - mn), w = mn == -INFINITY ? 0.f : expf(s - mn);
+  if (p.sinks != nullptr) {
+    m = p.sinks[h] * 1.4426950408889634f;
+    l = 1.f;
+  }
+  auto join = [&](const float* po, const float* pml) {
+    const float pm = pml[0], pl = pml[1];
+    if (pm == -INFINITY) return;
+    const float mn = fmaxf(m, pm);
+    const float a = m == -INFINITY ? 0.f : exp2f(m - mn), w = exp2f(pm - mn);
     m = mn;
-    l = l * a + w;
-    for (int i = 0; i < per; ++i) o[i] = o[i] * a + w * __bfloat162float(v[i]);
+    l = l * a + pl * w;
+#pragma unroll
+    for (int i = 0; i < N; ++i) o[i] = o[i] * a + po[lane * N + i] * w;
+  };
+  // the prefix comes first, then the sequence's own keys: a fixed order
+  for (int k = g >= 0 ? 0 : 1; k < 2; ++k) {
+    const int s = k == 0 ? p.B + g : b;
+    const int u0 = p.work[lay.src_unit + s];
+    if (u0 < 0) continue;
+    const int row0 = units[min(u0, n_units - 1)].row0;
+    const int pr = (r - row0) * p.G + h % p.G;
+    const int u = u0 + pr / kUnitRows;
+    if (u >= n_units) continue;
+    const int n = tiles[u + 1] - tiles[u];
+    if (n == 0) continue;
+    const int64_t t0 = (int64_t)tiles[u] * p.Hkv + (int64_t)kvh * n, t1 = t0 + n;
+    const int c0 = (int)(t0 / per), c1 = (int)((t1 - 1) / per);
+    if (c0 == c1) {
+      if (k == 1 && g < 0) return;               // finished by its piece
+      const int64_t at = (int64_t)(k == 0) * p.R * p.Hq + rh;
+      join(p.row_o + at * D, p.row_ml + at * 2);
+    } else {
+      for (int c = c0; c <= c1; ++c) {
+        const int64_t at = ((int64_t)c * 2 + (c == c0 ? 1 : 0)) * kUnitRows + pr % kUnitRows;
+        join(p.part_o + at * D, p.part_ml + at * 2);
+      }
+    }
   }
-  if (lane == 0) { sm_m[warp] = m; sm_l[warp] = l; }
-  for (int i = 0; i < per; ++i) sm_o[warp][lane * per + i] = o[i];
-  __syncthreads();
-  float mm = p.sinks != nullptr ? p.sinks[h] : -INFINITY;
-  for (int w = 0; w < 4; ++w) mm = fmaxf(mm, sm_m[w]);
-  float den = p.sinks != nullptr && mm != -INFINITY ? expf(p.sinks[h] - mm) : 0.f;
-  float f[4];
-  for (int w = 0; w < 4; ++w) {
-    f[w] = sm_m[w] == -INFINITY ? 0.f : expf(sm_m[w] - mm);
-    den += f[w] * sm_l[w];
-  }
-  for (int d = threadIdx.x; d < p.D; d += 128) {
-    float s = 0.f;
-    for (int w = 0; w < 4; ++w) s += f[w] * sm_o[w][d];
-    out[d] = __float2bfloat16_rn(den > 0.f ? s / den : 0.f);
-  }
+  store(o, l > 0.f ? 1.f / l : 0.f);
 }
 
 }  // namespace paged
@@ -347,32 +907,124 @@ void paged_write(const at::Tensor& k, const at::Tensor& v, at::Tensor k_pages, a
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
-void paged_attention_simple(const at::Tensor& q, const at::Tensor& k_pages, const at::Tensor& v_pages, const at::Tensor& table,
-                            const at::Tensor& slots, const at::Tensor& cached, const at::Tensor& row_start, double scale, int64_t window,
-                            const c10::optional<at::Tensor>& sinks, at::Tensor out, bool zero_tail) {
+// Units of a step at most: one per source and one more per kUnitRows pairs; every row belongs to at most two sources.
+static int64_t max_units(int64_t B, int64_t NG, int64_t R, int64_t G) {
+  const int64_t n = B + NG + (NG > 0 ? 2 : 1) * R * G / paged::kUnitRows + 1;
+  TORCH_CHECK(n < (1 << 28), "paged attention: too many rows");
+  return n;
+}
+
+// The attention work list of a step for one window (see "Work" above).
+at::Tensor paged_work(const at::Tensor& cached, const at::Tensor& row_start, const at::Tensor& slots, const c10::optional<at::Tensor>& group_start,
+                      const c10::optional<at::Tensor>& group_prefix, int64_t table_cols, int64_t page_size,
+                      int64_t total_rows, int64_t hq, int64_t hkv, int64_t window) {
+  TORCH_CHECK(cached.is_cuda(), "paged_work: CUDA tensors expected");
+  const auto dev = cached.device();
+  c10::cuda::CUDAGuard guard(dev);
+  const int64_t B = cached.numel();
+  TORCH_CHECK(hkv > 0 && hq > 0 && hq % hkv == 0, "paged_work: ", hq, " query heads on ", hkv, " key heads");
+  TORCH_CHECK(group_start.has_value() == group_prefix.has_value(), "paged_work: group_start and group_prefix come together");
+  TORCH_CHECK(window >= 0 && window <= INT32_MAX, "paged_work: bad window");
+  paged::WorkParams p{};
+  p.cached = int_vector(cached, B, dev, "cached");
+  p.row_start = int_vector(row_start, B + 1, dev, "row_start");
+  p.slots = int_vector(slots, B, dev, "slots");
+  int64_t NG = 0;
+  if (group_start.has_value()) {
+    NG = group_prefix->numel();
+    TORCH_CHECK(NG <= paged::kMaxSeqs, "page_plan: at most ", paged::kMaxSeqs, " groups");
+    p.group_prefix = int_vector(*group_prefix, NG, dev, "group_prefix");
+    p.group_start = int_vector(*group_start, NG + 1, dev, "group_start");
+  }
+  p.B = (int)B; p.NG = (int)NG; p.W = (int)table_cols; p.ps = (int)page_size;
+  p.G = (int)(hq / hkv); p.window = (int)window;
+  p.max_units = (int)max_units(B, NG, total_rows, p.G);
+  auto work = at::empty({paged::WorkLayout(B, NG, p.max_units).size}, cached.options());
+  p.work = work.data_ptr<int>();
+  p.status = status_word_ptr();
+  const int smem = (int)(sizeof(int) * (B + NG + 1 + 2 * NG));
+  if (smem > 48 * 1024) C10_CUDA_CHECK(cudaFuncSetAttribute(paged::work_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  paged::work_kernel<<<1, 1024, smem, at::cuda::getCurrentCUDAStream()>>>(p);
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return work;
+}
+
+// Pages as 128-byte wide, swizzled boxes of up to 64 slots of one page and head.
+static CUtensorMap page_map(const at::Tensor& t) {
+  CUtensorMap map;
+  const uint64_t e = 2;
+  const cuuint64_t dims[4] = {(cuuint64_t)t.size(3), (cuuint64_t)t.size(2), (cuuint64_t)t.size(1), (cuuint64_t)t.size(0)};
+  const cuuint64_t strides[3] = {(cuuint64_t)t.stride(2) * e, (cuuint64_t)t.stride(1) * e, (cuuint64_t)t.stride(0) * e};
+  const cuuint32_t box[4] = {64, (cuuint32_t)std::min<int64_t>(t.size(2), paged::kTile), 1, 1};
+  const cuuint32_t elem[4] = {1, 1, 1, 1};
+  const CUresult r = cuTensorMapEncodeTiled(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, t.data_ptr(), dims, strides, box, elem,
+                                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  TORCH_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled (pages) failed with code ", (int)r);
+  return map;
+}
+
+void paged_attention(const at::Tensor& q, const at::Tensor& k_pages, const at::Tensor& v_pages, const at::Tensor& table,
+                     const at::Tensor& cached, const at::Tensor& row_start, const at::Tensor& work, int64_t groups, double scale,
+                     int64_t window, const c10::optional<at::Tensor>& sinks, at::Tensor out, bool zero_tail) {
   check_pages(k_pages, v_pages, "paged_attention");
   const auto dev = k_pages.device();
+  const int64_t R = q.size(0), D = k_pages.size(3), ps = k_pages.size(2);
   TORCH_CHECK(q.device() == dev && q.dim() == 3 && q.scalar_type() == at::kBFloat16 && k_pages.scalar_type() == at::kBFloat16 &&
-                  q.size(2) == k_pages.size(3) && q.stride(2) == 1 && q.size(1) % k_pages.size(1) == 0,
+                  q.size(2) == D && k_pages.size(1) > 0 && q.size(1) > 0 && q.size(1) % k_pages.size(1) == 0,
               "paged_attention: q must be bf16 [R, Hq, D] beside bf16 pages");
-  TORCH_CHECK(q.size(2) % 32 == 0 && q.size(2) <= 256, "paged_attention: unsupported head dimension ", q.size(2));
-  TORCH_CHECK(out.is_contiguous() && out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type() && out.device() == dev);
+  TORCH_CHECK(q.stride(2) == 1 && q.stride(1) % 2 == 0 && q.stride(0) % 2 == 0 && reinterpret_cast<uintptr_t>(q.data_ptr()) % 4 == 0,
+              "paged_attention: query vectors must be contiguous and 4-byte aligned");
+  TORCH_CHECK(D == 64 || D == 128 || D == 256, "paged_attention: unsupported head dimension ", D);
+  TORCH_CHECK(ps == 16 || ps == 32 || (ps > 0 && ps % 64 == 0), "paged_attention: unsupported page size ", ps);
+  TORCH_CHECK(out.is_contiguous() && out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type() && out.device() == dev &&
+                  reinterpret_cast<uintptr_t>(out.data_ptr()) % 8 == 0,
+              "paged_attention: out must be a contiguous bf16 tensor of q's shape");
+  if (sinks.has_value())
+    TORCH_CHECK(sinks->device() == dev && sinks->scalar_type() == at::kFloat && sinks->is_contiguous() && sinks->numel() == q.size(1),
+                "paged_attention: sinks must be a contiguous fp32 vector [Hq]");
+  TORCH_CHECK(table.device() == dev && table.scalar_type() == at::kInt && table.dim() == 2 && table.is_contiguous());
   c10::cuda::CUDAGuard guard(dev);
-  if (q.numel() == 0) return;
-  paged::SimpleParams p{};
+  if (R == 0) return;
+  const int64_t B = cached.numel();
+  paged::AttnParams p{};
   p.q = (const __nv_bfloat16*)q.data_ptr(); p.q_row = q.stride(0); p.q_head = q.stride(1);
-  p.kp = (const __nv_bfloat16*)k_pages.data_ptr(); p.vp = (const __nv_bfloat16*)v_pages.data_ptr();
-  p.kp_page = k_pages.stride(0); p.kp_head = k_pages.stride(1); p.kp_slot = k_pages.stride(2);
-  p.vp_page = v_pages.stride(0); p.vp_head = v_pages.stride(1); p.vp_slot = v_pages.stride(2);
-  p.table = table.data_ptr<int>(); p.slots = slots.data_ptr<int>(); p.cached = cached.data_ptr<int>(); p.row_start = row_start.data_ptr<int>();
-  p.sinks = sinks.has_value() ? sinks->data_ptr<float>() : nullptr;
   p.out = (__nv_bfloat16*)out.data_ptr();
-  p.B = (int)slots.numel(); p.S = (int)table.size(0); p.W = (int)table.size(1); p.R = (int)q.size(0);
-  p.Hq = (int)q.size(1); p.Hkv = (int)k_pages.size(1); p.D = (int)q.size(2); p.ps = (int)k_pages.size(2);
-  p.num_pages = (int)k_pages.size(0); p.window = (int)window; p.scale = (float)scale; p.zero_tail = zero_tail;
+  p.sinks = sinks.has_value() ? sinks->data_ptr<float>() : nullptr;
+  p.table = table.data_ptr<int>();
+  p.cached = int_vector(cached, B, dev, "cached");
+  p.row_start = int_vector(row_start, B + 1, dev, "row_start");
+  p.B = (int)B; p.NG = (int)groups; p.S = (int)table.size(0); p.W = (int)table.size(1); p.R = (int)R;
+  p.Hq = (int)q.size(1); p.Hkv = (int)k_pages.size(1); p.G = p.Hq / p.Hkv; p.ps = (int)ps; p.num_pages = (int)k_pages.size(0);
+  p.window = (int)window; p.scale_log2 = (float)(scale * 1.4426950408889634); p.zero_tail = zero_tail;
+  p.max_units = (int)max_units(B, groups, R, p.G);
+  p.ctas = num_sms() * (D == 256 ? paged::Cfg<256>::kCtasPerSm : paged::Cfg<128>::kCtasPerSm);
+  p.work = int_vector(work, paged::WorkLayout(B, groups, p.max_units).size, dev, "work (made for other heads, rows or groups?)");
   p.status = status_word_ptr();
-  paged::simple_kernel<<<p.R * p.Hq, 128, 0, at::cuda::getCurrentCUDAStream()>>>(p);
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  const auto f32 = q.options().dtype(at::kFloat);
+  auto part = at::empty({(int64_t)p.ctas * 2 * paged::kUnitRows, D + 2}, f32);
+  p.part_o = part.data_ptr<float>();
+  p.part_ml = p.part_o + (int64_t)p.ctas * 2 * paged::kUnitRows * D;
+  at::Tensor rows;
+  if (groups > 0) {
+    rows = at::empty({2 * R * p.Hq, D + 2}, f32);
+    p.row_o = rows.data_ptr<float>();
+    p.row_ml = p.row_o + 2 * R * p.Hq * D;
+  }
+  const CUtensorMap mk = page_map(k_pages), mv = page_map(v_pages);
+  auto stream = at::cuda::getCurrentCUDAStream();
+  auto launch = [&](auto dim) {
+    constexpr int kD = decltype(dim)::value;
+    auto kernel = paged::attn_rows_kernel<kD>;
+    C10_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, paged::Cfg<kD>::kSmem));
+    kernel<<<p.ctas, 160, paged::Cfg<kD>::kSmem, stream>>>(mk, mv, p);
+    C10_CUDA_KERNEL_LAUNCH_CHECK();
+    paged::combine_kernel<kD><<<(unsigned)((R * p.Hq + 7) / 8), 256, 0, stream>>>(p);
+    C10_CUDA_KERNEL_LAUNCH_CHECK();
+  };
+  if (D == 64) launch(std::integral_constant<int, 64>{});
+  else if (D == 128) launch(std::integral_constant<int, 128>{});
+  else launch(std::integral_constant<int, 256>{});
 }
 
 }  // namespace tb200

@@ -16,7 +16,7 @@ raise instead.
 
 from __future__ import annotations
 
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 
 import torch
 
@@ -42,6 +42,9 @@ class PagePlan:
     page_size: int
     num_pages: int
     total_rows: int
+    heads: tuple[int, int] | None = None                                 # (query, key heads) of the attention work lists
+    groups: int = 0
+    work: dict[int, torch.Tensor] = field(default_factory=dict)          # by window
 
 
 def supported(q: torch.Tensor, k_pages: torch.Tensor) -> bool:
@@ -57,7 +60,12 @@ def page_plan(cached: torch.Tensor, new: torch.Tensor, block_table: torch.Tensor
 
     ``pages`` are the ids handed out, in the order of the sequences: sequence ``b`` takes as many as it needs for
     ``cached[b] + new[b]`` tokens beyond the ``mapped[b]`` columns of its table row that are filled already (default:
-    those that hold its cached tokens).  ``total_rows`` is the length of the flat stream, at least ``sum(new)``."""
+    those that hold its cached tokens).  ``total_rows`` is the length of the flat stream, at least ``sum(new)``.
+
+    With ``n_heads`` and ``n_kv_heads`` the plan also holds what ``attention`` needs for layers of these heads, for each of
+    ``windows`` (0 = no window).  ``group_start [groups + 1]`` and ``group_prefix [groups]`` declare that the sequences
+    ``group_start[g] .. group_start[g + 1]`` share their first ``group_prefix[g]`` tokens: their table rows begin with the
+    same pages.  ``max_rows``: an upper bound of the new rows of one sequence or group, if the caller knows one."""
     if page_size not in PAGE_SIZES:
         raise ValueError(f"page_plan: page_size must be one of {PAGE_SIZES}, got {page_size}")
     args = (cached, new, block_table, slots, pages, mapped, int(page_size), int(total_rows), int(num_pages))
@@ -66,7 +74,17 @@ def page_plan(cached: torch.Tensor, new: torch.Tensor, block_table: torch.Tensor
         row_start, positions, slot_map = ext.require().page_plan(*args)
     else:
         row_start, positions, slot_map = ref.page_plan(*args)
-    return PagePlan(row_start, positions, slot_map, cached, slots, block_table, int(page_size), int(num_pages), int(total_rows))
+    plan = PagePlan(row_start, positions, slot_map, cached, slots, block_table, int(page_size), int(num_pages), int(total_rows))
+    if n_heads is not None:
+        if not n_kv_heads or n_heads % n_kv_heads:
+            raise ValueError(f"page_plan: {n_heads} query heads on {n_kv_heads} key heads")
+        plan.heads, plan.groups = (int(n_heads), int(n_kv_heads)), 0 if group_prefix is None else group_prefix.numel()
+        if block_table.is_cuda:
+            for w in dict.fromkeys(int(w or 0) for w in windows):
+                _count()
+                plan.work[w] = ext.require().paged_work(cached, row_start, slots, group_start, group_prefix, block_table.shape[1],
+                                                        int(page_size), int(total_rows), *plan.heads, w)
+    return plan
 
 
 def _vectors(t: torch.Tensor) -> torch.Tensor:
@@ -108,9 +126,12 @@ def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pla
         n = int(plan.row_start[-1])
         out[:n] = o[:n]
         return out
-    _count()
+    if plan.heads != (q.shape[1], k_pages.shape[1]) or int(window) not in plan.work:
+        raise ValueError(f"paged attention: {q.shape[1]} / {k_pages.shape[1]} heads with window {window}, the plan was made for "
+                         f"{plan.heads} and windows {tuple(plan.work)}")
+    _count(2)
     dst = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
-    ext.require().paged_attention_simple(_vectors(q), k_pages, v_pages, plan.block_table, plan.slots, plan.cached, plan.row_start,
-                                         float(scale), int(window), None if sinks is None else sinks.float().contiguous(), dst,
-                                         out is None)
+    ext.require().paged_attention(q if q.stride(2) == 1 and not (q.stride(0) | q.stride(1)) % 2 and q.data_ptr() % 4 == 0 else q.clone(
+        memory_format=torch.contiguous_format), k_pages, v_pages, plan.block_table, plan.cached, plan.row_start, plan.work[int(window)],
+        plan.groups, float(scale), int(window), None if sinks is None else sinks.float().contiguous(), dst, out is None)
     return dst
