@@ -172,3 +172,6 @@ class KernelConfig:
     gemm: Literal["cublas", "tcgen05"] = "tcgen05"
     attention: Literal["sdpa", "native"] = "native"
     elementwise: Literal["native", "torch"] = "native"
+    qk_norm_rope: Literal["separate", "fused"] = "separate"
+    """Attention layers with per-head query / key norms: ``fused`` runs both norms and the rotary embedding in one pass over
+    the projection output (one rounding instead of two, so results differ from ``separate`` by roundings)."""

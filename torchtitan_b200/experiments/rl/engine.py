@@ -5,9 +5,10 @@ waiting requests (up to ``max_num_seqs`` sequences and ``max_batched_tokens`` pr
 prompts and one row for each sequence already decoding into ONE flat token stream, and runs the decoder once over
 it: projections, feed-forward / expert layers and the output projection see all rows together (weights are read
 once per step for all sequences), the attention core runs per sequence against that sequence's key/value cache
-(``models.common.attention.BatchedKVCache``).  Only the last row of each sequence reaches the output projection.
-Sampling (temperature, top-k, top-p, per-request seed) happens per sequence; a sequence ends on EOS, a stop token,
-a stop sequence (``finish_reason = "stop"``), its token limit (``"length"``) or engine shutdown (``"abort"``).
+(``models.common.attention.BatchedKVCache``), or with ``kv_cache = "paged"`` in one launch over all sequences' pages
+(``PagedKVCache``), where requests with the same leading tokens share them.  Only the last row of each sequence
+reaches the output projection.  Sampling (temperature, top-k, top-p, per-request seed) happens per sequence; a
+sequence ends on EOS, a stop token, a stop sequence (``finish_reason = "stop"``), its token limit (``"length"``) or engine shutdown (``"abort"``).
 
 New weights are applied between two steps (``pull_model_state_dict``): sequences in flight keep their caches and
 continue under the new policy, and each completion reports the oldest and newest policy version its tokens were
@@ -24,7 +25,7 @@ import asyncio
 import threading
 import time
 from dataclasses import dataclass, field
-from typing import Any, Callable
+from typing import Any, Callable, Literal
 
 import torch
 
@@ -111,6 +112,13 @@ class GenerationEngine(Configurable):
         """Run engine steps in a worker thread so that the controller's event loop (and a trainer on another
         device or stream) keeps going.  Must be off when the engine shares its model object with the trainer."""
         sampling: SamplingConfig = field(default_factory=SamplingConfig)
+        kv_cache: Literal["contiguous", "paged"] = "contiguous"
+        """``paged``: keys and values live in pages of one pool per layer, one attention launch serves all sequences, and
+        requests whose prompts begin with the same pages of tokens (the samples of one group) compute and read them once."""
+        kv_cache_tokens: int = 65536
+        """Paged cache: tokens of the pool.  A request is admitted when its prompt and all tokens it may still generate fit."""
+        kv_page_size: int = 64
+        share_prefixes: bool = True
 
     def __init__(self, config: Config | None = None, *, model, eos_id: int | None = None,
                  weight_source: Callable[["GenerationEngine"], None] | None = None):
@@ -128,6 +136,14 @@ class GenerationEngine(Configurable):
         self._closed = False
         self.steps = 0
         self.tokens_generated = 0
+        self._paged = None
+        if self.config.kv_cache == "paged":
+            from torchtitan_b200.models.common.attention import PagedKVCache
+
+            c = self.config
+            self._paged = PagedKVCache.for_model(
+                model, tokens=c.kv_cache_tokens, max_seqs=c.max_num_seqs, max_length=min(self.max_context or c.kv_cache_tokens, c.kv_cache_tokens),
+                page_size=c.kv_page_size, device=next(model.parameters()).device, share_prefixes=c.share_prefixes)
 
     # -- public API ----------------------------------------------------------------------------------------------
     async def generate(self, prompt_token_ids: list[int], *, request_id: str, routing_session_id: str | None = None,
@@ -143,9 +159,12 @@ class GenerationEngine(Configurable):
             raise ValueError(f"{request_id}: the prompt has {len(prompt_token_ids)} tokens, the model's context is "
                              f"{self.max_context}")
         s = sampling_config or self.config.sampling
+        if self._paged is not None and len(prompt_token_ids) >= self._paged.max_length:
+            raise ValueError(f"{request_id}: the prompt has {len(prompt_token_ids)} tokens, the paged cache holds "
+                             f"{self._paged.max_length} (kv_cache_tokens)")
         loop = asyncio.get_running_loop()
         seq = _Seq(request_id=request_id, pending=list(prompt_token_ids), sampling=s, future=loop.create_future(),
-                   loop=loop, cache=KVCache(), t_arrive=time.perf_counter(),
+                   loop=loop, cache=None if self._paged is not None else KVCache(), t_arrive=time.perf_counter(),
                    rng=None if s.seed is None else torch.Generator().manual_seed(s.seed))
         with self._lock:
             self._waiting.append(seq)
@@ -207,6 +226,8 @@ class GenerationEngine(Configurable):
     def _fail_inflight(self, error: Exception) -> None:
         with self._lock:
             hit, self._running = self._running, []
+        if self._paged is not None:
+            self._paged.reset()
         for seq in hit:
             seq.cache = None
             if not seq.future.done():
@@ -219,6 +240,8 @@ class GenerationEngine(Configurable):
             try:
                 if self.weight_source is not None:
                     self.weight_source(self)
+                if self._paged is not None:
+                    self._paged.forget_prefixes()    # new requests compute their prompts under the new weights
                 self.policy_version = version
                 loop.call_soon_threadsafe(lambda f=fut: f.done() or f.set_result(None))
             except Exception as e:              # the caller of the pull sees the failure
@@ -234,11 +257,19 @@ class GenerationEngine(Configurable):
         with self._lock:
             budget = c.max_batched_tokens
             while self._waiting and len(self._running) < c.max_num_seqs:
-                n = len(self._waiting[0].pending)
+                first = self._waiting[0]
+                n = len(first.pending) - (self._paged.shared_tokens(first.pending) if self._paged is not None else 0)
                 if n > budget and budget < c.max_batched_tokens:
                     break                          # next step; a prompt longer than the whole budget goes alone
+                if self._paged is not None:
+                    if not self._paged.can_add(first.pending, first.sampling.max_tokens):
+                        break                      # until sequences in flight give their pages back
+                    first.cache, cached = self._paged.add(first.pending, first.sampling.max_tokens)
+                    first.pending, first.pos = first.pending[cached:], cached
                 budget -= n
                 self._running.append(self._waiting.pop(0))
+        if self._paged is not None:                # the members of a prefix group are neighbours in the token stream
+            self._running.sort(key=lambda s: self._paged.group_of(s.cache))
         seqs = self._running
         if not seqs:
             return 0
@@ -249,7 +280,11 @@ class GenerationEngine(Configurable):
         last = torch.tensor(rows, device=dev).cumsum(0) - 1
         was_training = self.model.training
         self.model.eval()
-        ctx = AttentionContext(kv_cache=BatchedKVCache([s.cache for s in seqs], rows))
+        if self._paged is not None:
+            self._paged.begin_step([s.cache for s in seqs], rows)
+            ctx = AttentionContext(kv_cache=self._paged)
+        else:
+            ctx = AttentionContext(kv_cache=BatchedKVCache([s.cache for s in seqs], rows))
         try:
             with frozen_router_counters(self.model):
                 if hasattr(self.model, "output_logits") and getattr(self.model, "tp", None) is None:
@@ -259,6 +294,9 @@ class GenerationEngine(Configurable):
         finally:
             self.model.train(was_training)
         logits = logits.float()
+        if self._paged is not None:
+            self._paged.end_step()
+            self._check_pages(dev)
         now = time.perf_counter()
         still = []
         for i, s in enumerate(seqs):
@@ -282,6 +320,15 @@ class GenerationEngine(Configurable):
         self.tokens_generated += len(seqs)
         return len(seqs)
 
+    def _check_pages(self, device) -> None:
+        """The kernels skip a page or slot that is out of range and flag it; the tokens of such a step are not used."""
+        if device.type == "cuda":
+            from torchtitan_b200.ops import ext
+
+            if int(ext.require().status(False)) & 16:
+                ext.require().status(True)
+                raise RuntimeError("paged cache: a page table entry was out of range")
+
     def _finish_reason(self, s: _Seq, tok: int) -> str | None:
         sc = s.sampling
         if (self.eos_id is not None and tok == self.eos_id) or tok in sc.stop_token_ids:
@@ -290,6 +337,8 @@ class GenerationEngine(Configurable):
             if stop and s.out_ids[-len(stop):] == stop:
                 return "stop"
         if self.max_context and s.pos + 1 >= self.max_context:      # the next row would be past the context
+            return "length"
+        if self._paged is not None and s.pos >= self._paged.max_length:
             return "length"
         return "length" if len(s.out_ids) >= sc.max_tokens else None
 
@@ -303,6 +352,8 @@ class GenerationEngine(Configurable):
                               m.Metric("generator/request_latency_s", m.Mean(now - s.t_arrive)),
                               m.Metric("generator/response_length", m.Mean(len(s.out_ids))),
                               m.Metric("generator/response_length", m.Max(len(s.out_ids)))])
+        if self._paged is not None and s.cache is not None:
+            self._paged.release(s.cache)
         s.cache = None
         try:
             s.loop.call_soon_threadsafe(lambda: s.future.done() or s.future.set_result(done))

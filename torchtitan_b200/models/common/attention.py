@@ -27,7 +27,8 @@ from torchtitan_b200.parallel import tp_ops
 from .layers import Linear, RMSNorm, RoPE, TPContext
 from .module import InitSpec, Module, set_init
 
-__all__ = ["GQAttention", "AttentionContext", "KVCache", "BatchedKVCache", "cached_attention", "build_attention_context"]
+__all__ = ["GQAttention", "AttentionContext", "KVCache", "BatchedKVCache", "PagedKVCache", "cached_attention",
+           "fused_qk_norm_rope", "build_attention_context"]
 
 
 @dataclass
@@ -38,7 +39,7 @@ class AttentionContext:
     max_doc_len: int | None = None
     kv_first: torch.Tensor | None = None  # [T_local] int32: index of the first token of each token's document
     rope_positions: torch.Tensor | None = None  # [3, T_local] multimodal rotary positions (overrides ``positions``)
-    kv_cache: "KVCache | BatchedKVCache | None" = None  # incremental decoding: keys / values of earlier tokens, per attention layer
+    kv_cache: "KVCache | BatchedKVCache | PagedKVCache | None" = None  # incremental decoding: keys / values of earlier tokens, per attention layer
 
 
 class KVCache:
@@ -89,11 +90,191 @@ class BatchedKVCache:
         self.caches, self.rows = caches, rows
 
 
+class PagedKVCache:
+    """Keys and values of many sequences in pages of one pool per attention layer (``ops.paged``).
+
+    Every sequence has a *slot* (a row of the block table on the device); which pages it owns is known on the host as
+    well, where pages are handed out and taken back.  ``add`` admits a sequence, ``begin_step`` plans one forward pass
+    over some rows of some sequences (one H2D copy of their lengths and new page ids, the tables are built on the device),
+    ``attend`` is what a layer calls, ``end_step`` advances the lengths, ``release`` ends a sequence.
+
+    Sequences admitted with the same leading tokens share the pages of the whole pages among them (all but the last token
+    at most): the later ones start behind them, and attention reads them once for all rows of the group.  Whole requests are
+    reserved at ``add`` (prompt and the tokens to come), so a sequence in flight never runs out of pages."""
+
+    def __init__(self, heads: tuple[int, int], windows: tuple[int, ...], *, tokens: int, max_seqs: int, max_length: int,
+                 page_size: int = 64, device, share_prefixes: bool = True):
+        from torchtitan_b200.ops.paged import PAGE_SIZES
+
+        if page_size not in PAGE_SIZES:
+            raise ValueError(f"page size {page_size} (have {PAGE_SIZES})")
+        if tokens <= 0 or max_seqs <= 0 or max_length <= 0:
+            raise ValueError("a paged cache needs tokens, sequences and a maximum length")
+        self.heads, self.windows, self.page_size, self.device = heads, windows, page_size, torch.device(device)
+        self.num_pages = -(-tokens // page_size)
+        self.max_length, self.share_prefixes = max_length, share_prefixes
+        cols = min(-(-max_length // page_size), self.num_pages)
+        self.block_table = torch.full((max_seqs, cols), -1, dtype=torch.int32, device=self.device)
+        self.pools: dict[int, tuple[torch.Tensor, torch.Tensor]] = {}
+        self.plan = None
+        self.reset()
+
+    @classmethod
+    def for_model(cls, model, **kw) -> "PagedKVCache":
+        """A cache for a decoder whose attention layers are all grouped-query layers with the same head counts."""
+        from .mla import MLAttention
+
+        layers = [m for m in model.modules() if isinstance(m, GQAttention)]
+        heads = {(m.n_heads, m.n_kv_heads) for m in layers}
+        if any(isinstance(m, MLAttention) for m in model.modules()) or len(heads) != 1:
+            raise ValueError("the paged cache covers decoders whose attention layers are grouped-query layers of one shape "
+                             f"(found {sorted(heads)}); use the contiguous cache")
+        recurrent = any(type(b.attention).__name__ == "GatedDeltaNet" for b in model.modules() if hasattr(b, "attention"))
+        kw["share_prefixes"] = kw.get("share_prefixes", True) and not recurrent     # a recurrent state is not in the pages
+        return cls(heads.pop(), tuple(sorted({int(m.window or 0) for m in layers})), **kw)
+
+    # -- sequences ---------------------------------------------------------
+    def reset(self) -> None:
+        self._free = list(range(self.num_pages - 1, -1, -1))
+        self._slots = list(range(self.block_table.shape[0] - 1, -1, -1))
+        self._refs = [0] * self.num_pages
+        self._pages: dict[int, list[int]] = {}       # slot -> pages, prefix first
+        self._length: dict[int, int] = {}            # slot -> tokens in the pages
+        self._mapped: dict[int, int] = {}            # slot -> columns of its table row that are filled
+        self._group: dict[int, tuple] = {}           # slot -> (group number, prefix tokens)
+        self._index: dict[tuple, tuple[int, int]] = {}   # leading tokens -> (group number, a live slot that holds them)
+        self._states: dict[int, KVCache] = {}
+        self._groups_made = 0
+        self._step: tuple[list[int], list[int]] | None = None
+
+    def _prefix_key(self, prompt) -> tuple:
+        return tuple(prompt[:(len(prompt) - 1) // self.page_size * self.page_size]) if self.share_prefixes else ()
+
+    def shared_tokens(self, prompt) -> int:
+        """Leading tokens of ``prompt`` that a sequence in flight has in its pages."""
+        key = self._prefix_key(prompt)
+        return len(key) if key in self._index else 0
+
+    def pages_needed(self, prompt, new_tokens: int) -> int:
+        """Pages that ``add`` would take from the pool."""
+        total = -(-min(len(prompt) + new_tokens, self.max_length) // self.page_size)
+        return total - self.shared_tokens(prompt) // self.page_size
+
+    def can_add(self, prompt, new_tokens: int) -> bool:
+        return bool(self._slots) and self.pages_needed(prompt, new_tokens) <= len(self._free)
+
+    def add(self, prompt, new_tokens: int) -> tuple[int, int]:
+        """Admit a sequence of ``prompt`` and up to ``new_tokens`` more; returns ``(slot, tokens already cached)``."""
+        if len(prompt) > self.max_length or not prompt:
+            raise ValueError(f"a prompt of {len(prompt)} tokens in a cache for up to {self.max_length}")
+        if not self.can_add(prompt, new_tokens):
+            raise RuntimeError(f"the paged cache is full: {len(self._free)} pages and {len(self._slots)} sequences left")
+        need = self.pages_needed(prompt, new_tokens)
+        key = self._prefix_key(prompt)
+        slot = self._slots.pop()
+        pages, cached = [], 0
+        if key in self._index:
+            group, other = self._index[key]
+            cached = len(key)
+            pages = self._pages[other][:cached // self.page_size]
+            self._group[slot] = (group, cached)
+        elif key:
+            self._groups_made += 1
+            self._index[key] = (self._groups_made, slot)
+            self._group[slot] = (self._groups_made, len(key))
+        pages = pages + [self._free.pop() for _ in range(need)]
+        for i in pages:
+            self._refs[i] += 1
+        self._pages[slot], self._length[slot], self._mapped[slot] = pages, cached, 0
+        self._states[slot] = KVCache()
+        return slot, cached
+
+    def release(self, slot: int) -> None:
+        for i in self._pages.pop(slot):
+            self._refs[i] -= 1
+            if self._refs[i] == 0:
+                self._free.append(i)
+        del self._length[slot], self._mapped[slot], self._states[slot]
+        group = self._group.pop(slot, None)
+        for key, (g, holder) in list(self._index.items()):
+            if holder == slot:                       # hand the entry to another member, if there is one
+                other = next((s for s, m in self._group.items() if m == group), None)
+                if other is None:
+                    del self._index[key]
+                else:
+                    self._index[key] = (g, other)
+        self._slots.append(slot)
+
+    def forget_prefixes(self) -> None:
+        """New sequences do not join those in flight any more (the weights changed)."""
+        self._index.clear()
+
+    def group_of(self, slot: int) -> int:
+        """Sort key that brings the members of a group together."""
+        return self._group.get(slot, (0, 0))[0]
+
+    # -- one forward pass --------------------------------------------------
+    def begin_step(self, slots: list[int], rows: list[int]) -> None:
+        """The flat token stream will hold ``rows[i]`` consecutive rows of ``slots[i]``; members of a group are neighbours."""
+        from torchtitan_b200.ops import paged
+
+        ps = self.page_size
+        cached, mapped, pages, start, prefix, last = [], [], [], [], [], None
+        for i, (s, n) in enumerate(zip(slots, rows)):
+            c, m = self._length[s], self._mapped[s]
+            end = -(-(c + n) // ps)
+            if c + n > self.max_length or end > len(self._pages[s]):
+                raise RuntimeError(f"slot {s}: {c} + {n} tokens are more than were reserved")
+            cached.append(c)
+            mapped.append(m)
+            pages += self._pages[s][m:end]
+            self._mapped[s] = max(m, end)
+            g = self._group.get(s)
+            if g is None or g != last:
+                start.append(i)
+                prefix.append(0 if g is None else g[1])
+            last = g
+        B, NG = len(slots), len(start)
+        flat = torch.tensor(cached + rows + slots + mapped + start + [B] + prefix + pages, dtype=torch.int32)
+        if self.device.type == "cuda":
+            flat = flat.pin_memory().to(self.device, non_blocking=True)
+        c, r, s, m, st, pr, pg = flat.split([B, B, B, B, NG + 1, NG, len(pages)])
+        group_rows = [sum(rows[a:b]) for a, b in zip(start, start[1:] + [B])]
+        self.plan = paged.page_plan(c, r, self.block_table, s, pg, ps, sum(rows), num_pages=self.num_pages, mapped=m,
+                                    group_start=st, group_prefix=pr, n_heads=self.heads[0], n_kv_heads=self.heads[1],
+                                    windows=self.windows, max_rows=max(group_rows))
+        self._step = (list(slots), list(rows))
+
+    def end_step(self) -> None:
+        for s, n in zip(*self._step):
+            self._length[s] += n
+        self._step = None
+
+    @property
+    def caches(self) -> "list[KVCache]":             # free-form per-layer state of the step's sequences (recurrent layers)
+        return [self._states[s] for s in self._step[0]]
+
+    @property
+    def rows(self) -> list[int]:
+        return self._step[1]
+
+    def attend(self, layer, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float, *, window: int = 0,
+               sinks: torch.Tensor | None = None) -> torch.Tensor:
+        from torchtitan_b200.ops import paged
+
+        pool = self.pools.get(id(layer))
+        if pool is None:
+            shape = (self.num_pages, k.shape[1], self.page_size, k.shape[2])
+            pool = self.pools[id(layer)] = (k.new_zeros(shape), k.new_zeros(shape))
+        paged.write_kv(k.detach(), v.detach(), *pool, self.plan.slot_map)
+        return paged.attention(q.detach(), *pool, self.plan, scale, window=window, sinks=sinks)
+
+
 def cached_attention(layer, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_cache, scale: float, *, window: int = 0,
                      sinks: torch.Tensor | None = None) -> torch.Tensor:
     """Append the new keys / values to ``layer``'s cache and attend the new queries to everything cached (causal
-    among the new rows).  ``kv_cache``: one ``KVCache`` (all rows belong to one sequence) or a ``BatchedKVCache``
-    (consecutive row blocks of several sequences).  Query / key and value head dimensions may differ (latent
+    among the new rows).  ``kv_cache``: one ``KVCache`` (all rows belong to one sequence), a ``BatchedKVCache``
+    (consecutive row blocks of several sequences) or a ``PagedKVCache`` (the same in one launch over all pages).  Query / key and value head dimensions may differ (latent
     attention); shapes the flash kernels do not cover run the PyTorch block attention."""
     from torchtitan_b200.ops import flash as FL
 
@@ -105,6 +286,8 @@ def cached_attention(layer, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k
             o_ = (o_.float() * torch.sigmoid(lse - sinks.float()[:, None]).t()[..., None]).to(q_.dtype)
         return o_
 
+    if isinstance(kv_cache, PagedKVCache):
+        return kv_cache.attend(layer, q, k, v, scale, window=window, sinks=sinks)
     if not isinstance(kv_cache, BatchedKVCache):
         return attend(kv_cache, q, k, v)
     parts, r0 = [], 0
@@ -127,6 +310,24 @@ def build_attention_context(positions: torch.Tensor, *, assume_single_document: 
     index = q_pos if (cp is not None and q_pos is not None) else torch.arange(positions.shape[0], device=positions.device)
     kv_first = (index - positions).to(torch.int32)
     return AttentionContext(doc_ids, q_pos, cp, kv_first=kv_first)
+
+
+def fused_qk_norm_rope(qkv: torch.Tensor, hq: int, hkv: int, q_norm, k_norm, rope: RoPE | None, positions: torch.Tensor,
+                       q_scale: float = 1.0):
+    """``(q, k, v)`` of a packed projection output ``[T, Hq + 2 Hkv, D]`` from the one-pass norm + rotation, or None when
+    ``kernels.qk_norm_rope`` does not ask for it or the layer has no per-head norms or shapes that it does not cover."""
+    if OF.settings.qk_norm_rope != "fused" or q_norm is None or q_norm.eps != k_norm.eps:
+        return None
+    gain = getattr(q_norm, "gain_center", 0.0)
+    plain = all(type(n) is RMSNorm or hasattr(n, "gain_center") for n in (q_norm, k_norm))
+    D = qkv.shape[2]
+    rot = rope.cache.shape[1] if rope is not None else 0
+    if not plain or gain != getattr(k_norm, "gain_center", 0.0) or D % 8 or D > 256 or rot > D or (
+            rot % (8 if rope is not None and rope.interleaved else 16)):
+        return None
+    return OF.qk_norm_rope(qkv, hq, hkv, q_norm.weight, k_norm.weight, None if rope is None else rope.cache, positions,
+                           rope is not None and rope.interleaved, eps=q_norm.eps, gain_center=gain, q_scale=q_scale,
+                           axes=None if rope is None else rope.axes_for(positions))
 
 
 class GQAttention(Module):
@@ -233,7 +434,10 @@ class GQAttention(Module):
         if self.q_norm is None:
             qkv = self.rope.apply_packed_(qkv, positions, hq + hkv, hd)
         qkv = qkv.view(T, hq + 2 * hkv, hd)
-        if self.q_norm is not None:
+        fused_qk = fused_qk_norm_rope(qkv, hq, hkv, self.q_norm, self.k_norm, self.rope, positions)
+        if fused_qk is not None:
+            q, k, v = fused_qk
+        elif self.q_norm is not None:
             # QK-norm normalises each head vector before RoPE (Qwen3).
             qn = self.q_norm(qkv[:, :hq])
             kn = self.k_norm(qkv[:, hq:hq + hkv])

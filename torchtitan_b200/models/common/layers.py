@@ -206,6 +206,7 @@ class RoPE(Module):
     def __init__(self, config: "RoPE.Config", **_):
         super().__init__(config)
         self.interleaved = config.style == "complex"
+        self._axes: torch.Tensor | None = None
         if config.mrope_sections is not None and sum(config.mrope_sections) * 2 != config.dim:
             raise ValueError(f"mrope_sections {config.mrope_sections} must sum to dim / 2 = {config.dim // 2}")
         self.register_buffer("cache", torch.empty(config.max_context_length, config.dim), persistent=False)
@@ -248,6 +249,22 @@ class RoPE(Module):
         f = torch.arange(half, device=positions.device)
         table = torch.cat([self.cache[pos_tf, f], self.cache[pos_tf, f + half]], dim=1).contiguous()
         return table, torch.arange(positions.shape[1], device=positions.device, dtype=torch.int64)
+
+    def axes_for(self, positions: torch.Tensor) -> torch.Tensor | None:
+        """Position axis of every rotary frequency (int32) for ``[3, T]`` positions, None for one axis."""
+        if positions.dim() == 1:
+            return None
+        secs = self.config.mrope_sections
+        if secs is None:
+            raise ValueError("3-axis positions need RoPE.Config.mrope_sections")
+        if self._axes is None or self._axes.device != positions.device:
+            half = self.config.dim // 2
+            if self.config.mrope_interleaved:
+                axes = [f % 3 if f % 3 and f < 3 * secs[f % 3] else 0 for f in range(half)]
+            else:
+                axes = [a for a, n in enumerate(secs) for _ in range(n)]
+            self._axes = torch.tensor(axes, dtype=torch.int32, device=positions.device)
+        return self._axes
 
     def forward(self, x: torch.Tensor, positions: torch.Tensor) -> torch.Tensor:
         table, pos = self._table_for(positions)

@@ -11,7 +11,7 @@ from dataclasses import dataclass, field
 import torch
 import torch.nn as nn
 
-from torchtitan_b200.models.common.attention import AttentionContext, GQAttention
+from torchtitan_b200.models.common.attention import AttentionContext, GQAttention, fused_qk_norm_rope
 from torchtitan_b200.models.common.decoder import TransformerBlock
 from torchtitan_b200.models.common.layers import Linear, RMSNorm
 from torchtitan_b200.models.common.module import InitSpec, Module, set_init
@@ -67,12 +67,17 @@ class MuseAttention(GQAttention):
             x = tp_ops.all_gather_rows(x, tp) if tp.sequence_parallel else tp_ops.copy_to_tp(x, tp)
         T = x.shape[0]
         qkv = self.wqkv(x).view(T, hq + 2 * hkv, hd)
-        q = self.q_norm(qkv[:, :hq]) * self.scale_query_by
-        k = self.k_norm(qkv[:, hq:hq + hkv])
-        v = qkv[:, hq + hkv:]
-        if self.use_rope:
-            rp = ctx.rope_positions if ctx is not None and ctx.rope_positions is not None else positions
-            q, k = self.rope(q, rp), self.rope(k, rp)
+        rp = ctx.rope_positions if ctx is not None and ctx.rope_positions is not None else positions
+        fused_qk = fused_qk_norm_rope(qkv, hq, hkv, self.q_norm, self.k_norm, self.rope if self.use_rope else None, rp,
+                                      q_scale=self.scale_query_by)
+        if fused_qk is not None:
+            q, k, v = fused_qk
+        else:
+            q = self.q_norm(qkv[:, :hq]) * self.scale_query_by
+            k = self.k_norm(qkv[:, hq:hq + hkv])
+            v = qkv[:, hq + hkv:]
+            if self.use_rope:
+                q, k = self.rope(q, rp), self.rope(k, rp)
         ctx = ctx or AttentionContext()
         if ctx.kv_cache is not None:          # incremental decoding
             from torchtitan_b200.models.common.attention import cached_attention

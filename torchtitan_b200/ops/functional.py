@@ -43,6 +43,7 @@ __all__ = [
 class _Settings:
     gemm: str = "tcgen05"  # "cublas" | "tcgen05"
     attention: str = "native"  # "sdpa" | "native"
+    qk_norm_rope: str = "separate"  # "separate" | "fused": per-head norms and RoPE as kernels of their own, or in one pass
     recompute: bool = True  # fused functions recompute norm / SwiGLU activations in backward
     launches: int = 0  # count of launches of this package's own kernels
     count_launches: bool = False

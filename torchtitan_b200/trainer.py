@@ -168,6 +168,7 @@ class Trainer(Configurable):
                                                c.debug.deterministic_warn_only)
         OF.settings.gemm = c.kernels.gemm
         OF.settings.attention = c.kernels.attention
+        OF.settings.qk_norm_rope = c.kernels.qk_norm_rope
         OF.settings.strict_native = False
         if c.debug.batch_invariant:
             from torchtitan_b200.experiments.rl.batch_invariance import enable_batch_invariant_mode
