@@ -316,6 +316,13 @@ def test_attention_long(groups, hq, hkv, D, ps, window):
 
 
 @pytest.mark.gpu
+def test_a_wrong_bound_on_the_rows_costs_speed_only():
+    s = _Step([(128, [(c, 2) for c in range(9)]), (0, [(300, 40), (5, 1)])], hq=8, hkv=2, D=128, ps=32, device="cuda")
+    for claim in (1, 5, 1000):
+        s.check(paged.attention(s.q, s.kp, s.vp, s.plan(max_rows=claim), s.scale))
+
+
+@pytest.mark.gpu
 def test_attention_writes_into_out_and_leaves_the_padding_alone():
     s = _Step([(64, [(5, 1), (9, 1)]), (0, [(30, 2)])], hq=8, hkv=2, D=128, ps=16, device="cuda", pad=3)
     out = torch.full(s.q.shape, 7.0, dtype=s.q.dtype, device="cuda")

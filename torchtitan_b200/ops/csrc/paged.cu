@@ -189,34 +189,43 @@ __global__ void __launch_bounds__(256) write_kernel(const WriteParams p) {
 // ------------------------------------------------------------------------------------------------------------- attention
 // Work.  A *source* is a set of neighbouring rows that all look at one key range of one table row: the rows of a sequence
 // on what follows its group's prefix, or all rows of a group on the prefix.  Its (row, query head of one key head) pairs
-// are cut into *units* of kUnitRows; a unit's keys are cut into tiles.  The tiles of all units and key heads form one line
-// that is cut into equal stretches, one per CTA, whatever the lengths are: a CTA works through the *pieces* of units that
-// fall into its stretch.  A piece that covers its unit is finished where it is; the others leave (max, sum, unnormalised
-// fp32 output) behind, at most two per CTA (the first and the last of a stretch), which the combine kernel joins in the
-// order of the line, so results do not depend on scheduling.  A group's two sources are joined there as well.
-constexpr int kUnitRows = 16;                    // pairs of a unit: one m16 tile
-constexpr int kTile = 64;                        // keys per tile
+// are cut into *units*, a unit's keys into tiles.  The tiles of all units and key heads form one line that is cut into
+// equal stretches, one per CTA, whatever the lengths are: a CTA works through the *pieces* of units that fall into its
+// stretch.  A piece that covers its unit is finished where it is; the others leave (max, sum, unnormalised fp32 output)
+// behind, at most two per CTA (the first and the last of a stretch), which the combine kernel joins in the order of the
+// line, so results do not depend on scheduling.  A group's two sources are joined there as well.
+//
+// There are two lists with a line each: units of 16 pairs and 64-key tiles for the kernel on mma.sync, units of 128 pairs
+// and 128-key tiles for the one on tcgen05.  A source of more than kFewPairs pairs is *large*: it is in both lists, behind
+// the small ones in the first, and runs from the second where that kernel is launched.
+constexpr int kRowsA = 16, kTileA = 64;
+constexpr int kRowsB = 128, kTileB = 128;
+constexpr int kFewPairs = 16;
 
-struct Unit {
+struct __align__(16) Unit {
   int row0, pairs, pair0, slot;                  // first row and pair count of the source, first pair of the unit, table row
   int key_lo, key_hi, base, direct;              // keys [lo, hi); position of the source's first row, or -1 for a prefix; alone
 };
 
 // Layout of the int32 work buffer (one per window), from the sizes that the host knows.
 struct WorkLayout {
-  int64_t seq_group, src_unit, tiles, units, size;   // header: [0] units, [1] tiles (of one key head)
-  __host__ __device__ WorkLayout(int64_t B, int64_t NG, int64_t max_units) {
-    seq_group = 4;
-    src_unit = seq_group + B;
-    tiles = (src_unit + B + NG + 3) / 4 * 4;
-    units = (tiles + max_units + 1 + 3) / 4 * 4;
-    size = units + 8 * max_units;
+  int64_t seq_group, src_a, src_b, tiles_a, tiles_b, units_a, units_b, size;
+  // header: [0, 1] units and tiles (of one key head) of the small sources in list A, [2, 3] of all, [4, 5] of list B
+  __host__ __device__ WorkLayout(int64_t B, int64_t NG, int64_t max_a, int64_t max_b) {
+    seq_group = 8;
+    src_a = seq_group + B;                       // first unit of each source, -1 = none
+    src_b = src_a + B + NG;
+    tiles_a = src_b + B + NG;                    // running tile counts
+    tiles_b = tiles_a + max_a + 1;
+    units_a = (tiles_b + max_b + 1 + 3) / 4 * 4;
+    units_b = units_a + 8 * max_a;
+    size = units_b + 8 * max_b;
   }
 };
 
 struct WorkParams {
   const int *cached, *row_start, *slots, *group_start, *group_prefix;
-  int B, NG, W, ps, G, window, max_units;
+  int B, NG, W, ps, G, window, max_a, max_b;
   int* work;
   int* status;
 };
@@ -224,15 +233,12 @@ struct WorkParams {
 __global__ void __launch_bounds__(1024) work_kernel(const WorkParams p) {
   extern __shared__ int sm[];
   const int n_src = p.B + p.NG;
-  int* unit_start = sm;                          // [n_src + 1]
-  int* prefix = sm + n_src + 1;                  // [NG] tokens of the group's prefix, as used
+  int* start = sm;                               // [n_src + 1] first unit of each source in the list at hand
+  int* prefix = start + n_src + 1;               // [NG] tokens of the group's prefix, as used
   int* leader = prefix + p.NG;                   // [NG] first sequence with rows
   __shared__ int part[33];
-  const WorkLayout lay(p.B, p.NG, p.max_units);
+  const WorkLayout lay(p.B, p.NG, p.max_a, p.max_b);
   int* seq_group = p.work + lay.seq_group;
-  int* src_unit = p.work + lay.src_unit;
-  int* tiles = p.work + lay.tiles;
-  Unit* units = reinterpret_cast<Unit*>(p.work + lay.units);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   bool bad = false;
   for (int b = threadIdx.x; b < p.B; b += blockDim.x) seq_group[b] = -1;
@@ -248,12 +254,9 @@ __global__ void __launch_bounds__(1024) work_kernel(const WorkParams p) {
       shortest = min(shortest, p.cached[b]);
       first = min(first, b);
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      live += __shfl_xor_sync(0xffffffffu, live, o);
-      shortest = min(shortest, __shfl_xor_sync(0xffffffffu, shortest, o));
-      first = min(first, __shfl_xor_sync(0xffffffffu, first, o));
-    }
+    live = __reduce_add_sync(0xffffffffu, live);
+    shortest = __reduce_min_sync(0xffffffffu, shortest);
+    first = __reduce_min_sync(0xffffffffu, first);
     const int use = live > 1 ? max(0, min(p.group_prefix[g], shortest)) : 0;
     if (lane == 0) { prefix[g] = use; leader[g] = first; }
     if (use > 0)
@@ -273,83 +276,108 @@ __global__ void __launch_bounds__(1024) work_kernel(const WorkParams p) {
       }
     }
   };
-  int n_units = 0;
-  for (int s0 = 0; s0 < n_src; s0 += blockDim.x) {
-    const int s = s0 + threadIdx.x;
-    int n = 0;
-    if (s < n_src) {
-      int r0, r1;
-      source_rows(s, r0, r1);
-      n = (int)(((int64_t)(r1 - r0) * p.G + kUnitRows - 1) / kUnitRows);
-    }
-    int total;
-    const int e = block_scan(n, part, total);
-    if (s < n_src) {
-      unit_start[s] = n_units + e - n;
-      src_unit[s] = n > 0 ? n_units + e - n : -1;
-    }
-    n_units += total;
-  }
-  if (threadIdx.x == 0) unit_start[n_src] = n_units;
-  if (n_units > p.max_units) {                   // overlapping groups: device data that is flagged
-    bad = true;
-    n_units = p.max_units;
-  }
-  __syncthreads();
-  int n_tiles = 0;
-  for (int u0 = 0; u0 < n_units; u0 += blockDim.x) {
-    const int u = u0 + threadIdx.x;
-    int n = 0;
-    if (u < n_units) {
-      const int s = find_segment(unit_start, n_src, u);
-      int r0, r1;
-      source_rows(s, r0, r1);
-      Unit w;
-      w.row0 = r0;
-      w.pairs = (r1 - r0) * p.G;
-      w.pair0 = (u - unit_start[s]) * kUnitRows;
-      const int last = min(w.pair0 + kUnitRows, w.pairs) - 1;
-      const int64_t room = (int64_t)p.W * p.ps;
-      if (s < p.B) {
-        const int g = seq_group[s], c = p.cached[s];
-        w.slot = p.slots[s];
-        w.base = c;
-        w.direct = g < 0;
-        w.key_lo = g < 0 ? 0 : prefix[g];
-        if (p.window > 0) w.key_lo = max(w.key_lo, c + w.pair0 / p.G - p.window + 1);
-        w.key_hi = (int)min((int64_t)c + last / p.G + 1, room);
-      } else {
-        const int g = s - p.B;
-        w.slot = p.slots[min(leader[g], p.B - 1)];
-        w.base = -1;
-        w.direct = 0;
-        // the smallest position of the group's rows bounds the window of all of them
-        int from = 0;
-        if (p.window > 0) {
-          from = INT_MAX;
-          const int a = min(max(p.group_start[g], 0), p.B), e = min(max(p.group_start[g + 1], a), p.B);
-          for (int b = a; b < e; ++b)
-            if (p.row_start[b + 1] > p.row_start[b]) from = min(from, p.cached[b]);
-          from = max(0, from - p.window + 1);
-        }
-        w.key_lo = from;
-        w.key_hi = (int)min((int64_t)prefix[g], room);
+  // Appends the units of the small or the large sources to a list that has `n0` units and `t0` tiles already.
+  auto list = [&](bool large, int rows, int tile, int max_units, int* src, int* tiles, Unit* units, int& n0, int& t0) {
+    int n_units = 0;
+    for (int s0 = 0; s0 < n_src; s0 += blockDim.x) {
+      const int s = s0 + threadIdx.x;
+      int n = 0;
+      bool mine = false;
+      if (s < n_src) {
+        int r0, r1;
+        source_rows(s, r0, r1);
+        const int64_t pairs = (int64_t)max(0, r1 - r0) * p.G;
+        mine = (pairs > kFewPairs) == large;
+        if (mine) n = (int)((pairs + rows - 1) / rows);
       }
-      n = w.key_hi > w.key_lo ? (w.key_hi - 1) / kTile - w.key_lo / kTile + 1 : 0;
-      units[u] = w;
+      int total;
+      const int e = block_scan(n, part, total);
+      if (s < n_src) {
+        start[s] = n_units + e - n;
+        if (mine) src[s] = n > 0 ? n0 + n_units + e - n : -1;
+        else if (large && rows == kRowsB) src[s] = -1;
+      }
+      n_units += total;
     }
-    int total;
-    const int e = block_scan(n, part, total);
-    if (u < n_units) tiles[u] = n_tiles + e - n;
-    n_tiles += total;
-  }
-  if (threadIdx.x == 0) {
-    tiles[n_units] = n_tiles;
-    p.work[0] = n_units;
-    p.work[1] = n_tiles;
-  }
+    if (threadIdx.x == 0) start[n_src] = n_units;
+    if (n_units > max_units - n0) {              // overlapping groups: device data that is flagged
+      bad = true;
+      n_units = max_units - n0;
+    }
+    __syncthreads();
+    int n_tiles = 0;
+    for (int u0 = 0; u0 < n_units; u0 += blockDim.x) {
+      const int u = u0 + threadIdx.x;
+      int n = 0;
+      if (u < n_units) {
+        const int s = find_segment(start, n_src, u);
+        int r0, r1;
+        source_rows(s, r0, r1);
+        Unit w;
+        w.row0 = r0;
+        w.pairs = (r1 - r0) * p.G;
+        w.pair0 = (u - start[s]) * rows;
+        const int last = min(w.pair0 + rows, w.pairs) - 1;
+        const int64_t room = (int64_t)p.W * p.ps;
+        if (s < p.B) {
+          const int g = seq_group[s], c = p.cached[s];
+          w.slot = p.slots[s];
+          w.base = c;
+          w.direct = g < 0;
+          w.key_lo = g < 0 ? 0 : prefix[g];
+          if (p.window > 0) w.key_lo = max(w.key_lo, c + w.pair0 / p.G - p.window + 1);
+          w.key_hi = (int)min((int64_t)c + last / p.G + 1, room);
+        } else {
+          const int g = s - p.B;
+          w.slot = p.slots[min(leader[g], p.B - 1)];
+          w.base = -1;
+          w.direct = 0;
+          // the smallest position of the group's rows bounds the window of all of them
+          int from = 0;
+          if (p.window > 0) {
+            from = INT_MAX;
+            const int a = min(max(p.group_start[g], 0), p.B), e = min(max(p.group_start[g + 1], a), p.B);
+            for (int b = a; b < e; ++b)
+              if (p.row_start[b + 1] > p.row_start[b]) from = min(from, p.cached[b]);
+            from = max(0, from - p.window + 1);
+          }
+          w.key_lo = from;
+          w.key_hi = (int)min((int64_t)prefix[g], room);
+        }
+        n = w.key_hi > w.key_lo ? (w.key_hi - 1) / tile - w.key_lo / tile + 1 : 0;
+        units[n0 + u] = w;
+      }
+      int total;
+      const int e = block_scan(n, part, total);
+      if (u < n_units) tiles[n0 + u] = t0 + n_tiles + e - n;
+      n_tiles += total;
+    }
+    n0 += n_units;
+    t0 += n_tiles;
+    if (threadIdx.x == 0) tiles[n0] = t0;
+    __syncthreads();
+  };
+  int n = 0, t = 0;
+  int *src_a = p.work + lay.src_a, *src_b = p.work + lay.src_b, *tiles_a = p.work + lay.tiles_a, *tiles_b = p.work + lay.tiles_b;
+  Unit *units_a = reinterpret_cast<Unit*>(p.work + lay.units_a), *units_b = reinterpret_cast<Unit*>(p.work + lay.units_b);
+  list(false, kRowsA, kTileA, p.max_a, src_a, tiles_a, units_a, n, t);
+  if (threadIdx.x == 0) { p.work[0] = n; p.work[1] = t; }
+  list(true, kRowsA, kTileA, p.max_a, src_a, tiles_a, units_a, n, t);
+  if (threadIdx.x == 0) { p.work[2] = n; p.work[3] = t; }
+  n = t = 0;
+  list(true, kRowsB, kTileB, p.max_b, src_b, tiles_b, units_b, n, t);
+  if (threadIdx.x == 0) { p.work[4] = n; p.work[5] = t; }
   if (bad) atomicOr(p.status, kStatusPagePlanInvalid);
 }
+
+// One kernel's view of its list.
+struct List {
+  const int* tiles;
+  const Unit* units;
+  int n_units, n_tiles, ctas;
+  // Tiles of a CTA's stretch.
+  __device__ __forceinline__ int64_t stretch(int Hkv) const { return max((int64_t)kMinTiles, ((int64_t)n_tiles * Hkv + ctas - 1) / ctas); }
+};
 
 struct AttnParams {
   const __nv_bfloat16* q;
@@ -357,22 +385,31 @@ struct AttnParams {
   __nv_bfloat16* out;                            // [R, Hq, D]
   const float* sinks;                            // [Hq] or null
   const int *table, *cached, *row_start, *work;
-  int B, NG, S, W, R, Hq, Hkv, G, ps, num_pages, window, max_units, ctas;
+  int B, NG, W, R, Hq, Hkv, G, ps, num_pages, window, max_a, max_b, ctas_a, ctas_b;
   float scale_log2;
-  bool zero_tail;
-  float *part_o, *part_ml;                       // [ctas, 2, kUnitRows, D], [ctas, 2, kUnitRows, 2]: pieces
+  bool zero_tail, use_b;                         // use_b: large sources run on the tcgen05 kernel
+  float *part_a, *part_a_ml;                     // [ctas_a, 2, kRowsA, D], [ctas_a, 2, kRowsA, 2]: pieces
+  float *part_b, *part_b_ml;                     // [ctas_b, 2, kRowsB, D], [ctas_b, 2, kRowsB, 2]
   float *row_o, *row_ml;                         // [2, R, Hq, D], [2, R, Hq, 2]: whole units of groups (own keys, prefix)
   int* status;
+
+  __device__ __forceinline__ List list_a(const WorkLayout& lay) const {
+    const int h = use_b ? 0 : 2;
+    return {work + lay.tiles_a, reinterpret_cast<const Unit*>(work + lay.units_a), work[h], work[h + 1], ctas_a};
+  }
+  __device__ __forceinline__ List list_b(const WorkLayout& lay) const {
+    return {work + lay.tiles_b, reinterpret_cast<const Unit*>(work + lay.units_b), work[4], work[5], ctas_b};
+  }
 };
 
 template <int D>
 struct Cfg {
   static constexpr int kStages = D == 64 ? 4 : D == 128 ? 3 : 2;
   static constexpr int kCtasPerSm = D == 256 ? 1 : 2;
-  static constexpr uint32_t kHalfBytes = kTile * D * 2;          // keys (or values) of a tile
+  static constexpr uint32_t kHalfBytes = kTileA * D * 2;         // keys (or values) of a tile
   static constexpr uint32_t kStageBytes = 2 * kHalfBytes;
-  static constexpr uint32_t kExchange = 2 * kUnitRows * D * 4;   // two fp32 output tiles
-  static constexpr uint32_t kSmem = kStages * kStageBytes + kExchange + 4 * kUnitRows * 2 * 4 + 16 * kStages + 16;
+  static constexpr uint32_t kExchange = 2 * kRowsA * D * 4;   // two fp32 output tiles
+  static constexpr uint32_t kSmem = kStages * kStageBytes + kExchange + 4 * kRowsA * 2 * 4 + 16 * kStages + 16;
 };
 
 __device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
@@ -404,28 +441,31 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
       : "memory");
 }
 
-// Tiles of a CTA's stretch.
-__device__ __forceinline__ int64_t stretch(const int* work, int Hkv, int ctas) {
-  return max((int64_t)kMinTiles, ((int64_t)work[1] * Hkv + ctas - 1) / ctas);
+// A bounded wait whose outcome is the same for all lanes, so that a warp leaves as one.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+  return __all_sync(0xffffffffu, tc::mbar_wait(bar, parity, abort_flag));
+}
+
+// After an abort: the copies of the last tiles are waited for (with a limit) before the block may end.
+template <typename F>
+__device__ __forceinline__ void drain(int it, int stages, F full) {
+  volatile int quiet = 0;
+  for (int j = max(0, it - stages); j < it; ++j) tc::mbar_wait(full(j % stages), (j / stages) & 1, &quiet);
 }
 
 // A CTA's walk over its stretch of the line.
 struct Walk {
   const int* tiles;
-  const Unit* units;
-  int n_units, Hkv;
+  int Hkv;
   int64_t at, end;
   int u, head, first, count;                     // current piece: unit, key head, first tile of the unit, tiles
   int unit_tiles;
 
-  __device__ __forceinline__ Walk(const int* work, const WorkLayout& lay, int Hkv_, int cta, int ctas) : Hkv(Hkv_) {
-    tiles = work + lay.tiles;
-    units = reinterpret_cast<const Unit*>(work + lay.units);
-    n_units = work[0];
-    const int64_t line = (int64_t)work[1] * Hkv, per = stretch(work, Hkv, ctas);
+  __device__ __forceinline__ Walk(const List& l, int Hkv_, int cta) : tiles(l.tiles), Hkv(Hkv_) {
+    const int64_t line = (int64_t)l.n_tiles * Hkv, per = l.stretch(Hkv);
     at = min(line, cta * per);
     end = min(line, at + per);
-    u = at < end ? find_segment(tiles, n_units, (int)(at / Hkv)) : 0;
+    u = at < end ? find_segment(tiles, l.n_units, (int)(at / Hkv)) : 0;
   }
   __device__ __forceinline__ bool next() {
     if (at >= end) return false;
@@ -453,8 +493,8 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t base = smem_u32(smem);
   float* exch = reinterpret_cast<float*>(smem + C::kStages * C::kStageBytes);
-  float* ml = exch + C::kExchange / 4;                                   // [4][kUnitRows][2]
-  const uint32_t bars = base + C::kStages * C::kStageBytes + C::kExchange + 4 * kUnitRows * 2 * 4;
+  float* ml = exch + C::kExchange / 4;                                   // [4][kRowsA][2]
+  const uint32_t bars = base + C::kStages * C::kStageBytes + C::kExchange + 4 * kRowsA * 2 * 4;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + (bars - base) + 16 * C::kStages);
   auto full = [&](int s) { return bars + 16u * s; };
   auto empty = [&](int s) { return bars + 16u * s + 8u; };
@@ -468,23 +508,23 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
     mbar_fence_init();
   }
   __syncthreads();
-  const WorkLayout lay(p.B, p.NG, p.max_units);
-  Walk walk(p.work, lay, p.Hkv, blockIdx.x, p.ctas);
+  const List list = p.list_a(WorkLayout(p.B, p.NG, p.max_a, p.max_b));
+  Walk walk(list, p.Hkv, blockIdx.x);
   int it = 0;
 
   if (warp == 4) {
     // ---------------------------------------------------------------------------------------------------- producer
-    const int box = min(p.ps, kTile), subs = kTile / box;
+    const int box = min(p.ps, kTileA), subs = kTileA / box;
     const int loads = 2 * (D / 64) * subs;       // at most 2 * 4 * 4 = 32: one lane each
     const int kv = lane / ((D / 64) * subs), col = (lane / subs) % (D / 64), sub = lane % subs;
     const CUtensorMap* map = kv ? &tmap_v : &tmap_k;
     bool ok = true;
     while (ok && walk.next()) {
-      const Unit u = walk.units[walk.u];
+      const Unit u = list.units[walk.u];
       const int* row = p.table + (int64_t)u.slot * p.W;
-      const int t0 = u.key_lo / kTile + walk.first;
+      const int t0 = u.key_lo / kTileA + walk.first;
       auto entry = [&](int t) {                  // page of this lane's box of tile t, -1 when no key of it is needed
-        const int64_t key = (int64_t)t * kTile + sub * box;
+        const int64_t key = (int64_t)t * kTileA + sub * box;
         return lane < loads && key < u.key_hi ? row[key / p.ps] : INT_MIN;
       };
       int page = entry(t0);
@@ -492,7 +532,7 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
         const int st = it % C::kStages;
         const int t = t0 + i;
         const int after = i + 1 < walk.count ? entry(t + 1) : INT_MIN;
-        if (!mbar_wait(empty(st), ((it / C::kStages) & 1) ^ 1, abort_flag)) { ok = false; break; }
+        if (!warp_wait(empty(st), ((it / C::kStages) & 1) ^ 1, abort_flag)) { ok = false; break; }
         const int need = __popc(__ballot_sync(0xffffffffu, page != INT_MIN));
         if (lane == 0) mbar_expect_tx(full(st), need * box * 128);
         __syncwarp();
@@ -501,19 +541,20 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
             atomicOr(p.status, kStatusPagePlanInvalid);
             page = p.num_pages;
           }
-          const int key = t * kTile + sub * box;
-          tma_load_4d(base + st * C::kStageBytes + kv * C::kHalfBytes + col * (kTile * 128) + sub * box * 128, map, full(st),
+          const int key = t * kTileA + sub * box;
+          tma_load_4d(base + st * C::kStageBytes + kv * C::kHalfBytes + col * (kTileA * 128) + sub * box * 128, map, full(st),
                       col * 64, key % p.ps, walk.head, page);
         }
         page = after;
       }
     }
+    if (!ok) drain(it, C::kStages, full);
   } else {
     // ---------------------------------------------------------------------------------------------------- consumers
     const int quad = lane & 3, r_lo = lane >> 2;                         // this thread's rows: r_lo and r_lo + 8
     bool ok = true;
     while (ok && walk.next()) {
-      const Unit u = walk.units[walk.u];
+      const Unit u = list.units[walk.u];
       // rows: queries as A fragments, visible key range
       uint32_t qf[D / 16][4];
       int lo[2], hi[2];
@@ -556,12 +597,12 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
         for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
       float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 
-      const int t0 = u.key_lo / kTile + walk.first;
+      const int t0 = u.key_lo / kTileA + walk.first;
       for (int i = 0; i < walk.count; ++i, ++it) {
         const int st = it % C::kStages;
-        if (!mbar_wait(full(st), (it / C::kStages) & 1, abort_flag)) { ok = false; break; }
+        if (!warp_wait(full(st), (it / C::kStages) & 1, abort_flag)) { ok = false; break; }
         const uint32_t ks = base + st * C::kStageBytes, vs = ks + C::kHalfBytes;
-        const int k0 = (t0 + i) * kTile + warp * 16;                     // this warp's first key
+        const int k0 = (t0 + i) * kTileA + warp * 16;                     // this warp's first key
         const int kr = warp * 16;
         if (k0 <= hi_max && k0 + 15 >= lo_min) {
           // S = Q K^T
@@ -577,7 +618,7 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
             for (int k = 0; k < D / 16; ++k) {
               const int chunk = (k & 3) * 2 + ((lane >> 3) & 1);
               uint32_t b[4];
-              ldmatrix4(rowa + (k >> 2) * (kTile * 128) + ((chunk ^ (key & 7)) << 4), b);
+              ldmatrix4(rowa + (k >> 2) * (kTileA * 128) + ((chunk ^ (key & 7)) << 4), b);
               mma16816(s[0], qf[k], b[0], b[1]);
               mma16816(s[1], qf[k], b[2], b[3]);
             }
@@ -596,7 +637,7 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
               for (int c = lane; c < 16 * (D / 8); c += 32) {
                 const int key = c / (D / 8), ch = c % (D / 8);
                 if (k0 + key > hi_max || k0 + key < lo_min)
-                  asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(vs + (ch >> 3) * (kTile * 128) + (kr + key) * 128 +
+                  asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(vs + (ch >> 3) * (kTileA * 128) + (kr + key) * 128 +
                                (((ch & 7) ^ ((kr + key) & 7)) << 4)), "r"(0) : "memory");
               }
               fence_proxy_async_smem();
@@ -644,7 +685,7 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
             for (int n = 0; n < D / 16; ++n) {
               const int chunk = (n & 3) * 2 + (lane >> 4);
               uint32_t b[4];
-              ldmatrix4_t(rowa + (n >> 2) * (kTile * 128) + ((chunk ^ (key & 7)) << 4), b);
+              ldmatrix4_t(rowa + (n >> 2) * (kTileA * 128) + ((chunk ^ (key & 7)) << 4), b);
               mma16816(o[2 * n], pf, b[0], b[1]);
               mma16816(o[2 * n + 1], pf, b[2], b[3]);
             }
@@ -659,15 +700,15 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
         l[j] += __shfl_xor_sync(0xffffffffu, l[j], 1);
         l[j] += __shfl_xor_sync(0xffffffffu, l[j], 2);
         if (quad == 0) {
-          ml[(warp * kUnitRows + r_lo + 8 * j) * 2] = m[j];
-          ml[(warp * kUnitRows + r_lo + 8 * j) * 2 + 1] = l[j];
+          ml[(warp * kRowsA + r_lo + 8 * j) * 2] = m[j];
+          ml[(warp * kRowsA + r_lo + 8 * j) * 2 + 1] = l[j];
         }
       }
       if (consumer_any(!ok)) break;              // a wait ran out: all four leave together
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         float mm = -INFINITY;
-        for (int w = 0; w < 4; ++w) mm = fmaxf(mm, ml[(w * kUnitRows + r_lo + 8 * j) * 2]);
+        for (int w = 0; w < 4; ++w) mm = fmaxf(mm, ml[(w * kRowsA + r_lo + 8 * j) * 2]);
         const float f = m[j] == -INFINITY ? 0.f : exp2f(m[j] - mm);
 #pragma unroll
         for (int n = 0; n < D / 8; ++n) {
@@ -676,7 +717,7 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
         }
       }
       // an fp32 tile in shared memory: column blocks of eight are spread over the banks by the row
-      auto slot = [&](int which, int row, int c) { return exch + which * (kUnitRows * D) + row * D + (c ^ ((row & 7) << 3)); };
+      auto slot = [&](int which, int row, int c) { return exch + which * (kRowsA * D) + row * D + (c ^ ((row & 7) << 3)); };
       auto put = [&](int which) {
 #pragma unroll
         for (int n = 0; n < D / 8; ++n)
@@ -707,16 +748,16 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
       const bool whole = walk.count == walk.unit_tiles;
       const int which = walk.first > 0 ? 0 : 1;
       const int64_t cta = blockIdx.x;
-      for (int c = threadIdx.x; c < kUnitRows * (D / 4); c += 128) {
+      for (int c = threadIdx.x; c < kRowsA * (D / 4); c += 128) {
         const int row = c / (D / 4), d = (c % (D / 4)) * 4;
         const int pr = u.pair0 + row;
         if (pr >= u.pairs) continue;
         const float4 v = *reinterpret_cast<const float4*>(slot(0, row, d));
         float mm = -INFINITY, ll = 0.f;
-        for (int w = 0; w < 4; ++w) mm = fmaxf(mm, ml[(w * kUnitRows + row) * 2]);
+        for (int w = 0; w < 4; ++w) mm = fmaxf(mm, ml[(w * kRowsA + row) * 2]);
         for (int w = 0; w < 4; ++w) {
-          const float mw = ml[(w * kUnitRows + row) * 2];
-          ll += mw == -INFINITY ? 0.f : exp2f(mw - mm) * ml[(w * kUnitRows + row) * 2 + 1];
+          const float mw = ml[(w * kRowsA + row) * 2];
+          ll += mw == -INFINITY ? 0.f : exp2f(mw - mm) * ml[(w * kRowsA + row) * 2 + 1];
         }
         const int64_t rh = (int64_t)(u.row0 + pr / p.G) * p.Hq + walk.head * p.G + pr % p.G;
         if (whole && u.direct) {
@@ -734,15 +775,391 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
           *reinterpret_cast<float4*>(p.row_o + at * D + d) = v;
           if (d == 0) *reinterpret_cast<float2*>(p.row_ml + at * 2) = make_float2(mm, ll);
         } else {
-          const int64_t at = (cta * 2 + which) * kUnitRows + row;
-          *reinterpret_cast<float4*>(p.part_o + at * D + d) = v;
-          if (d == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(mm, ll);
+          const int64_t at = (cta * 2 + which) * kRowsA + row;
+          *reinterpret_cast<float4*>(p.part_a + at * D + d) = v;
+          if (d == 0) *reinterpret_cast<float2*>(p.part_a_ml + at * 2) = make_float2(mm, ll);
         }
       }
       consumer_sync();
     }
   }
   __syncthreads();
+  if (threadIdx.x == 0 && *abort_flag) atomicOr(p.status, kStatusWaitTimedOut);
+}
+
+// Many rows behind one key range (a prefix with the rows of its group, the rows of a prompt chunk): tcgen05.
+//
+// A unit is 128 pairs, one TMEM lane each; tiles of 128 keys alternate between two softmax warpgroups, which keep their own
+// running maximum, sum and output accumulator, so neither waits for the other and the softmax of one tile runs under the
+// MMAs of the next.  Per tile: S = Q K^T into tensor memory, P = exp2(S - m) written over S as bf16, O += P V with P read
+// from tensor memory.  An S is issued behind the P V of the same warpgroup's previous tile, so "S is there" also says that
+// the accumulator may be rescaled.  Bound by the exponentials (128 x 128 per tile on a 16-per-clock unit are 1024 clocks, as
+// many as the MMAs take) when many units share their keys through L2, by HBM when each key range has one unit.
+//   warp 0: TMA producer    warp 1: TMEM, MMA issue    warps 2..5, 6..9: softmax of even / odd tiles, then the output
+// Tensor memory: S of warpgroup g at column 128 g, O at 256 + 128 g.
+template <int D>
+struct CfgB {
+  static constexpr int kStages = 3;
+  static constexpr uint32_t kTileBytes = kTileB * D * 2;         // keys (or values) of a tile, or the queries of a unit
+  static constexpr uint32_t kBars = kTileBytes * (1 + 2 * kStages);
+  static constexpr int kNumBars = 4 * kStages + 7;
+  static constexpr uint32_t kMl = kBars + 8 * kNumBars + 8;      // TMEM address, abort flag
+  static constexpr uint32_t kSmem = kMl + 2 * kRowsB * 2 * 4;
+};
+
+// Named barrier of the eight softmax warps; true for all when any thread brings true.
+__device__ __forceinline__ bool softmax_any(bool v) {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred a, b;\n\tsetp.ne.u32 a, %1, 0;\n\tbar.red.or.pred b, 2, 256, a;\n\tselp.u32 %0, 1, 0, b;\n\t}"
+               : "=r"(r) : "r"((uint32_t)v) : "memory");
+  return r != 0;
+}
+
+template <int D>
+__global__ void __launch_bounds__(320, 1)
+attn_block_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const AttnParams p) {
+  using C = CfgB<D>;
+  using namespace tc;
+  constexpr uint32_t kColBytes = kTileB * 128;                   // one 64-column block of a tile
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const uint32_t base = smem_u32(smem);
+  const uint32_t q_smem = base;
+  auto k_smem = [&](int s) { return base + C::kTileBytes * (1 + 2 * s); };
+  auto v_smem = [&](int s) { return base + C::kTileBytes * (2 + 2 * s); };
+  const uint32_t bars = base + C::kBars;
+  auto k_full = [&](int s) { return bars + 8u * s; };
+  auto k_empty = [&](int s) { return bars + 8u * (C::kStages + s); };
+  auto v_full = [&](int s) { return bars + 8u * (2 * C::kStages + s); };
+  auto v_empty = [&](int s) { return bars + 8u * (3 * C::kStages + s); };
+  auto s_full = [&](int g) { return bars + 8u * (4 * C::kStages + g); };
+  auto p_ready = [&](int g) { return bars + 8u * (4 * C::kStages + 2 + g); };
+  const uint32_t o_full = bars + 8u * (4 * C::kStages + 4), q_ready = o_full + 8u, o_free = o_full + 16u;
+  uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(smem + C::kBars + 8 * C::kNumBars);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_ptr + 1);
+  float* ml = reinterpret_cast<float*>(smem + C::kMl);           // [2][kRowsB][2]
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  const List list = p.list_b(WorkLayout(p.B, p.NG, p.max_a, p.max_b));
+  Walk walk(list, p.Hkv, blockIdx.x);
+  if (walk.at >= walk.end) return;                               // the same for the whole block
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(k_full(s), 1);
+      mbar_init(k_empty(s), 1);
+      mbar_init(v_full(s), 1);
+      mbar_init(v_empty(s), 1);
+    }
+    for (int g = 0; g < 2; ++g) {
+      mbar_init(s_full(g), 1);
+      mbar_init(p_ready(g), 4);
+    }
+    mbar_init(o_full, 1);
+    mbar_init(q_ready, 8);
+    mbar_init(o_free, 8);
+    *abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(tmem_ptr), 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_ptr;
+
+  if (warp == 0) {
+    // ---------------------------------------------------------------------------------------------------- producer
+    const int box = min(p.ps, 64), subs = kTileB / box;
+    const int loads = (D / 64) * subs;           // at most 2 * 8 = 16 per operand: lanes 0..15 keys, 16..31 values
+    const int kv = lane >> 4, li = lane & 15, col = li / subs, sub = li % subs;
+    const CUtensorMap* map = kv ? &tmap_v : &tmap_k;
+    bool ok = true;
+    int it = 0, issued_k = 0, issued_v = 0;
+    while (ok && walk.next()) {
+      const Unit u = list.units[walk.u];
+      const int* row = p.table + (int64_t)u.slot * p.W;
+      const int t0 = u.key_lo / kTileB + walk.first;
+      auto entry = [&](int t) {
+        const int64_t key = (int64_t)t * kTileB + sub * box;
+        return li < loads && key < u.key_hi ? row[key / p.ps] : INT_MIN;
+      };
+      int page = entry(t0);
+      for (int i = 0; i < walk.count; ++i, ++it) {
+        const int st = it % C::kStages;
+        const uint32_t parity = ((it / C::kStages) & 1) ^ 1;
+        const int t = t0 + i;
+        const int after = i + 1 < walk.count ? entry(t + 1) : INT_MIN;
+        const bool wanted = page != INT_MIN;
+        const int need = __popc(__ballot_sync(0xffffffffu, wanted) & 0xffffu);
+        if (wanted && (page < 0 || page >= p.num_pages)) {        // out of range: the load fills zeros
+          atomicOr(p.status, kStatusPagePlanInvalid);
+          page = p.num_pages;
+        }
+        const int slot = (int)(((int64_t)t * kTileB + sub * box) % p.ps);
+        const uint32_t off = col * kColBytes + sub * box * 128;
+        if (!warp_wait(k_empty(st), parity, abort_flag)) { ok = false; break; }
+        if (lane == 0) mbar_expect_tx(k_full(st), need * box * 128);
+        __syncwarp();
+        if (wanted && kv == 0) tma_load_4d(k_smem(st) + off, map, k_full(st), col * 64, slot, walk.head, page);
+        issued_k = it + 1;
+        if (!warp_wait(v_empty(st), parity, abort_flag)) { ok = false; break; }
+        if (lane == 0) mbar_expect_tx(v_full(st), need * box * 128);
+        __syncwarp();
+        if (wanted && kv == 1) tma_load_4d(v_smem(st) + off, map, v_full(st), col * 64, slot, walk.head, page);
+        issued_v = it + 1;
+        page = after;
+      }
+    }
+    if (!ok) {
+      drain(issued_k, C::kStages, k_full);
+      drain(issued_v, C::kStages, v_full);
+    }
+  } else if (warp == 1) {
+    // ---------------------------------------------------------------------------------------------------- MMA issue
+    if (lane == 0) {
+      const uint32_t idesc_s = make_idesc(false, false, kRowsB, kTileB);
+      const uint32_t idesc_pv = make_idesc(false, true, kRowsB, D);       // values are [keys, D]: MN-major
+      auto issue_s = [&](int g, int st) {
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const uint32_t off = (uint32_t)(k >> 2) * kColBytes + (uint32_t)(k & 3) * 32u;
+          umma_bf16<1>(tmem + 128 * g, make_desc(q_smem + off, 16, 1024), make_desc(k_smem(st) + off, 16, 1024), idesc_s, k != 0);
+        }
+      };
+      int it = 0, piece = 0;
+      int turn[2] = {0, 0};                      // tiles so far of each warpgroup
+      bool ok = true;
+      while (ok && walk.next()) {
+        const int n = walk.count;
+        ok = mbar_wait(q_ready, piece & 1, abort_flag);
+        for (int j = 0; j < min(n, 2) && ok; ++j) {
+          const int st = (it + j) % C::kStages;
+          ok = mbar_wait(k_full(st), ((it + j) / C::kStages) & 1, abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+          issue_s(j, st);
+          umma_commit(s_full(j));
+          umma_commit(k_empty(st));
+        }
+        // the output of the piece before has been read
+        ok = ok && (piece == 0 || mbar_wait(o_free, (piece - 1) & 1, abort_flag));
+        for (int j = 0; j < n && ok; ++j) {
+          const int g = j & 1, st = (it + j) % C::kStages;
+          ok = mbar_wait(v_full(st), ((it + j) / C::kStages) & 1, abort_flag) && mbar_wait(p_ready(g), turn[g] & 1, abort_flag);
+          if (!ok) break;
+          ++turn[g];
+          tc_fence_after();
+#pragma unroll
+          for (int k = 0; k < kTileB / 16; ++k)  // 16 keys: 8 packed columns of P, 16 rows of V
+            umma_bf16_ts(tmem + 256 + 128 * g, tmem + 128 * g + k * 8, make_desc(v_smem(st) + k * 2048, kColBytes, 1024), idesc_pv,
+                         j >= 2 || k != 0);
+          umma_commit(v_empty(st));
+          if (j + 2 < n) {
+            const int st2 = (it + j + 2) % C::kStages;
+            ok = mbar_wait(k_full(st2), ((it + j + 2) / C::kStages) & 1, abort_flag);
+            if (!ok) break;
+            tc_fence_after();
+            issue_s(g, st2);
+            umma_commit(s_full(g));
+            umma_commit(k_empty(st2));
+          }
+        }
+        if (ok) umma_commit(o_full);
+        it += n;
+        ++piece;
+      }
+    }
+    __syncwarp();
+  } else {
+    // ---------------------------------------------------------------------------------------------------- softmax
+    const int g = (warp - 2) >> 2, quarter = warp & 3;
+    const int r = quarter * 32 + lane;           // this thread's pair in the unit, and its TMEM lane
+    const uint32_t s_t = tmem + ((uint32_t)(quarter * 32) << 16) + 128 * g;
+    const uint32_t o_t = tmem + ((uint32_t)(quarter * 32) << 16) + 256;
+    int it = 0, piece = 0, turn = 0;
+    bool ok = true;
+    while (ok && walk.next()) {
+      const Unit u = list.units[walk.u];
+      const int n = walk.count;
+      // queries, swizzled as TMA would: warpgroup g takes half of the 16-byte chunks of each row
+      const int first_row = (warp - 2) * 16;
+#pragma unroll 4
+      for (int c = lane; c < 16 * (D / 8); c += 32) {
+        const int row = first_row + c / (D / 8), ch = c % (D / 8);
+        const int pr = u.pair0 + row;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (pr < u.pairs)
+          v = *reinterpret_cast<const uint4*>(p.q + (int64_t)(u.row0 + pr / p.G) * p.q_row + (int64_t)(walk.head * p.G + pr % p.G) * p.q_head + ch * 8);
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(q_smem + (ch >> 3) * kColBytes + row * 128 + (((ch & 7) ^ (row & 7)) << 4)),
+                     "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_ready);
+      // visible keys of this pair; the unit's rows together see [lo_min, hi_max]
+      const int pr = u.pair0 + r;
+      const bool live = pr < u.pairs;
+      int lo = u.key_lo, hi = u.key_hi - 1;
+      if (live) {
+        const int row = u.row0 + pr / p.G;
+        if (u.base >= 0) {
+          hi = min(hi, u.base + row - u.row0);
+          if (p.window > 0) lo = max(lo, u.base + row - u.row0 - p.window + 1);
+        } else if (p.window > 0) {
+          const int b = find_segment(p.row_start, p.B, row);
+          lo = max(lo, p.cached[b] + row - p.row_start[b] - p.window + 1);
+        }
+      }
+      const bool warp_live = u.pair0 + quarter * 32 < u.pairs;
+      float m = -INFINITY, l = 0.f;
+      for (int j = g; j < n; j += 2, ++turn) {
+        if (!warp_wait(s_full(g), turn & 1, abort_flag)) { ok = false; break; }
+        tc_fence_after();
+        const int c0 = (u.key_lo / kTileB + walk.first + j) * kTileB;
+        if (warp_live) {
+          // The scores are read twice, 32 columns at a time, instead of being held: 128 of them and what the loop needs
+          // do not fit the 168 registers of a 320-thread block.
+          const bool edge = c0 + kTileB - 1 > hi || c0 < lo;
+          auto scores = [&](int c, uint32_t (&x)[32]) {
+            tmem_ld32(s_t + c * 32, x);
+            tmem_ld_wait();
+            if (edge) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) {
+                const int key = c0 + c * 32 + e;
+                if (key > hi || key < lo) x[e] = __float_as_uint(-INFINITY);
+              }
+            }
+          };
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t x[32];
+            scores(c, x);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) mx[e & 3] = fmaxf(mx[e & 3], __uint_as_float(x[e]));
+          }
+          const float m_new = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2);
+          if (__any_sync(0xffffffffu, m_new > m + 8.f)) {
+            const float alpha = m == -INFINITY ? 0.f : exp2f(m - m_new);
+            l *= alpha;
+            if (j >= 2) {
+#pragma unroll 1
+              for (int c = 0; c < D / 32; ++c) {
+                uint32_t o[32];
+                tmem_ld32(o_t + 128 * g + c * 32, o);
+                tmem_ld_wait();
+                uint32_t a[16], b[16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                  a[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+                  b[e] = __float_as_uint(__uint_as_float(o[16 + e]) * alpha);
+                }
+                tmem_st16(o_t + 128 * g + c * 32, a);
+                tmem_st16(o_t + 128 * g + c * 32 + 16, b);
+              }
+            }
+            m = m_new;
+          }
+          const float neg = m == -INFINITY ? 0.f : -m;
+          float ls[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {            // P of 32 keys takes 16 columns, all of scores that were read
+            uint32_t x[32], pk[16];
+            scores(c, x);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const float a = exp2f(fmaf(__uint_as_float(x[2 * e]), p.scale_log2, neg));
+              const float b = exp2f(fmaf(__uint_as_float(x[2 * e + 1]), p.scale_log2, neg));
+              ls[e & 3] += a + b;
+              pk[e] = pack2bf(a, b);
+            }
+            tmem_st16(s_t + c * 16, pk);
+          }
+          l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
+          tmem_st_wait();
+        }
+        // values outside the keys of the unit may be anything, and a zero weight does not silence an infinity
+        if (c0 + kTileB > u.key_hi || c0 < u.key_lo) {
+          const int st = (it + j) % C::kStages;
+          if (!warp_wait(v_full(st), ((it + j) / C::kStages) & 1, abort_flag)) { ok = false; break; }
+          for (int c = r; c < kTileB * (D / 8); c += 128) {
+            const int key = c / (D / 8), ch = c % (D / 8);
+            if (c0 + key >= u.key_hi || c0 + key < u.key_lo)
+              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(v_smem(st) + (ch >> 3) * kColBytes + key * 128 +
+                           (((ch & 7) ^ (key & 7)) << 4)), "r"(0) : "memory");
+          }
+          fence_proxy_async_smem();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_ready(g));
+      }
+      it += n;
+      // ---- join the two warpgroups; each writes half of the columns of every row
+      ok = ok && warp_wait(o_full, piece & 1, abort_flag);
+      ml[(g * kRowsB + r) * 2] = m;
+      ml[(g * kRowsB + r) * 2 + 1] = l;
+      if (softmax_any(!ok)) break;
+      tc_fence_after();
+      const float m0 = ml[r * 2], m1 = n > 1 ? ml[(kRowsB + r) * 2] : -INFINITY;
+      const float mm = fmaxf(m0, m1);
+      const float f0 = m0 == -INFINITY ? 0.f : exp2f(m0 - mm), f1 = m1 == -INFINITY ? 0.f : exp2f(m1 - mm);
+      const float ll = f0 * ml[r * 2 + 1] + f1 * ml[(kRowsB + r) * 2 + 1];
+      const bool whole = walk.count == walk.unit_tiles;
+      const bool last = whole && u.direct;
+      const int64_t rh = live ? (int64_t)(u.row0 + pr / p.G) * p.Hq + walk.head * p.G + pr % p.G : 0;
+      float f = 1.f;
+      if (last) {
+        float den = ll;
+        if (p.sinks != nullptr) {
+          const float sk = p.sinks[rh % p.Hq] * 1.4426950408889634f, top = fmaxf(sk, mm);
+          f = mm == -INFINITY ? 0.f : exp2f(mm - top);
+          den = ll * f + exp2f(sk - top);
+        }
+        f = den > 0.f ? f / den : 0.f;
+      }
+      const int64_t at = whole ? (int64_t)(u.base < 0) * p.R * p.Hq + rh : ((int64_t)blockIdx.x * 2 + (walk.first > 0 ? 0 : 1)) * kRowsB + r;
+      float* dst = (whole ? p.row_o : p.part_b) + at * D;
+      if (!last && live && g == 0) *reinterpret_cast<float2*>((whole ? p.row_ml : p.part_b_ml) + at * 2) = make_float2(mm, ll);
+      if (warp_live) {
+#pragma unroll 1
+        for (int c = 0; c < D / 64; ++c) {
+          const int col = g * (D / 2) + c * 32;
+          uint32_t a[32], b[32];
+          tmem_ld32(o_t + col, a);
+          if (n > 1) tmem_ld32(o_t + 128 + col, b);
+          tmem_ld_wait();
+          float v[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) v[e] = (f0 * __uint_as_float(a[e]) + (n > 1 ? f1 * __uint_as_float(b[e]) : 0.f)) * f;
+          if (live) {
+            if (last) {
+#pragma unroll
+              for (int e = 0; e < 32; e += 8)
+                *reinterpret_cast<uint4*>(p.out + rh * D + col + e) = make_uint4(pack2bf(v[e], v[e + 1]), pack2bf(v[e + 2], v[e + 3]),
+                                                                                pack2bf(v[e + 4], v[e + 5]), pack2bf(v[e + 6], v[e + 7]));
+            } else {
+#pragma unroll
+              for (int e = 0; e < 32; e += 4) *reinterpret_cast<float4*>(dst + col + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+            }
+          }
+        }
+      }
+      tc_fence_before();
+      if (softmax_any(false)) break;             // ml is read before the next piece writes it
+      if (lane == 0) mbar_arrive(o_free);
+      ++piece;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
   if (threadIdx.x == 0 && *abort_flag) atomicOr(p.status, kStatusWaitTimedOut);
 }
 
@@ -766,51 +1183,70 @@ __global__ void __launch_bounds__(256) combine_kernel(const AttnParams p) {
     if (p.zero_tail) store(o, 0.f);
     return;
   }
-  const WorkLayout lay(p.B, p.NG, p.max_units);
+  const WorkLayout lay(p.B, p.NG, p.max_a, p.max_b);
   const int b = find_segment(p.row_start, p.B, r);
   const int g = p.work[lay.seq_group + b];
-  const int* tiles = p.work + lay.tiles;
-  const Unit* units = reinterpret_cast<const Unit*>(p.work + lay.units);
-  const int n_units = p.work[0];
-  const int64_t per = stretch(p.work, p.Hkv, p.ctas);
   const int kvh = h / p.G;
   float m = -INFINITY, l = 0.f;
   if (p.sinks != nullptr) {
     m = p.sinks[h] * 1.4426950408889634f;
     l = 1.f;
   }
-  auto join = [&](const float* po, const float* pml) {
-    const float pm = pml[0], pl = pml[1];
-    if (pm == -INFINITY) return;
-    const float mn = fmaxf(m, pm);
-    const float a = m == -INFINITY ? 0.f : exp2f(m - mn), w = exp2f(pm - mn);
-    m = mn;
-    l = l * a + pl * w;
+  // Joins parts `first`, `first + step`, ... (n of them): lanes fetch the maxima and sums of 32 parts at once, then the
+  // outputs are added four at a time so that their loads overlap.
+  auto join = [&](const float* po, const float* pml, int64_t first, int64_t step, int n) {
+    for (int i0 = 0; i0 < n; i0 += 32) {
+      const int cnt = min(32, n - i0);
+      float pm = -INFINITY, pl = 0.f;
+      if (lane < cnt) {
+        const float2 v = *reinterpret_cast<const float2*>(pml + (first + (int64_t)(i0 + lane) * step) * 2);
+        pm = v.x;
+        pl = v.y;
+      }
+      const float mn = fmaxf(m, warp_max(pm));
+      if (mn == -INFINITY) continue;
+      const float a = m == -INFINITY ? 0.f : exp2f(m - mn);
+      const float w = pm == -INFINITY ? 0.f : exp2f(pm - mn);
+      m = mn;
+      l = l * a + warp_sum(pl * w);
 #pragma unroll
-    for (int i = 0; i < N; ++i) o[i] = o[i] * a + po[lane * N + i] * w;
+      for (int e = 0; e < N; ++e) o[e] *= a;
+#pragma unroll 4
+      for (int i = 0; i < cnt; ++i) {
+        const float wi = __shfl_sync(0xffffffffu, w, i);
+        const float* q = po + (first + (int64_t)(i0 + i) * step) * D + lane * N;
+        if (wi > 0.f) {                          // a part without a visible key may hold anything
+#pragma unroll
+          for (int e = 0; e < N; ++e) o[e] += q[e] * wi;
+        }
+      }
+    }
   };
   // the prefix comes first, then the sequence's own keys: a fixed order
   for (int k = g >= 0 ? 0 : 1; k < 2; ++k) {
     const int s = k == 0 ? p.B + g : b;
-    const int u0 = p.work[lay.src_unit + s];
-    if (u0 < 0) continue;
-    const int row0 = units[min(u0, n_units - 1)].row0;
-    const int pr = (r - row0) * p.G + h % p.G;
-    const int u = u0 + pr / kUnitRows;
-    if (u >= n_units) continue;
-    const int n = tiles[u + 1] - tiles[u];
+    const int ub = p.use_b ? p.work[lay.src_b + s] : -1;
+    const bool big = ub >= 0;
+    const List list = big ? p.list_b(lay) : p.list_a(lay);
+    const int rows = big ? kRowsB : kRowsA;
+    const int u0 = big ? ub : p.work[lay.src_a + s];
+    if (u0 < 0 || u0 >= list.n_units) continue;
+    const int pr = (r - list.units[u0].row0) * p.G + h % p.G;
+    const int u = u0 + pr / rows;
+    if (u >= list.n_units) continue;
+    const int n = list.tiles[u + 1] - list.tiles[u];
     if (n == 0) continue;
-    const int64_t t0 = (int64_t)tiles[u] * p.Hkv + (int64_t)kvh * n, t1 = t0 + n;
-    const int c0 = (int)(t0 / per), c1 = (int)((t1 - 1) / per);
+    const int64_t per = list.stretch(p.Hkv);
+    const int64_t t0 = (int64_t)list.tiles[u] * p.Hkv + (int64_t)kvh * n;
+    const int c0 = (int)(t0 / per), c1 = (int)((t0 + n - 1) / per);
     if (c0 == c1) {
       if (k == 1 && g < 0) return;               // finished by its piece
-      const int64_t at = (int64_t)(k == 0) * p.R * p.Hq + rh;
-      join(p.row_o + at * D, p.row_ml + at * 2);
+      join(p.row_o, p.row_ml, (int64_t)(k == 0) * p.R * p.Hq + rh, 0, 1);
     } else {
-      for (int c = c0; c <= c1; ++c) {
-        const int64_t at = ((int64_t)c * 2 + (c == c0 ? 1 : 0)) * kUnitRows + pr % kUnitRows;
-        join(p.part_o + at * D, p.part_ml + at * 2);
-      }
+      const float* po = big ? p.part_b : p.part_a;
+      const float* pml = big ? p.part_b_ml : p.part_a_ml;
+      join(po, pml, ((int64_t)c0 * 2 + 1) * rows + pr % rows, 0, 1);
+      join(po, pml, (int64_t)(c0 + 1) * 2 * rows + pr % rows, 2 * rows, c1 - c0);
     }
   }
   store(o, l > 0.f ? 1.f / l : 0.f);
@@ -907,10 +1343,10 @@ void paged_write(const at::Tensor& k, const at::Tensor& v, at::Tensor k_pages, a
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
-// Units of a step at most: one per source and one more per kUnitRows pairs; every row belongs to at most two sources.
-static int64_t max_units(int64_t B, int64_t NG, int64_t R, int64_t G) {
-  const int64_t n = B + NG + (NG > 0 ? 2 : 1) * R * G / paged::kUnitRows + 1;
-  TORCH_CHECK(n < (1 << 28), "paged attention: too many rows");
+// Units of a step at most: one per source and one more per so many pairs; every row belongs to at most two sources.
+static int64_t max_units(int64_t B, int64_t NG, int64_t R, int64_t G, int64_t rows) {
+  const int64_t n = B + NG + (NG > 0 ? 2 : 1) * R * G / rows + 1;
+  TORCH_CHECK(n < (1 << 26), "paged attention: too many rows");
   return n;
 }
 
@@ -938,8 +1374,9 @@ at::Tensor paged_work(const at::Tensor& cached, const at::Tensor& row_start, con
   }
   p.B = (int)B; p.NG = (int)NG; p.W = (int)table_cols; p.ps = (int)page_size;
   p.G = (int)(hq / hkv); p.window = (int)window;
-  p.max_units = (int)max_units(B, NG, total_rows, p.G);
-  auto work = at::empty({paged::WorkLayout(B, NG, p.max_units).size}, cached.options());
+  p.max_a = (int)max_units(B, NG, total_rows, p.G, paged::kRowsA);
+  p.max_b = (int)max_units(B, NG, total_rows, p.G, paged::kRowsB);
+  auto work = at::empty({paged::WorkLayout(B, NG, p.max_a, p.max_b).size}, cached.options());
   p.work = work.data_ptr<int>();
   p.status = status_word_ptr();
   const int smem = (int)(sizeof(int) * (B + NG + 1 + 2 * NG));
@@ -955,7 +1392,7 @@ static CUtensorMap page_map(const at::Tensor& t) {
   const uint64_t e = 2;
   const cuuint64_t dims[4] = {(cuuint64_t)t.size(3), (cuuint64_t)t.size(2), (cuuint64_t)t.size(1), (cuuint64_t)t.size(0)};
   const cuuint64_t strides[3] = {(cuuint64_t)t.stride(2) * e, (cuuint64_t)t.stride(1) * e, (cuuint64_t)t.stride(0) * e};
-  const cuuint32_t box[4] = {64, (cuuint32_t)std::min<int64_t>(t.size(2), paged::kTile), 1, 1};
+  const cuuint32_t box[4] = {64, (cuuint32_t)std::min<int64_t>(t.size(2), 64), 1, 1};
   const cuuint32_t elem[4] = {1, 1, 1, 1};
   const CUresult r = cuTensorMapEncodeTiled(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, t.data_ptr(), dims, strides, box, elem,
                                             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
@@ -965,8 +1402,8 @@ static CUtensorMap page_map(const at::Tensor& t) {
 }
 
 void paged_attention(const at::Tensor& q, const at::Tensor& k_pages, const at::Tensor& v_pages, const at::Tensor& table,
-                     const at::Tensor& cached, const at::Tensor& row_start, const at::Tensor& work, int64_t groups, double scale,
-                     int64_t window, const c10::optional<at::Tensor>& sinks, at::Tensor out, bool zero_tail) {
+                     const at::Tensor& cached, const at::Tensor& row_start, const at::Tensor& work, int64_t groups, int64_t max_rows,
+                     double scale, int64_t window, const c10::optional<at::Tensor>& sinks, at::Tensor out, bool zero_tail) {
   check_pages(k_pages, v_pages, "paged_attention");
   const auto dev = k_pages.device();
   const int64_t R = q.size(0), D = k_pages.size(3), ps = k_pages.size(2);
@@ -994,30 +1431,46 @@ void paged_attention(const at::Tensor& q, const at::Tensor& k_pages, const at::T
   p.table = table.data_ptr<int>();
   p.cached = int_vector(cached, B, dev, "cached");
   p.row_start = int_vector(row_start, B + 1, dev, "row_start");
-  p.B = (int)B; p.NG = (int)groups; p.S = (int)table.size(0); p.W = (int)table.size(1); p.R = (int)R;
+  p.B = (int)B; p.NG = (int)groups; p.W = (int)table.size(1); p.R = (int)R;
   p.Hq = (int)q.size(1); p.Hkv = (int)k_pages.size(1); p.G = p.Hq / p.Hkv; p.ps = (int)ps; p.num_pages = (int)k_pages.size(0);
   p.window = (int)window; p.scale_log2 = (float)(scale * 1.4426950408889634); p.zero_tail = zero_tail;
-  p.max_units = (int)max_units(B, groups, R, p.G);
-  p.ctas = num_sms() * (D == 256 ? paged::Cfg<256>::kCtasPerSm : paged::Cfg<128>::kCtasPerSm);
-  p.work = int_vector(work, paged::WorkLayout(B, groups, p.max_units).size, dev, "work (made for other heads, rows or groups?)");
+  p.max_a = (int)max_units(B, groups, R, p.G, paged::kRowsA);
+  p.max_b = (int)max_units(B, groups, R, p.G, paged::kRowsB);
+  p.work = int_vector(work, paged::WorkLayout(B, groups, p.max_a, p.max_b).size, dev, "work (made for other heads, rows or groups?)");
   p.status = status_word_ptr();
+  // 256-wide heads would need more tensor memory than there is for two accumulators: they stay on the first kernel.
+  p.use_b = D <= 128 && max_rows * p.G > paged::kFewPairs;
+  p.ctas_a = num_sms() * (D == 256 ? paged::Cfg<256>::kCtasPerSm : paged::Cfg<128>::kCtasPerSm);
+  p.ctas_b = num_sms();
+  if (p.use_b)
+    TORCH_CHECK(q.stride(0) % 8 == 0 && q.stride(1) % 8 == 0 && reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0 &&
+                    reinterpret_cast<uintptr_t>(out.data_ptr()) % 16 == 0,
+                "paged_attention: query and output vectors must be 16-byte aligned");
   const auto f32 = q.options().dtype(at::kFloat);
-  auto part = at::empty({(int64_t)p.ctas * 2 * paged::kUnitRows, D + 2}, f32);
-  p.part_o = part.data_ptr<float>();
-  p.part_ml = p.part_o + (int64_t)p.ctas * 2 * paged::kUnitRows * D;
-  at::Tensor rows;
-  if (groups > 0) {
-    rows = at::empty({2 * R * p.Hq, D + 2}, f32);
-    p.row_o = rows.data_ptr<float>();
-    p.row_ml = p.row_o + 2 * R * p.Hq * D;
-  }
+  const int64_t na = (int64_t)p.ctas_a * 2 * paged::kRowsA, nb = p.use_b ? (int64_t)p.ctas_b * 2 * paged::kRowsB : 0;
+  const int64_t nr = groups > 0 ? 2 * R * p.Hq : 0;
+  auto scratch = at::empty({(na + nb + nr) * (D + 2)}, f32);
+  p.part_a = scratch.data_ptr<float>();
+  p.part_b = p.part_a + na * D;
+  p.row_o = p.part_b + nb * D;
+  p.part_a_ml = p.row_o + nr * D;
+  p.part_b_ml = p.part_a_ml + na * 2;
+  p.row_ml = p.part_b_ml + nb * 2;
   const CUtensorMap mk = page_map(k_pages), mv = page_map(v_pages);
   auto stream = at::cuda::getCurrentCUDAStream();
   auto launch = [&](auto dim) {
     constexpr int kD = decltype(dim)::value;
     auto kernel = paged::attn_rows_kernel<kD>;
     C10_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, paged::Cfg<kD>::kSmem));
-    kernel<<<p.ctas, 160, paged::Cfg<kD>::kSmem, stream>>>(mk, mv, p);
+    if constexpr (kD <= 128) {
+      if (p.use_b) {
+        auto block = paged::attn_block_kernel<kD>;
+        C10_CUDA_CHECK(cudaFuncSetAttribute(block, cudaFuncAttributeMaxDynamicSharedMemorySize, paged::CfgB<kD>::kSmem));
+        block<<<p.ctas_b, 320, paged::CfgB<kD>::kSmem, stream>>>(mk, mv, p);
+        C10_CUDA_KERNEL_LAUNCH_CHECK();
+      }
+    }
+    kernel<<<p.ctas_a, 160, paged::Cfg<kD>::kSmem, stream>>>(mk, mv, p);
     C10_CUDA_KERNEL_LAUNCH_CHECK();
     paged::combine_kernel<kD><<<(unsigned)((R * p.Hq + 7) / 8), 256, 0, stream>>>(p);
     C10_CUDA_KERNEL_LAUNCH_CHECK();

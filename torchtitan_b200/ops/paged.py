@@ -44,6 +44,7 @@ class PagePlan:
     total_rows: int
     heads: tuple[int, int] | None = None                                 # (query, key heads) of the attention work lists
     groups: int = 0
+    max_rows: int = 0                                                    # of one sequence or group
     work: dict[int, torch.Tensor] = field(default_factory=dict)          # by window
 
 
@@ -79,6 +80,7 @@ def page_plan(cached: torch.Tensor, new: torch.Tensor, block_table: torch.Tensor
         if not n_kv_heads or n_heads % n_kv_heads:
             raise ValueError(f"page_plan: {n_heads} query heads on {n_kv_heads} key heads")
         plan.heads, plan.groups = (int(n_heads), int(n_kv_heads)), 0 if group_prefix is None else group_prefix.numel()
+        plan.max_rows = int(total_rows) if max_rows is None else min(int(max_rows), int(total_rows))
         if block_table.is_cuda:
             for w in dict.fromkeys(int(w or 0) for w in windows):
                 _count()
@@ -131,7 +133,7 @@ def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pla
                          f"{plan.heads} and windows {tuple(plan.work)}")
     _count(2)
     dst = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
-    ext.require().paged_attention(q if q.stride(2) == 1 and not (q.stride(0) | q.stride(1)) % 2 and q.data_ptr() % 4 == 0 else q.clone(
-        memory_format=torch.contiguous_format), k_pages, v_pages, plan.block_table, plan.cached, plan.row_start, plan.work[int(window)],
-        plan.groups, float(scale), int(window), None if sinks is None else sinks.float().contiguous(), dst, out is None)
+    ext.require().paged_attention(_vectors(q), k_pages, v_pages, plan.block_table, plan.cached, plan.row_start, plan.work[int(window)],
+                                  plan.groups, plan.max_rows, float(scale), int(window),
+                                  None if sinks is None else sinks.float().contiguous(), dst, out is None)
     return dst
