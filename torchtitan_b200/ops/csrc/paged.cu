@@ -59,6 +59,21 @@ __device__ __forceinline__ int find_segment(const int* start, int n, int x) {
   return lo;
 }
 
+// The same by a whole warp: 32 probes at a time, so one round of dependent loads per factor of 32.
+__device__ __forceinline__ int find_segment_warp(const int* start, int n, int x) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 31) / 32;
+    const int at = lo + lane * step;
+    const unsigned below = __ballot_sync(0xffffffffu, at < hi && start[at] <= x);
+    const int k = 31 - __clz((int)below);        // lane 0 is always below
+    lo += k * step;
+    hi = min(hi, lo + step);
+  }
+  return lo;
+}
+
 struct PlanParams {
   const int *cached, *fresh, *slots, *pages, *mapped;   // [B], [B], [B], [F], [B] or null
   int* table;                                           // [S, W]
@@ -195,11 +210,11 @@ __global__ void __launch_bounds__(256) write_kernel(const WriteParams p) {
 // behind, at most two per CTA (the first and the last of a stretch), which the combine kernel joins in the order of the
 // line, so results do not depend on scheduling.  A group's two sources are joined there as well.
 //
-// There are two lists with a line each: units of 16 pairs and 64-key tiles for the kernel on mma.sync, units of 128 pairs
-// and 128-key tiles for the one on tcgen05.  A source of more than kFewPairs pairs is *large*: it is in both lists, behind
+// There are two lists with a line each: units of 16 pairs and 64-key tiles for the kernel on mma.sync, units of up to 128
+// pairs (whole rows) and 64-key tiles for the one on tcgen05.  A source of more than kFewPairs pairs is *large*: it is in both lists, behind
 // the small ones in the first, and runs from the second where that kernel is launched.
 constexpr int kRowsA = 16, kTileA = 64;
-constexpr int kRowsB = 128, kTileB = 128;
+constexpr int kRowsB = 128, kTileB = 64;
 constexpr int kFewPairs = 16;
 
 struct __align__(16) Unit {
@@ -209,11 +224,13 @@ struct __align__(16) Unit {
 
 // Layout of the int32 work buffer (one per window), from the sizes that the host knows.
 struct WorkLayout {
-  int64_t seq_group, src_a, src_b, tiles_a, tiles_b, units_a, units_b, size;
+  int64_t seq_group, shared, group_row, src_a, src_b, tiles_a, tiles_b, units_a, units_b, size;
   // header: [0, 1] units and tiles (of one key head) of the small sources in list A, [2, 3] of all, [4, 5] of list B
   __host__ __device__ WorkLayout(int64_t B, int64_t NG, int64_t max_a, int64_t max_b) {
     seq_group = 8;
-    src_a = seq_group + B;                       // first unit of each source, -1 = none
+    shared = seq_group + B;                      // rows of the groups that share, as running counts
+    group_row = shared + NG + 1;                 // first row of each group
+    src_a = group_row + NG;                      // first unit of each source, -1 = none
     src_b = src_a + B + NG;
     tiles_a = src_b + B + NG;                    // running tile counts
     tiles_b = tiles_a + max_a + 1;
@@ -225,7 +242,7 @@ struct WorkLayout {
 
 struct WorkParams {
   const int *cached, *row_start, *slots, *group_start, *group_prefix;
-  int B, NG, W, ps, G, window, max_a, max_b;
+  int B, NG, W, ps, G, window, max_a, max_b, rows_b;   // rows_b: token rows of a unit in list B
   int* work;
   int* status;
 };
@@ -263,6 +280,24 @@ __global__ void __launch_bounds__(1024) work_kernel(const WorkParams p) {
       for (int b = a + lane; b < e; b += 32) seq_group[b] = g;
   }
   __syncthreads();
+  {
+    int* shared = p.work + lay.shared;           // running row counts of the groups that share a prefix
+    int rows = 0;
+    for (int g0 = 0; g0 < p.NG; g0 += blockDim.x) {
+      const int g = g0 + threadIdx.x;
+      int n = 0;
+      if (g < p.NG) {
+        const int r0 = p.row_start[min(max(p.group_start[g], 0), p.B)];
+        if (prefix[g] > 0) n = max(0, p.row_start[min(max(p.group_start[g + 1], 0), p.B)] - r0);
+        p.work[lay.group_row + g] = r0;
+      }
+      int total;
+      const int e = block_scan(n, part, total);
+      if (g < p.NG) shared[g] = rows + e - n;
+      rows += total;
+    }
+    if (threadIdx.x == 0) shared[p.NG] = rows;
+  }
   auto source_rows = [&](int s, int& r0, int& r1) {
     if (s < p.B) {
       r0 = p.row_start[s];
@@ -276,6 +311,8 @@ __global__ void __launch_bounds__(1024) work_kernel(const WorkParams p) {
       }
     }
   };
+  int *src_a = p.work + lay.src_a, *src_b = p.work + lay.src_b, *tiles_a = p.work + lay.tiles_a, *tiles_b = p.work + lay.tiles_b;
+  Unit *units_a = reinterpret_cast<Unit*>(p.work + lay.units_a), *units_b = reinterpret_cast<Unit*>(p.work + lay.units_b);
   // Appends the units of the small or the large sources to a list that has `n0` units and `t0` tiles already.
   auto list = [&](bool large, int rows, int tile, int max_units, int* src, int* tiles, Unit* units, int& n0, int& t0) {
     int n_units = 0;
@@ -295,7 +332,7 @@ __global__ void __launch_bounds__(1024) work_kernel(const WorkParams p) {
       if (s < n_src) {
         start[s] = n_units + e - n;
         if (mine) src[s] = n > 0 ? n0 + n_units + e - n : -1;
-        else if (large && rows == kRowsB) src[s] = -1;
+        else if (src == src_b) src[s] = -1;
       }
       n_units += total;
     }
@@ -358,14 +395,12 @@ __global__ void __launch_bounds__(1024) work_kernel(const WorkParams p) {
     __syncthreads();
   };
   int n = 0, t = 0;
-  int *src_a = p.work + lay.src_a, *src_b = p.work + lay.src_b, *tiles_a = p.work + lay.tiles_a, *tiles_b = p.work + lay.tiles_b;
-  Unit *units_a = reinterpret_cast<Unit*>(p.work + lay.units_a), *units_b = reinterpret_cast<Unit*>(p.work + lay.units_b);
   list(false, kRowsA, kTileA, p.max_a, src_a, tiles_a, units_a, n, t);
   if (threadIdx.x == 0) { p.work[0] = n; p.work[1] = t; }
   list(true, kRowsA, kTileA, p.max_a, src_a, tiles_a, units_a, n, t);
   if (threadIdx.x == 0) { p.work[2] = n; p.work[3] = t; }
   n = t = 0;
-  list(true, kRowsB, kTileB, p.max_b, src_b, tiles_b, units_b, n, t);
+  if (p.rows_b > 0) list(true, p.rows_b * p.G, kTileB, p.max_b, src_b, tiles_b, units_b, n, t);
   if (threadIdx.x == 0) { p.work[4] = n; p.work[5] = t; }
   if (bad) atomicOr(p.status, kStatusPagePlanInvalid);
 }
@@ -385,7 +420,7 @@ struct AttnParams {
   __nv_bfloat16* out;                            // [R, Hq, D]
   const float* sinks;                            // [Hq] or null
   const int *table, *cached, *row_start, *work;
-  int B, NG, W, R, Hq, Hkv, G, ps, num_pages, window, max_a, max_b, ctas_a, ctas_b;
+  int B, NG, W, R, Hq, Hkv, G, ps, num_pages, window, max_a, max_b, ctas_a, ctas_b, rows_b, ps_shift;
   float scale_log2;
   bool zero_tail, use_b;                         // use_b: large sources run on the tcgen05 kernel
   float *part_a, *part_a_ml;                     // [ctas_a, 2, kRowsA, D], [ctas_a, 2, kRowsA, 2]: pieces
@@ -434,12 +469,17 @@ __device__ __forceinline__ bool consumer_any(bool v) {
                : "=r"(r) : "r"((uint32_t)v) : "memory");
   return r != 0;
 }
-__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2, int c3) {
+__device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2, int c3, int c4) {
   asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
-      ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
+      ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4)
       : "memory");
 }
+
+// Programmatic launches.  The three kernels of a call are chained: each lets the next one start while it runs, and a
+// kernel that needs what came before waits for it here (all memory of the earlier grids is visible then).
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_earlier() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // A bounded wait whose outcome is the same for all lanes, so that a warp leaves as one.
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
@@ -465,7 +505,7 @@ struct Walk {
     const int64_t line = (int64_t)l.n_tiles * Hkv, per = l.stretch(Hkv);
     at = min(line, cta * per);
     end = min(line, at + per);
-    u = at < end ? find_segment(tiles, l.n_units, (int)(at / Hkv)) : 0;
+    u = at < end ? find_segment_warp(tiles, l.n_units, (int)(at / Hkv)) : 0;
   }
   __device__ __forceinline__ bool next() {
     if (at >= end) return false;
@@ -499,6 +539,7 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
   auto full = [&](int s) { return bars + 16u * s; };
   auto empty = [&](int s) { return bars + 16u * s + 8u; };
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  let_next_start();
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kStages; ++s) {
       mbar_init(full(s), 1);
@@ -515,8 +556,8 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
   if (warp == 4) {
     // ---------------------------------------------------------------------------------------------------- producer
     const int box = min(p.ps, kTileA), subs = kTileA / box;
-    const int loads = 2 * (D / 64) * subs;       // at most 2 * 4 * 4 = 32: one lane each
-    const int kv = lane / ((D / 64) * subs), col = (lane / subs) % (D / 64), sub = lane % subs;
+    const int loads = 2 * subs;                  // at most 8: one lane each
+    const int kv = lane / subs, sub = lane % subs;
     const CUtensorMap* map = kv ? &tmap_v : &tmap_k;
     bool ok = true;
     while (ok && walk.next()) {
@@ -524,17 +565,17 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
       const int* row = p.table + (int64_t)u.slot * p.W;
       const int t0 = u.key_lo / kTileA + walk.first;
       auto entry = [&](int t) {                  // page of this lane's box of tile t, -1 when no key of it is needed
-        const int64_t key = (int64_t)t * kTileA + sub * box;
-        return lane < loads && key < u.key_hi ? row[key / p.ps] : INT_MIN;
+        const int key = t * kTileA + sub * box;
+        return lane < loads && key < u.key_hi ? row[key >> p.ps_shift] : INT_MIN;
       };
-      int page = entry(t0);
+      int page = entry(t0), page1 = walk.count > 1 ? entry(t0 + 1) : INT_MIN;
       for (int i = 0; i < walk.count; ++i, ++it) {
         const int st = it % C::kStages;
         const int t = t0 + i;
-        const int after = i + 1 < walk.count ? entry(t + 1) : INT_MIN;
+        const int page2 = i + 2 < walk.count ? entry(t + 2) : INT_MIN;      // fetched two tiles ahead
         if (!warp_wait(empty(st), ((it / C::kStages) & 1) ^ 1, abort_flag)) { ok = false; break; }
         const int need = __popc(__ballot_sync(0xffffffffu, page != INT_MIN));
-        if (lane == 0) mbar_expect_tx(full(st), need * box * 128);
+        if (lane == 0) mbar_expect_tx(full(st), need * box * D * 2);
         __syncwarp();
         if (page != INT_MIN) {
           if (page < 0 || page >= p.num_pages) {  // out of range: the load fills zeros
@@ -542,16 +583,19 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
             page = p.num_pages;
           }
           const int key = t * kTileA + sub * box;
-          tma_load_4d(base + st * C::kStageBytes + kv * C::kHalfBytes + col * (kTileA * 128) + sub * box * 128, map, full(st),
-                      col * 64, key % p.ps, walk.head, page);
+          tma_load_5d(base + st * C::kStageBytes + kv * C::kHalfBytes + sub * box * D * 2, map, full(st), 0, key & (p.ps - 1), 0, walk.head, page);
         }
-        page = after;
+        page = page1;
+        page1 = page2;
       }
     }
     if (!ok) drain(it, C::kStages, full);
   } else {
     // ---------------------------------------------------------------------------------------------------- consumers
     const int quad = lane & 3, r_lo = lane >> 2;                         // this thread's rows: r_lo and r_lo + 8
+    // a page's box is [64-column block][key][128 bytes]; this warp's 16 keys lie in one box
+    const int box = min(p.ps, kTileA);
+    const uint32_t block = box * 128, mine = (warp * 16) / box * (box * D * 2) + (warp * 16) % box * 128;
     bool ok = true;
     while (ok && walk.next()) {
       const Unit u = list.units[walk.u];
@@ -603,7 +647,6 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
         if (!warp_wait(full(st), (it / C::kStages) & 1, abort_flag)) { ok = false; break; }
         const uint32_t ks = base + st * C::kStageBytes, vs = ks + C::kHalfBytes;
         const int k0 = (t0 + i) * kTileA + warp * 16;                     // this warp's first key
-        const int kr = warp * 16;
         if (k0 <= hi_max && k0 + 15 >= lo_min) {
           // S = Q K^T
           float s[2][4];
@@ -612,13 +655,13 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
 #pragma unroll
             for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
           {
-            const int key = kr + ((lane >> 4) << 3) + (lane & 7);
-            const uint32_t rowa = ks + key * 128;
+            const int key = ((lane >> 4) << 3) + (lane & 7);
+            const uint32_t rowa = ks + mine + key * 128;
 #pragma unroll
             for (int k = 0; k < D / 16; ++k) {
               const int chunk = (k & 3) * 2 + ((lane >> 3) & 1);
               uint32_t b[4];
-              ldmatrix4(rowa + (k >> 2) * (kTileA * 128) + ((chunk ^ (key & 7)) << 4), b);
+              ldmatrix4(rowa + (k >> 2) * block + ((chunk ^ (key & 7)) << 4), b);
               mma16816(s[0], qf[k], b[0], b[1]);
               mma16816(s[1], qf[k], b[2], b[3]);
             }
@@ -637,8 +680,8 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
               for (int c = lane; c < 16 * (D / 8); c += 32) {
                 const int key = c / (D / 8), ch = c % (D / 8);
                 if (k0 + key > hi_max || k0 + key < lo_min)
-                  asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(vs + (ch >> 3) * (kTileA * 128) + (kr + key) * 128 +
-                               (((ch & 7) ^ ((kr + key) & 7)) << 4)), "r"(0) : "memory");
+                  asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(vs + mine + (ch >> 3) * block + key * 128 + (((ch & 7) ^ (key & 7)) << 4)),
+                               "r"(0) : "memory");
               }
               fence_proxy_async_smem();
               __syncwarp();
@@ -679,13 +722,13 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
           }
           // O += P V
           {
-            const int key = kr + (((lane >> 3) & 1) << 3) + (lane & 7);
-            const uint32_t rowa = vs + key * 128;
+            const int key = (((lane >> 3) & 1) << 3) + (lane & 7);
+            const uint32_t rowa = vs + mine + key * 128;
 #pragma unroll
             for (int n = 0; n < D / 16; ++n) {
               const int chunk = (n & 3) * 2 + (lane >> 4);
               uint32_t b[4];
-              ldmatrix4_t(rowa + (n >> 2) * (kTileA * 128) + ((chunk ^ (key & 7)) << 4), b);
+              ldmatrix4_t(rowa + (n >> 2) * block + ((chunk ^ (key & 7)) << 4), b);
               mma16816(o[2 * n], pf, b[0], b[1]);
               mma16816(o[2 * n + 1], pf, b[2], b[3]);
             }
@@ -783,29 +826,51 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
       consumer_sync();
     }
   }
+  wait_for_earlier();                            // the tcgen05 kernel runs at the same time; what follows needs both
   __syncthreads();
   if (threadIdx.x == 0 && *abort_flag) atomicOr(p.status, kStatusWaitTimedOut);
 }
 
 // Many rows behind one key range (a prefix with the rows of its group, the rows of a prompt chunk): tcgen05.
 //
-// A unit is 128 pairs, one TMEM lane each; tiles of 128 keys alternate between two softmax warpgroups, which keep their own
-// running maximum, sum and output accumulator, so neither waits for the other and the softmax of one tile runs under the
-// MMAs of the next.  Per tile: S = Q K^T into tensor memory, P = exp2(S - m) written over S as bf16, O += P V with P read
-// from tensor memory.  An S is issued behind the P V of the same warpgroup's previous tile, so "S is there" also says that
-// the accumulator may be rescaled.  Bound by the exponentials (128 x 128 per tile on a 16-per-clock unit are 1024 clocks, as
-// many as the MMAs take) when many units share their keys through L2, by HBM when each key range has one unit.
+// A unit is up to 128 pairs (whole rows), one TMEM lane each; 64-key tiles alternate between two softmax warpgroups, which
+// keep their own running maximum, sum and output accumulator, so neither waits for the other, and each has two score
+// buffers, so that the softmax of one tile runs under the MMAs of the next.  Per tile: S = Q K^T into tensor memory,
+// P = exp2(S - m) written over S as bf16, O += P V with P read from tensor memory.  Behind every P V the issuer puts the S
+// of the tile four later, into the same buffer, and a commit (a bare one at the end), so "the next S of a buffer is there"
+// also says that its P V is done: a warpgroup that has to rescale its accumulator waits for that of its other buffer.
+// Queries come by TMA too (boxes of rows x heads of the key head), the next piece's while the present one runs.
+// Bound by the exponentials (64 x 128 per tile on a 16-per-clock unit are 512 clocks, as many as the MMAs take) when many
+// units share their keys through L2, by HBM when each key range has one unit.
 //   warp 0: TMA producer    warp 1: TMEM, MMA issue    warps 2..5, 6..9: softmax of even / odd tiles, then the output
-// Tensor memory: S of warpgroup g at column 128 g, O at 256 + 128 g.
+// Tensor memory: score buffer b (of warpgroup b % 2) at column 64 b, accumulator of warpgroup g at 256 + 128 g.
 template <int D>
 struct CfgB {
-  static constexpr int kStages = 3;
-  static constexpr uint32_t kTileBytes = kTileB * D * 2;         // keys (or values) of a tile, or the queries of a unit
-  static constexpr uint32_t kBars = kTileBytes * (1 + 2 * kStages);
-  static constexpr int kNumBars = 4 * kStages + 7;
+  static constexpr int kStages = D == 64 ? 8 : 4;                // tiles of keys and of values in flight
+  static constexpr uint32_t kQBytes = kRowsB * D * 2;
+  static constexpr uint32_t kTileBytes = kTileB * D * 2;
+  static constexpr uint32_t kStage = 2 * kQBytes + 2 * kStages * kTileBytes;     // fp32 rows on their way out, 2 KB a warp
+  static constexpr uint32_t kBars = kStage + 8 * 2048;
+  static constexpr int kNumBars = 4 * kStages + 14;
   static constexpr uint32_t kMl = kBars + 8 * kNumBars + 8;      // TMEM address, abort flag
   static constexpr uint32_t kSmem = kMl + 2 * kRowsB * 2 * 4;
 };
+
+// tcgen05 with the elected lane as a predicate instead of a branch.
+__device__ __forceinline__ void mma_ss(uint32_t elected, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+               "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+               ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(elected) : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t elected, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+               "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+               ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(elected) : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint32_t elected, uint32_t bar) {
+  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+               "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(elected) : "memory");
+}
 
 // Named barrier of the eight softmax warps; true for all when any thread brings true.
 __device__ __forceinline__ bool softmax_any(bool v) {
@@ -814,34 +879,54 @@ __device__ __forceinline__ bool softmax_any(bool v) {
                : "=r"(r) : "r"((uint32_t)v) : "memory");
   return r != 0;
 }
+__device__ __forceinline__ uint64_t pack_f2(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpack_f2(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma_f2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add_f2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
 
 template <int D>
 __global__ void __launch_bounds__(320, 1)
-attn_block_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const AttnParams p) {
+attn_block_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
+                  const __grid_constant__ CUtensorMap tmap_v, const AttnParams p) {
   using C = CfgB<D>;
   using namespace tc;
-  constexpr uint32_t kColBytes = kTileB * 128;                   // one 64-column block of a tile
+  constexpr uint32_t kQCol = kRowsB * 128, kCol = kTileB * 128;   // one 64-column block of the queries, of a tile
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t base = smem_u32(smem);
-  const uint32_t q_smem = base;
-  auto k_smem = [&](int s) { return base + C::kTileBytes * (1 + 2 * s); };
-  auto v_smem = [&](int s) { return base + C::kTileBytes * (2 + 2 * s); };
+  auto q_smem = [&](int i) { return base + C::kQBytes * i; };
+  auto k_smem = [&](int s) { return base + 2 * C::kQBytes + C::kTileBytes * (2 * s); };
+  auto v_smem = [&](int s) { return base + 2 * C::kQBytes + C::kTileBytes * (2 * s + 1); };
   const uint32_t bars = base + C::kBars;
   auto k_full = [&](int s) { return bars + 8u * s; };
   auto k_empty = [&](int s) { return bars + 8u * (C::kStages + s); };
   auto v_full = [&](int s) { return bars + 8u * (2 * C::kStages + s); };
   auto v_empty = [&](int s) { return bars + 8u * (3 * C::kStages + s); };
-  auto s_full = [&](int g) { return bars + 8u * (4 * C::kStages + g); };
-  auto p_ready = [&](int g) { return bars + 8u * (4 * C::kStages + 2 + g); };
-  const uint32_t o_full = bars + 8u * (4 * C::kStages + 4), q_ready = o_full + 8u, o_free = o_full + 16u;
+  auto s_full = [&](int b) { return bars + 8u * (4 * C::kStages + b); };
+  auto p_ready = [&](int b) { return bars + 8u * (4 * C::kStages + 4 + b); };
+  auto q_full = [&](int i) { return bars + 8u * (4 * C::kStages + 8 + i); };
+  auto q_empty = [&](int i) { return bars + 8u * (4 * C::kStages + 10 + i); };
+  const uint32_t o_full = bars + 8u * (4 * C::kStages + 12), o_free = o_full + 8u;
   uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(smem + C::kBars + 8 * C::kNumBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_ptr + 1);
-  float* ml = reinterpret_cast<float*>(smem + C::kMl);           // [2][kRowsB][2]
+  float* ml = reinterpret_cast<float*>(smem + C::kMl);            // [2][kRowsB][2]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
+  let_next_start();
   const List list = p.list_b(WorkLayout(p.B, p.NG, p.max_a, p.max_b));
   Walk walk(list, p.Hkv, blockIdx.x);
-  if (walk.at >= walk.end) return;                               // the same for the whole block
+  if (walk.at >= walk.end) return;                                // the same for the whole block
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kStages; ++s) {
@@ -850,12 +935,15 @@ attn_block_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
       mbar_init(v_full(s), 1);
       mbar_init(v_empty(s), 1);
     }
-    for (int g = 0; g < 2; ++g) {
-      mbar_init(s_full(g), 1);
-      mbar_init(p_ready(g), 4);
+    for (int b = 0; b < 4; ++b) {
+      mbar_init(s_full(b), 1);
+      mbar_init(p_ready(b), 4);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(q_full(i), 1);
+      mbar_init(q_empty(i), 1);
     }
     mbar_init(o_full, 1);
-    mbar_init(q_ready, 8);
     mbar_init(o_free, 8);
     *abort_flag = 0;
     mbar_fence_init();
@@ -871,136 +959,130 @@ attn_block_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
 
   if (warp == 0) {
     // ---------------------------------------------------------------------------------------------------- producer
-    const int box = min(p.ps, 64), subs = kTileB / box;
-    const int loads = (D / 64) * subs;           // at most 2 * 8 = 16 per operand: lanes 0..15 keys, 16..31 values
+    const int box = min(p.ps, kTileB), subs = kTileB / box;
+    // A tile is [64-column block][key][128 bytes]: one box where a page holds the whole tile, else one per page and block
+    const int loads = subs == 1 ? 1 : (D / 64) * subs;            // at most 2 * 4 per operand: lanes 0..15 keys, 16..31 values
+    const uint32_t bytes = box * 128 * (subs == 1 ? D / 64 : 1);
     const int kv = lane >> 4, li = lane & 15, col = li / subs, sub = li % subs;
     const CUtensorMap* map = kv ? &tmap_v : &tmap_k;
+    const uint32_t q_bytes = (uint32_t)(p.rows_b * p.G) * D * 2;   // a whole box: rows behind the tensor are filled with zeros
     bool ok = true;
-    int it = 0, issued_k = 0, issued_v = 0;
+    int it = 0, piece = 0, issued_k = 0, issued_v = 0, issued_q = 0;
     while (ok && walk.next()) {
       const Unit u = list.units[walk.u];
       const int* row = p.table + (int64_t)u.slot * p.W;
       const int t0 = u.key_lo / kTileB + walk.first;
       auto entry = [&](int t) {
-        const int64_t key = (int64_t)t * kTileB + sub * box;
-        return li < loads && key < u.key_hi ? row[key / p.ps] : INT_MIN;
+        const int key = t * kTileB + sub * box;
+        return li < loads && key < u.key_hi ? row[key >> p.ps_shift] : INT_MIN;
       };
-      int page = entry(t0);
+      int page = entry(t0), page1 = walk.count > 1 ? entry(t0 + 1) : INT_MIN;
+      if (!warp_wait(q_empty(piece & 1), ((piece >> 1) & 1) ^ 1, abort_flag)) break;
+      if (lane == 0) {
+        mbar_expect_tx(q_full(piece & 1), q_bytes);
+        for (int c = 0; c < D / 64; ++c)
+          tma_load_3d(q_smem(piece & 1) + c * kQCol, &tmap_q, q_full(piece & 1), c * 64, walk.head * p.G, u.row0 + u.pair0 / p.G);
+      }
+      issued_q = ++piece;
       for (int i = 0; i < walk.count; ++i, ++it) {
         const int st = it % C::kStages;
         const uint32_t parity = ((it / C::kStages) & 1) ^ 1;
         const int t = t0 + i;
-        const int after = i + 1 < walk.count ? entry(t + 1) : INT_MIN;
+        const int page2 = i + 2 < walk.count ? entry(t + 2) : INT_MIN;      // fetched two tiles ahead
         const bool wanted = page != INT_MIN;
         const int need = __popc(__ballot_sync(0xffffffffu, wanted) & 0xffffu);
         if (wanted && (page < 0 || page >= p.num_pages)) {        // out of range: the load fills zeros
           atomicOr(p.status, kStatusPagePlanInvalid);
           page = p.num_pages;
         }
-        const int slot = (int)(((int64_t)t * kTileB + sub * box) % p.ps);
-        const uint32_t off = col * kColBytes + sub * box * 128;
+        const int slot = (t * kTileB + sub * box) & (p.ps - 1);
+        const uint32_t off = col * kCol + sub * box * 128;
         if (!warp_wait(k_empty(st), parity, abort_flag)) { ok = false; break; }
-        if (lane == 0) mbar_expect_tx(k_full(st), need * box * 128);
+        if (lane == 0) mbar_expect_tx(k_full(st), need * bytes);
         __syncwarp();
-        if (wanted && kv == 0) tma_load_4d(k_smem(st) + off, map, k_full(st), col * 64, slot, walk.head, page);
+        if (wanted && kv == 0) tma_load_5d(k_smem(st) + off, map, k_full(st), 0, slot, col, walk.head, page);
         issued_k = it + 1;
         if (!warp_wait(v_empty(st), parity, abort_flag)) { ok = false; break; }
-        if (lane == 0) mbar_expect_tx(v_full(st), need * box * 128);
+        if (lane == 0) mbar_expect_tx(v_full(st), need * bytes);
         __syncwarp();
-        if (wanted && kv == 1) tma_load_4d(v_smem(st) + off, map, v_full(st), col * 64, slot, walk.head, page);
+        if (wanted && kv == 1) tma_load_5d(v_smem(st) + off, map, v_full(st), 0, slot, col, walk.head, page);
         issued_v = it + 1;
-        page = after;
+        page = page1;
+        page1 = page2;
       }
     }
-    if (!ok) {
+    if (*abort_flag) {
       drain(issued_k, C::kStages, k_full);
       drain(issued_v, C::kStages, v_full);
+      drain(issued_q, 2, q_full);
     }
   } else if (warp == 1) {
     // ---------------------------------------------------------------------------------------------------- MMA issue
-    if (lane == 0) {
-      const uint32_t idesc_s = make_idesc(false, false, kRowsB, kTileB);
-      const uint32_t idesc_pv = make_idesc(false, true, kRowsB, D);       // values are [keys, D]: MN-major
-      auto issue_s = [&](int g, int st) {
+    // The whole warp runs the loop, so that its values stay in uniform registers; one lane's MMAs and commits take effect.
+    // (In a branch of one lane every operand is moved to a uniform register for every MMA: 60 to 75 clocks each.)
+    const uint32_t idesc_s = make_idesc(false, false, kRowsB, kTileB);
+    const uint32_t idesc_pv = make_idesc(false, true, kRowsB, D);         // values are [keys, D]: MN-major
+    const uint32_t elected = lane == 0;
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+    // an operand's descriptor is its base plus 16-byte units
+    const uint64_t q_desc = make_desc(q_smem(0), 16, 1024), k_desc = make_desc(k_smem(0), 16, 1024), v_desc = make_desc(v_smem(0), kCol, 1024);
+    int it = 0, piece = 0;
+    uint32_t ready = 0;                          // parities of p_ready, one bit per buffer
+    bool ok = true;
+    while (ok && walk.next()) {
+      const int n = __shfl_sync(0xffffffffu, walk.count, 0);
+      const uint64_t qd = q_desc + (piece & 1) * (C::kQBytes >> 4);
+      auto issue_s = [&](int j) {
+        const int st = (it + j) % C::kStages;
+        if (!warp_wait(k_full(st), ((it + j) / C::kStages) & 1, abort_flag)) return false;
+        tc_fence_after();
+        const uint64_t kd = k_desc + st * (2 * C::kTileBytes >> 4);
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const uint32_t off = (uint32_t)(k >> 2) * kColBytes + (uint32_t)(k & 3) * 32u;
-          umma_bf16<1>(tmem + 128 * g, make_desc(q_smem + off, 16, 1024), make_desc(k_smem(st) + off, 16, 1024), idesc_s, k != 0);
-        }
+        for (int k = 0; k < D / 16; ++k)
+          mma_ss(elected, tm + 64 * (j & 3), qd + (((k >> 2) * kQCol + (k & 3) * 32u) >> 4), kd + (((k >> 2) * kCol + (k & 3) * 32u) >> 4), idesc_s, k != 0);
+        mma_commit(elected, s_full(j & 3));
+        mma_commit(elected, k_empty(st));
+        if (j == n - 1) mma_commit(elected, q_empty(piece & 1));
+        return true;
       };
-      int it = 0, piece = 0;
-      int turn[2] = {0, 0};                      // tiles so far of each warpgroup
-      bool ok = true;
-      while (ok && walk.next()) {
-        const int n = walk.count;
-        ok = mbar_wait(q_ready, piece & 1, abort_flag);
-        for (int j = 0; j < min(n, 2) && ok; ++j) {
-          const int st = (it + j) % C::kStages;
-          ok = mbar_wait(k_full(st), ((it + j) / C::kStages) & 1, abort_flag);
-          if (!ok) break;
-          tc_fence_after();
-          issue_s(j, st);
-          umma_commit(s_full(j));
-          umma_commit(k_empty(st));
-        }
-        // the output of the piece before has been read
-        ok = ok && (piece == 0 || mbar_wait(o_free, (piece - 1) & 1, abort_flag));
-        for (int j = 0; j < n && ok; ++j) {
-          const int g = j & 1, st = (it + j) % C::kStages;
-          ok = mbar_wait(v_full(st), ((it + j) / C::kStages) & 1, abort_flag) && mbar_wait(p_ready(g), turn[g] & 1, abort_flag);
-          if (!ok) break;
-          ++turn[g];
-          tc_fence_after();
+      ok = warp_wait(q_full(piece & 1), (piece >> 1) & 1, abort_flag);
+      for (int j = 0; j < min(n, 4) && ok; ++j) ok = issue_s(j);
+      // the output of the piece before has been read
+      ok = ok && (piece == 0 || warp_wait(o_free, (piece - 1) & 1, abort_flag));
+      for (int j = 0; j < n && ok; ++j) {
+        const int b = j & 3, g = j & 1, st = (it + j) % C::kStages;
+        ok = warp_wait(v_full(st), ((it + j) / C::kStages) & 1, abort_flag) && warp_wait(p_ready(b), (ready >> b) & 1, abort_flag);
+        if (!ok) break;
+        ready ^= 1u << b;
+        tc_fence_after();
+        const uint64_t vd = v_desc + st * (2 * C::kTileBytes >> 4);
 #pragma unroll
-          for (int k = 0; k < kTileB / 16; ++k)  // 16 keys: 8 packed columns of P, 16 rows of V
-            umma_bf16_ts(tmem + 256 + 128 * g, tmem + 128 * g + k * 8, make_desc(v_smem(st) + k * 2048, kColBytes, 1024), idesc_pv,
-                         j >= 2 || k != 0);
-          umma_commit(v_empty(st));
-          if (j + 2 < n) {
-            const int st2 = (it + j + 2) % C::kStages;
-            ok = mbar_wait(k_full(st2), ((it + j + 2) / C::kStages) & 1, abort_flag);
-            if (!ok) break;
-            tc_fence_after();
-            issue_s(g, st2);
-            umma_commit(s_full(g));
-            umma_commit(k_empty(st2));
-          }
-        }
-        if (ok) umma_commit(o_full);
-        it += n;
-        ++piece;
+        for (int k = 0; k < kTileB / 16; ++k)    // 16 keys: 8 packed columns of P, 16 rows of V
+          mma_ts(elected, tm + 256 + 128 * g, tm + 64 * b + k * 8, vd + k * (2048 >> 4), idesc_pv, j >= 2 || k != 0);
+        mma_commit(elected, v_empty(st));
+        if (j + 4 < n) ok = issue_s(j + 4);
+        else mma_commit(elected, s_full(b));
       }
+      if (ok) mma_commit(elected, o_full);
+      it += n;
+      ++piece;
     }
-    __syncwarp();
   } else {
     // ---------------------------------------------------------------------------------------------------- softmax
     const int g = (warp - 2) >> 2, quarter = warp & 3;
     const int r = quarter * 32 + lane;           // this thread's pair in the unit, and its TMEM lane
-    const uint32_t s_t = tmem + ((uint32_t)(quarter * 32) << 16) + 128 * g;
-    const uint32_t o_t = tmem + ((uint32_t)(quarter * 32) << 16) + 256;
-    int it = 0, piece = 0, turn = 0;
+    const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16);
+    const uint32_t o_t = lane_base + 256;
+    float* stage = reinterpret_cast<float*>(smem + C::kStage + (warp - 2) * 2048);
+    int it = 0, piece = 0;
+    uint32_t full = 0;                           // parities of s_full, one bit per buffer
     bool ok = true;
     while (ok && walk.next()) {
       const Unit u = list.units[walk.u];
       const int n = walk.count;
-      // queries, swizzled as TMA would: warpgroup g takes half of the 16-byte chunks of each row
-      const int first_row = (warp - 2) * 16;
-#pragma unroll 4
-      for (int c = lane; c < 16 * (D / 8); c += 32) {
-        const int row = first_row + c / (D / 8), ch = c % (D / 8);
-        const int pr = u.pair0 + row;
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (pr < u.pairs)
-          v = *reinterpret_cast<const uint4*>(p.q + (int64_t)(u.row0 + pr / p.G) * p.q_row + (int64_t)(walk.head * p.G + pr % p.G) * p.q_head + ch * 8);
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(q_smem + (ch >> 3) * kColBytes + row * 128 + (((ch & 7) ^ (row & 7)) << 4)),
-                     "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
-      }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(q_ready);
-      // visible keys of this pair; the unit's rows together see [lo_min, hi_max]
+      // visible keys of this pair
       const int pr = u.pair0 + r;
-      const bool live = pr < u.pairs;
+      const bool live = pr < u.pairs && r < p.rows_b * p.G;
       int lo = u.key_lo, hi = u.key_hi - 1;
       if (live) {
         const int row = u.row0 + pr / p.G;
@@ -1012,91 +1094,96 @@ attn_block_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
           lo = max(lo, p.cached[b] + row - p.row_start[b] - p.window + 1);
         }
       }
-      const bool warp_live = u.pair0 + quarter * 32 < u.pairs;
+      const bool warp_live = __any_sync(0xffffffffu, live);
       float m = -INFINITY, l = 0.f;
-      for (int j = g; j < n; j += 2, ++turn) {
-        if (!warp_wait(s_full(g), turn & 1, abort_flag)) { ok = false; break; }
+      for (int j = g; j < n; j += 2) {
+        const int b = j & 3;
+        const uint32_t s_t = lane_base + 64 * b;
+        if (!warp_wait(s_full(b), (full >> b) & 1, abort_flag)) { ok = false; break; }
+        full ^= 1u << b;
         tc_fence_after();
         const int c0 = (u.key_lo / kTileB + walk.first + j) * kTileB;
         if (warp_live) {
-          // The scores are read twice, 32 columns at a time, instead of being held: 128 of them and what the loop needs
-          // do not fit the 168 registers of a 320-thread block.
-          const bool edge = c0 + kTileB - 1 > hi || c0 < lo;
-          auto scores = [&](int c, uint32_t (&x)[32]) {
-            tmem_ld32(s_t + c * 32, x);
-            tmem_ld_wait();
-            if (edge) {
+          uint32_t x[2][32];
+          tmem_ld32(s_t, x[0]);
+          tmem_ld32(s_t + 32, x[1]);
+          tmem_ld_wait();
+          const int rlo = lo - c0, rhi = hi - c0;
+          if (rhi < kTileB - 1 || rlo > 0) {
 #pragma unroll
-              for (int e = 0; e < 32; ++e) {
-                const int key = c0 + c * 32 + e;
-                if (key > hi || key < lo) x[e] = __float_as_uint(-INFINITY);
-              }
-            }
-          };
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                if (c * 32 + e > rhi || c * 32 + e < rlo) x[c][e] = __float_as_uint(-INFINITY);
+          }
           float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t x[32];
-            scores(c, x);
+          for (int c = 0; c < 2; ++c)
 #pragma unroll
-            for (int e = 0; e < 32; ++e) mx[e & 3] = fmaxf(mx[e & 3], __uint_as_float(x[e]));
-          }
+            for (int e = 0; e < 32; ++e) mx[e & 3] = fmaxf(mx[e & 3], __uint_as_float(x[c][e]));
           const float m_new = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2);
           if (__any_sync(0xffffffffu, m_new > m + 8.f)) {
             const float alpha = m == -INFINITY ? 0.f : exp2f(m - m_new);
             l *= alpha;
             if (j >= 2) {
+              // P V of this warpgroup's previous tile is done once the next commit of that buffer has come (see above)
+              const int ob = (j + 2) & 3;
+              if (!warp_wait(s_full(ob), (full >> ob) & 1, abort_flag)) { ok = false; break; }
+              tc_fence_after();
 #pragma unroll 1
-              for (int c = 0; c < D / 32; ++c) {
-                uint32_t o[32];
-                tmem_ld32(o_t + 128 * g + c * 32, o);
+              for (int c = 0; c < D / 16; ++c) {
+                uint32_t o[16];
+                tmem_ld16(o_t + 128 * g + c * 16, o);
                 tmem_ld_wait();
-                uint32_t a[16], b[16];
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                  a[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-                  b[e] = __float_as_uint(__uint_as_float(o[16 + e]) * alpha);
-                }
-                tmem_st16(o_t + 128 * g + c * 32, a);
-                tmem_st16(o_t + 128 * g + c * 32 + 16, b);
+                for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+                tmem_st16(o_t + 128 * g + c * 16, o);
               }
             }
             m = m_new;
           }
           const float neg = m == -INFINITY ? 0.f : -m;
-          float ls[4] = {0.f, 0.f, 0.f, 0.f};
+          const uint64_t sc2 = pack_f2(p.scale_log2, p.scale_log2), neg2 = pack_f2(neg, neg);
+          uint64_t ls[2] = {pack_f2(0.f, 0.f), pack_f2(0.f, 0.f)};
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {            // P of 32 keys takes 16 columns, all of scores that were read
-            uint32_t x[32], pk[16];
-            scores(c, x);
+          for (int c = 0; c < 2; ++c) {
+            uint32_t pk[16];
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-              const float a = exp2f(fmaf(__uint_as_float(x[2 * e]), p.scale_log2, neg));
-              const float b = exp2f(fmaf(__uint_as_float(x[2 * e + 1]), p.scale_log2, neg));
-              ls[e & 3] += a + b;
-              pk[e] = pack2bf(a, b);
+              float a, d;
+              unpack_f2(fma_f2(pack_f2(__uint_as_float(x[c][2 * e]), __uint_as_float(x[c][2 * e + 1])), sc2, neg2), a, d);
+              a = exp2f(a);
+              d = exp2f(d);
+              ls[e & 1] = add_f2(ls[e & 1], pack_f2(a, d));
+              pk[e] = pack2bf(a, d);
             }
             tmem_st16(s_t + c * 16, pk);
           }
-          l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
+          float a0, a1, b0, b1;
+          unpack_f2(ls[0], a0, a1);
+          unpack_f2(ls[1], b0, b1);
+          l += (a0 + a1) + (b0 + b1);
           tmem_st_wait();
         }
         // values outside the keys of the unit may be anything, and a zero weight does not silence an infinity
         if (c0 + kTileB > u.key_hi || c0 < u.key_lo) {
           const int st = (it + j) % C::kStages;
           if (!warp_wait(v_full(st), ((it + j) / C::kStages) & 1, abort_flag)) { ok = false; break; }
-          for (int c = r; c < kTileB * (D / 8); c += 128) {
-            const int key = c / (D / 8), ch = c % (D / 8);
-            if (c0 + key >= u.key_hi || c0 + key < u.key_lo)
-              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(v_smem(st) + (ch >> 3) * kColBytes + key * 128 +
-                           (((ch & 7) ^ (key & 7)) << 4)), "r"(0) : "memory");
+          const int from = max(0, u.key_hi - c0), before = max(0, u.key_lo - c0);
+          for (int key = r / (D / 8); key < kTileB; key += 128 / (D / 8)) {
+            const int ch = r % (D / 8);
+            if (key >= from || key < before)
+              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(v_smem(st) + (ch >> 3) * kCol + key * 128 + (((ch & 7) ^ (key & 7)) << 4)),
+                           "r"(0) : "memory");
           }
           fence_proxy_async_smem();
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(p_ready(g));
+        if (lane == 0) mbar_arrive(p_ready(b));
       }
+      // every buffer that was used this piece has one more commit behind its last P V
+      for (int b = g; b < min(n, 4); b += 2) full ^= 1u << b;
       it += n;
       // ---- join the two warpgroups; each writes half of the columns of every row
       ok = ok && warp_wait(o_full, piece & 1, abort_flag);
@@ -1106,45 +1193,59 @@ attn_block_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
       tc_fence_after();
       const float m0 = ml[r * 2], m1 = n > 1 ? ml[(kRowsB + r) * 2] : -INFINITY;
       const float mm = fmaxf(m0, m1);
-      const float f0 = m0 == -INFINITY ? 0.f : exp2f(m0 - mm), f1 = m1 == -INFINITY ? 0.f : exp2f(m1 - mm);
+      float f0 = m0 == -INFINITY ? 0.f : exp2f(m0 - mm), f1 = m1 == -INFINITY ? 0.f : exp2f(m1 - mm);
       const float ll = f0 * ml[r * 2 + 1] + f1 * ml[(kRowsB + r) * 2 + 1];
       const bool whole = walk.count == walk.unit_tiles;
       const bool last = whole && u.direct;
       const int64_t rh = live ? (int64_t)(u.row0 + pr / p.G) * p.Hq + walk.head * p.G + pr % p.G : 0;
-      float f = 1.f;
       if (last) {
-        float den = ll;
+        float den = ll, f = 1.f;
         if (p.sinks != nullptr) {
           const float sk = p.sinks[rh % p.Hq] * 1.4426950408889634f, top = fmaxf(sk, mm);
           f = mm == -INFINITY ? 0.f : exp2f(mm - top);
           den = ll * f + exp2f(sk - top);
         }
         f = den > 0.f ? f / den : 0.f;
+        f0 *= f;
+        f1 *= f;
       }
-      const int64_t at = whole ? (int64_t)(u.base < 0) * p.R * p.Hq + rh : ((int64_t)blockIdx.x * 2 + (walk.first > 0 ? 0 : 1)) * kRowsB + r;
-      float* dst = (whole ? p.row_o : p.part_b) + at * D;
-      if (!last && live && g == 0) *reinterpret_cast<float2*>((whole ? p.row_ml : p.part_b_ml) + at * 2) = make_float2(mm, ll);
       if (warp_live) {
+        // 16 columns of the warp's 32 rows at a time go through shared memory, so that four lanes write the 64 bytes of a row
+        const int64_t at = whole ? (int64_t)(u.base < 0) * p.R * p.Hq + rh : ((int64_t)blockIdx.x * 2 + (walk.first > 0 ? 0 : 1)) * kRowsB + r;
+        if (!last && live && g == 0) *reinterpret_cast<float2*>((whole ? p.row_ml : p.part_b_ml) + at * 2) = make_float2(mm, ll);
+        const int sub = lane >> 2, quad = lane & 3;
+        char* mine = !live ? nullptr : last ? reinterpret_cast<char*>(p.out + rh * D) : reinterpret_cast<char*>((whole ? p.row_o : p.part_b) + at * D);
+        char* dst[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          dst[k] = reinterpret_cast<char*>(__shfl_sync(0xffffffffu, (unsigned long long)mine, k * 8 + sub));
 #pragma unroll 1
-        for (int c = 0; c < D / 64; ++c) {
-          const int col = g * (D / 2) + c * 32;
-          uint32_t a[32], b[32];
-          tmem_ld32(o_t + col, a);
-          if (n > 1) tmem_ld32(o_t + 128 + col, b);
+        for (int c = 0; c < D / 32; ++c) {
+          const int col = g * (D / 2) + c * 16;
+          uint32_t a[16], b[16];
+          tmem_ld16(o_t + col, a);
+          tmem_ld16(o_t + 128 + col, b);         // with one tile the second accumulator is not read below
           tmem_ld_wait();
-          float v[32];
+          __syncwarp();
 #pragma unroll
-          for (int e = 0; e < 32; ++e) v[e] = (f0 * __uint_as_float(a[e]) + (n > 1 ? f1 * __uint_as_float(b[e]) : 0.f)) * f;
-          if (live) {
-            if (last) {
+          for (int e = 0; e < 4; ++e) {
+            float v[4];
 #pragma unroll
-              for (int e = 0; e < 32; e += 8)
-                *reinterpret_cast<uint4*>(p.out + rh * D + col + e) = make_uint4(pack2bf(v[e], v[e + 1]), pack2bf(v[e + 2], v[e + 3]),
-                                                                                pack2bf(v[e + 4], v[e + 5]), pack2bf(v[e + 6], v[e + 7]));
-            } else {
+            for (int i = 0; i < 4; ++i) v[i] = f0 * __uint_as_float(a[4 * e + i]) + (n > 1 ? f1 * __uint_as_float(b[4 * e + i]) : 0.f);
+            *reinterpret_cast<float4*>(stage + lane * 16 + ((e ^ (lane >> 1)) & 3) * 4) = make_float4(v[0], v[1], v[2], v[3]);
+          }
+          __syncwarp();
+          float4 v[4];
 #pragma unroll
-              for (int e = 0; e < 32; e += 4) *reinterpret_cast<float4*>(dst + col + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
-            }
+          for (int k = 0; k < 4; ++k) v[k] = *reinterpret_cast<const float4*>(stage + (k * 8 + sub) * 16 + ((quad ^ ((k * 8 + sub) >> 1)) & 3) * 4);
+          if (last) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if (dst[k] != nullptr) *reinterpret_cast<uint2*>(dst[k] + (col + quad * 4) * 2) = make_uint2(pack2bf(v[k].x, v[k].y), pack2bf(v[k].z, v[k].w));
+          } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if (dst[k] != nullptr) *reinterpret_cast<float4*>(dst[k] + (col + quad * 4) * 4) = v[k];
           }
         }
       }
@@ -1163,45 +1264,147 @@ attn_block_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_const
   if (threadIdx.x == 0 && *abort_flag) atomicOr(p.status, kStatusWaitTimedOut);
 }
 
-// One warp per (row, query head): joins the pieces of its units; rows that were finished by one piece are left alone.
+// Joins what the attention kernels left in parts.  The index work depends on the plan alone and runs before the wait for
+// them.  Blocks [0, cuts): a sequence that shares nothing is in parts where a stretch boundary cuts one of its units; a CTA
+// has at most one cut unit that begins in its stretch and goes on behind it, and the block(s) of that CTA join it.  The other
+// blocks: a (row, query head) of a group that shares always has two sources; a warp joins the parts of both, those of the
+// prefix first.  All orders are fixed.  Rows behind the last sequence are cleared on the way.
+constexpr int kSlices = 8;                       // blocks that share a cut unit of 128 pairs
+
 template <int D>
-__global__ void __launch_bounds__(256) combine_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(128, 8) finish_kernel(const AttnParams p) {
   constexpr int N = D / 32;
   const int lane = threadIdx.x & 31;
-  const int64_t rh = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (rh >= (int64_t)p.R * p.Hq) return;
-  const int r = (int)(rh / p.Hq), h = (int)(rh % p.Hq);
-  __nv_bfloat16* out = p.out + rh * D + lane * N;
-  auto store = [&](const float (&o)[N], float f) {
-#pragma unroll
-    for (int i = 0; i < N; i += 2) *reinterpret_cast<uint32_t*>(out + i) = pack2bf(o[i] * f, o[i + 1] * f);
+  const WorkLayout lay(p.B, p.NG, p.max_a, p.max_b);
+  const int cuts = p.ctas_a + (p.use_b ? p.ctas_b * kSlices : 0);
+  const int last_row = p.row_start[p.B];
+  auto finish = [&](int64_t rh, float m, float l) {              // 1 / denominator, with the head's sink
+    float f = 1.f;
+    if (p.sinks != nullptr) {
+      const float sk = p.sinks[rh % p.Hq] * 1.4426950408889634f, top = fmaxf(sk, m);
+      f = m == -INFINITY ? 0.f : exp2f(m - top);
+      l = l * f + exp2f(sk - top);
+    }
+    return l > 0.f ? f / l : 0.f;
   };
-  float o[N];
-#pragma unroll
-  for (int i = 0; i < N; ++i) o[i] = 0.f;
-  if (r >= p.row_start[p.B]) {
-    if (p.zero_tail) store(o, 0.f);
+  if ((int)blockIdx.x < cuts) {
+    const bool big = (int)blockIdx.x >= p.ctas_a;
+    const int c0 = big ? (blockIdx.x - p.ctas_a) / kSlices : blockIdx.x;
+    const int row0 = big ? (blockIdx.x - p.ctas_a) % kSlices * (kRowsB / kSlices) : 0;      // this block's rows of the unit
+    const List list = big ? p.list_b(lay) : p.list_a(lay);
+    const int rows = big ? kRowsB : kRowsA;
+    const int64_t line = (int64_t)list.n_tiles * p.Hkv, per = list.stretch(p.Hkv);
+    const int64_t end = min(line, (c0 + 1) * per);
+    int parts = 0, head = 0;
+    Unit unit;
+    if (c0 * per < end && end < line) {
+      const int u = find_segment_warp(list.tiles, list.n_units, (int)((end - 1) / p.Hkv));
+      const int nt = list.tiles[u + 1] - list.tiles[u];
+      head = (int)((end - 1 - (int64_t)list.tiles[u] * p.Hkv) / nt);
+      const int64_t t0 = (int64_t)list.tiles[u] * p.Hkv + (int64_t)head * nt, t1 = t0 + nt;
+      unit = list.units[u];
+      if (t0 >= c0 * per && t1 > end && unit.direct) parts = (int)((t1 - 1) / per) - c0 + 1;
+    }
+    wait_for_earlier();
+    if (p.zero_tail) {
+      const int64_t n = (int64_t)(p.R - last_row) * p.Hq * D / 8;
+      uint4* tail = reinterpret_cast<uint4*>(p.out + (int64_t)last_row * p.Hq * D);
+      for (int64_t i = (int64_t)blockIdx.x * 128 + threadIdx.x; i < n; i += (int64_t)cuts * 128) tail[i] = make_uint4(0, 0, 0, 0);
+    }
+    if (parts == 0) return;
+    const float* po = big ? p.part_b : p.part_a;
+    const float* pml = big ? p.part_b_ml : p.part_a_ml;
+    auto part = [&](int i, int row) { return i == 0 ? ((int64_t)c0 * 2 + 1) * rows + row : (int64_t)(c0 + i) * 2 * rows + row; };
+    const int live = min(big ? min(row0 + kRowsB / kSlices, p.rows_b * p.G) : rows, unit.pairs - unit.pair0);
+    for (int c = threadIdx.x; c < (live - row0) * (D / 4); c += 128) {
+      const int row = row0 + c / (D / 4), d = (c % (D / 4)) * 4;
+      float m = -INFINITY, l = 0.f;
+#pragma unroll 8
+      for (int i = 0; i < parts; ++i) m = fmaxf(m, pml[part(i, row) * 2]);
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+      for (int i = 0; i < parts; ++i) {
+        const int64_t at = part(i, row);
+        const float2 v = *reinterpret_cast<const float2*>(pml + at * 2);
+        const float w = v.x == -INFINITY ? 0.f : exp2f(v.x - m);
+        const float4 q = *reinterpret_cast<const float4*>(po + at * D + d);
+        l += v.y * w;
+        o.x += w > 0.f ? q.x * w : 0.f;          // a part without a visible key may hold anything
+        o.y += w > 0.f ? q.y * w : 0.f;
+        o.z += w > 0.f ? q.z * w : 0.f;
+        o.w += w > 0.f ? q.w * w : 0.f;
+      }
+      const int pr = unit.pair0 + row;
+      const int64_t rh = (int64_t)(unit.row0 + pr / p.G) * p.Hq + head * p.G + pr % p.G;
+      const float f = finish(rh, m, l);
+      *reinterpret_cast<uint2*>(p.out + rh * D + d) = make_uint2(pack2bf(o.x * f, o.y * f), pack2bf(o.z * f, o.w * f));
+    }
     return;
   }
-  const WorkLayout lay(p.B, p.NG, p.max_a, p.max_b);
-  const int b = find_segment(p.row_start, p.B, r);
-  const int g = p.work[lay.seq_group + b];
-  const int kvh = h / p.G;
-  float m = -INFINITY, l = 0.f;
-  if (p.sinks != nullptr) {
-    m = p.sinks[h] * 1.4426950408889634f;
-    l = 1.f;
-  }
-  // Joins parts `first`, `first + step`, ... (n of them): lanes fetch the maxima and sums of 32 parts at once, then the
-  // outputs are added four at a time so that their loads overlap.
-  auto join = [&](const float* po, const float* pml, int64_t first, int64_t step, int n) {
-    for (int i0 = 0; i0 < n; i0 += 32) {
-      const int cnt = min(32, n - i0);
+
+  const int* shared = p.work + lay.shared;
+  const int64_t n_rh = (int64_t)shared[p.NG] * p.Hq;
+  const int64_t stride = (int64_t)(gridDim.x - cuts) * 4;
+  bool waited = false;
+  for (int64_t i = (int64_t)(blockIdx.x - cuts) * 4 + (threadIdx.x >> 5); i < n_rh; i += stride) {
+    const int in = (int)(i / p.Hq), h = (int)(i % p.Hq);
+    const int g = find_segment_warp(shared, p.NG, in);
+    const int r = p.work[lay.group_row + g] + in - shared[g];
+    const int64_t rh = (int64_t)r * p.Hq + h;
+    const int b = find_segment_warp(p.row_start, p.B, r);
+    const float *po[2], *pml[2];
+    int64_t at0[2], at1[2];
+    int step[2], n[2] = {0, 0};
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int s = k == 0 ? p.B + g : b;
+      const int ub = p.use_b ? p.work[lay.src_b + s] : -1;
+      const bool big = ub >= 0;
+      const List list = big ? p.list_b(lay) : p.list_a(lay);
+      const int rows = big ? kRowsB : kRowsA;
+      const int u0 = big ? ub : p.work[lay.src_a + s];
+      if (u0 < 0 || u0 >= list.n_units) continue;
+      const int per_unit = big ? p.rows_b * p.G : kRowsA;
+      const int pr = (r - list.units[u0].row0) * p.G + h % p.G;
+      const int u = u0 + pr / per_unit;
+      if (u >= list.n_units) continue;
+      const int nt = list.tiles[u + 1] - list.tiles[u];
+      if (nt == 0) continue;
+      const int64_t per = list.stretch(p.Hkv);
+      const int64_t t0 = (int64_t)list.tiles[u] * p.Hkv + (int64_t)(h / p.G) * nt;
+      const int c0 = (int)(t0 / per), c1 = (int)((t0 + nt - 1) / per);
+      n[k] = c1 - c0 + 1;
+      if (c0 == c1) {
+        po[k] = p.row_o;
+        pml[k] = p.row_ml;
+        at0[k] = (int64_t)(k == 0) * p.R * p.Hq + rh;
+        at1[k] = step[k] = 0;
+      } else {
+        po[k] = big ? p.part_b : p.part_a;
+        pml[k] = big ? p.part_b_ml : p.part_a_ml;
+        at0[k] = ((int64_t)c0 * 2 + 1) * rows + pr % per_unit;
+        at1[k] = (int64_t)(c0 + 1) * 2 * rows + pr % per_unit;
+        step[k] = 2 * rows;
+      }
+    }
+    if (!waited) wait_for_earlier();
+    waited = true;
+    float o[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) o[e] = 0.f;
+    float m = -INFINITY, l = 0.f;
+    const int total = n[0] + n[1];
+    for (int i0 = 0; i0 < total; i0 += 32) {     // the lanes fetch the maxima and sums of 32 parts at once
+      const int mine = i0 + lane;
       float pm = -INFINITY, pl = 0.f;
-      if (lane < cnt) {
-        const float2 v = *reinterpret_cast<const float2*>(pml + (first + (int64_t)(i0 + lane) * step) * 2);
+      const float* src = nullptr;
+      if (mine < total) {
+        const int k = mine < n[0] ? 0 : 1, j = k == 0 ? mine : mine - n[0];
+        const int64_t at = j == 0 ? at0[k] : at1[k] + (int64_t)(j - 1) * step[k];
+        const float2 v = *reinterpret_cast<const float2*>(pml[k] + at * 2);
         pm = v.x;
         pl = v.y;
+        src = po[k] + at * D;
       }
       const float mn = fmaxf(m, warp_max(pm));
       if (mn == -INFINITY) continue;
@@ -1211,45 +1414,24 @@ __global__ void __launch_bounds__(256) combine_kernel(const AttnParams p) {
       l = l * a + warp_sum(pl * w);
 #pragma unroll
       for (int e = 0; e < N; ++e) o[e] *= a;
+      const int cnt = min(32, total - i0);
 #pragma unroll 4
-      for (int i = 0; i < cnt; ++i) {
-        const float wi = __shfl_sync(0xffffffffu, w, i);
-        const float* q = po + (first + (int64_t)(i0 + i) * step) * D + lane * N;
-        if (wi > 0.f) {                          // a part without a visible key may hold anything
+      for (int j = 0; j < cnt; ++j) {
+        const float wi = __shfl_sync(0xffffffffu, w, j);
+        const float* q = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, (unsigned long long)src, j)) + lane * N;
+        float v[N];
 #pragma unroll
-          for (int e = 0; e < N; ++e) o[e] += q[e] * wi;
-        }
+        for (int e = 0; e < N; ++e) v[e] = wi > 0.f ? q[e] : 0.f;
+#pragma unroll
+        for (int e = 0; e < N; ++e) o[e] += v[e] * wi;
       }
     }
-  };
-  // the prefix comes first, then the sequence's own keys: a fixed order
-  for (int k = g >= 0 ? 0 : 1; k < 2; ++k) {
-    const int s = k == 0 ? p.B + g : b;
-    const int ub = p.use_b ? p.work[lay.src_b + s] : -1;
-    const bool big = ub >= 0;
-    const List list = big ? p.list_b(lay) : p.list_a(lay);
-    const int rows = big ? kRowsB : kRowsA;
-    const int u0 = big ? ub : p.work[lay.src_a + s];
-    if (u0 < 0 || u0 >= list.n_units) continue;
-    const int pr = (r - list.units[u0].row0) * p.G + h % p.G;
-    const int u = u0 + pr / rows;
-    if (u >= list.n_units) continue;
-    const int n = list.tiles[u + 1] - list.tiles[u];
-    if (n == 0) continue;
-    const int64_t per = list.stretch(p.Hkv);
-    const int64_t t0 = (int64_t)list.tiles[u] * p.Hkv + (int64_t)kvh * n;
-    const int c0 = (int)(t0 / per), c1 = (int)((t0 + n - 1) / per);
-    if (c0 == c1) {
-      if (k == 1 && g < 0) return;               // finished by its piece
-      join(p.row_o, p.row_ml, (int64_t)(k == 0) * p.R * p.Hq + rh, 0, 1);
-    } else {
-      const float* po = big ? p.part_b : p.part_a;
-      const float* pml = big ? p.part_b_ml : p.part_a_ml;
-      join(po, pml, ((int64_t)c0 * 2 + 1) * rows + pr % rows, 0, 1);
-      join(po, pml, (int64_t)(c0 + 1) * 2 * rows + pr % rows, 2 * rows, c1 - c0);
-    }
+    const float f = finish(rh, m, l);
+    __nv_bfloat16* out = p.out + rh * D + lane * N;
+#pragma unroll
+    for (int e = 0; e < N; e += 2) *reinterpret_cast<uint32_t*>(out + e) = pack2bf(o[e] * f, o[e + 1] * f);
   }
-  store(o, l > 0.f ? 1.f / l : 0.f);
+  if (!waited) wait_for_earlier();               // a block without a row still ends behind the earlier kernels
 }
 
 }  // namespace paged
@@ -1375,7 +1557,8 @@ at::Tensor paged_work(const at::Tensor& cached, const at::Tensor& row_start, con
   p.B = (int)B; p.NG = (int)NG; p.W = (int)table_cols; p.ps = (int)page_size;
   p.G = (int)(hq / hkv); p.window = (int)window;
   p.max_a = (int)max_units(B, NG, total_rows, p.G, paged::kRowsA);
-  p.max_b = (int)max_units(B, NG, total_rows, p.G, paged::kRowsB);
+  p.rows_b = paged::kRowsB / p.G;
+  p.max_b = (int)max_units(B, NG, total_rows, p.G, p.rows_b > 0 ? p.rows_b * p.G : paged::kRowsB);
   auto work = at::empty({paged::WorkLayout(B, NG, p.max_a, p.max_b).size}, cached.options());
   p.work = work.data_ptr<int>();
   p.status = status_word_ptr();
@@ -1386,18 +1569,33 @@ at::Tensor paged_work(const at::Tensor& cached, const at::Tensor& row_start, con
   return work;
 }
 
-// Pages as 128-byte wide, swizzled boxes of up to 64 slots of one page and head.
-static CUtensorMap page_map(const at::Tensor& t) {
+// Pages as [page, head, 64-column block, slot, 64 columns], fetched in 128-byte swizzled boxes of up to 64 slots of one page
+// and head and `blocks` column blocks.
+static CUtensorMap page_map(const at::Tensor& t, int blocks) {
   CUtensorMap map;
   const uint64_t e = 2;
-  const cuuint64_t dims[4] = {(cuuint64_t)t.size(3), (cuuint64_t)t.size(2), (cuuint64_t)t.size(1), (cuuint64_t)t.size(0)};
-  const cuuint64_t strides[3] = {(cuuint64_t)t.stride(2) * e, (cuuint64_t)t.stride(1) * e, (cuuint64_t)t.stride(0) * e};
-  const cuuint32_t box[4] = {64, (cuuint32_t)std::min<int64_t>(t.size(2), 64), 1, 1};
-  const cuuint32_t elem[4] = {1, 1, 1, 1};
-  const CUresult r = cuTensorMapEncodeTiled(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, t.data_ptr(), dims, strides, box, elem,
+  const cuuint64_t dims[5] = {64, (cuuint64_t)t.size(2), (cuuint64_t)t.size(3) / 64, (cuuint64_t)t.size(1), (cuuint64_t)t.size(0)};
+  const cuuint64_t strides[4] = {(cuuint64_t)t.stride(2) * e, 128, (cuuint64_t)t.stride(1) * e, (cuuint64_t)t.stride(0) * e};
+  const cuuint32_t box[5] = {64, (cuuint32_t)std::min<int64_t>(t.size(2), 64), (cuuint32_t)blocks, 1, 1};
+  const cuuint32_t elem[5] = {1, 1, 1, 1, 1};
+  const CUresult r = cuTensorMapEncodeTiled(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, t.data_ptr(), dims, strides, box, elem,
                                             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                                             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   TORCH_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled (pages) failed with code ", (int)r);
+  return map;
+}
+
+// Queries [R, Hq, D] as 128-byte wide, swizzled boxes of `rows` rows x the query heads of one key head.
+static CUtensorMap query_map(const at::Tensor& q, int group, int rows) {
+  CUtensorMap map;
+  const cuuint64_t dims[3] = {(cuuint64_t)q.size(2), (cuuint64_t)q.size(1), (cuuint64_t)q.size(0)};
+  const cuuint64_t strides[2] = {(cuuint64_t)q.stride(1) * 2, (cuuint64_t)q.stride(0) * 2};
+  const cuuint32_t box[3] = {64, (cuuint32_t)group, (cuuint32_t)rows};
+  const cuuint32_t elem[3] = {1, 1, 1};
+  const CUresult r = cuTensorMapEncodeTiled(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, q.data_ptr(), dims, strides, box, elem,
+                                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  TORCH_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled (queries) failed with code ", (int)r);
   return map;
 }
 
@@ -1413,10 +1611,10 @@ void paged_attention(const at::Tensor& q, const at::Tensor& k_pages, const at::T
   TORCH_CHECK(q.stride(2) == 1 && q.stride(1) % 2 == 0 && q.stride(0) % 2 == 0 && reinterpret_cast<uintptr_t>(q.data_ptr()) % 4 == 0,
               "paged_attention: query vectors must be contiguous and 4-byte aligned");
   TORCH_CHECK(D == 64 || D == 128 || D == 256, "paged_attention: unsupported head dimension ", D);
-  TORCH_CHECK(ps == 16 || ps == 32 || (ps > 0 && ps % 64 == 0), "paged_attention: unsupported page size ", ps);
+  TORCH_CHECK(ps >= 16 && ps <= 256 && (ps & (ps - 1)) == 0, "paged_attention: unsupported page size ", ps);
   TORCH_CHECK(out.is_contiguous() && out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type() && out.device() == dev &&
-                  reinterpret_cast<uintptr_t>(out.data_ptr()) % 8 == 0,
-              "paged_attention: out must be a contiguous bf16 tensor of q's shape");
+                  reinterpret_cast<uintptr_t>(out.data_ptr()) % 16 == 0,
+              "paged_attention: out must be a contiguous, 16-byte aligned bf16 tensor of q's shape");
   if (sinks.has_value())
     TORCH_CHECK(sinks->device() == dev && sinks->scalar_type() == at::kFloat && sinks->is_contiguous() && sinks->numel() == q.size(1),
                 "paged_attention: sinks must be a contiguous fp32 vector [Hq]");
@@ -1433,19 +1631,21 @@ void paged_attention(const at::Tensor& q, const at::Tensor& k_pages, const at::T
   p.row_start = int_vector(row_start, B + 1, dev, "row_start");
   p.B = (int)B; p.NG = (int)groups; p.W = (int)table.size(1); p.R = (int)R;
   p.Hq = (int)q.size(1); p.Hkv = (int)k_pages.size(1); p.G = p.Hq / p.Hkv; p.ps = (int)ps; p.num_pages = (int)k_pages.size(0);
+  p.ps_shift = __builtin_ctz((unsigned)ps);
   p.window = (int)window; p.scale_log2 = (float)(scale * 1.4426950408889634); p.zero_tail = zero_tail;
   p.max_a = (int)max_units(B, groups, R, p.G, paged::kRowsA);
-  p.max_b = (int)max_units(B, groups, R, p.G, paged::kRowsB);
+  p.rows_b = paged::kRowsB / p.G;
+  p.max_b = (int)max_units(B, groups, R, p.G, p.rows_b > 0 ? p.rows_b * p.G : paged::kRowsB);
   p.work = int_vector(work, paged::WorkLayout(B, groups, p.max_a, p.max_b).size, dev, "work (made for other heads, rows or groups?)");
   p.status = status_word_ptr();
-  // 256-wide heads would need more tensor memory than there is for two accumulators: they stay on the first kernel.
-  p.use_b = D <= 128 && max_rows * p.G > paged::kFewPairs;
+  // 256-wide heads would need more tensor memory than there is for two accumulators, and a unit holds whole rows of up
+  // to 128 query heads per key head: the rest stays on the first kernel.
+  p.use_b = D <= 128 && p.rows_b > 0 && max_rows * p.G > paged::kFewPairs;
   p.ctas_a = num_sms() * (D == 256 ? paged::Cfg<256>::kCtasPerSm : paged::Cfg<128>::kCtasPerSm);
   p.ctas_b = num_sms();
   if (p.use_b)
-    TORCH_CHECK(q.stride(0) % 8 == 0 && q.stride(1) % 8 == 0 && reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0 &&
-                    reinterpret_cast<uintptr_t>(out.data_ptr()) % 16 == 0,
-                "paged_attention: query and output vectors must be 16-byte aligned");
+    TORCH_CHECK(q.stride(0) % 8 == 0 && q.stride(1) % 8 == 0 && reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0,
+                "paged_attention: query vectors must be 16-byte aligned");
   const auto f32 = q.options().dtype(at::kFloat);
   const int64_t na = (int64_t)p.ctas_a * 2 * paged::kRowsA, nb = p.use_b ? (int64_t)p.ctas_b * 2 * paged::kRowsB : 0;
   const int64_t nr = groups > 0 ? 2 * R * p.Hq : 0;
@@ -1456,24 +1656,33 @@ void paged_attention(const at::Tensor& q, const at::Tensor& k_pages, const at::T
   p.part_a_ml = p.row_o + nr * D;
   p.part_b_ml = p.part_a_ml + na * 2;
   p.row_ml = p.part_b_ml + nb * 2;
-  const CUtensorMap mk = page_map(k_pages), mv = page_map(v_pages);
+  const int blocks = (int)(D / 64);
+  const CUtensorMap mk = page_map(k_pages, blocks), mv = page_map(v_pages, blocks);
+  const CUtensorMap mq = p.use_b ? query_map(q, p.G, p.rows_b) : mk;
+  const bool split = p.use_b && ps < paged::kTileB && blocks > 1;      // the second kernel's tiles are not whole boxes
+  const CUtensorMap bk = split ? page_map(k_pages, 1) : mk, bv = split ? page_map(v_pages, 1) : mv;
   auto stream = at::cuda::getCurrentCUDAStream();
+  auto run = [&](auto kernel, int64_t grid, int threads, int smem, bool chained, auto... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = chained ? 1 : 0;
+    if (smem > 0) C10_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, args...));
+  };
   auto launch = [&](auto dim) {
     constexpr int kD = decltype(dim)::value;
-    auto kernel = paged::attn_rows_kernel<kD>;
-    C10_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, paged::Cfg<kD>::kSmem));
-    if constexpr (kD <= 128) {
-      if (p.use_b) {
-        auto block = paged::attn_block_kernel<kD>;
-        C10_CUDA_CHECK(cudaFuncSetAttribute(block, cudaFuncAttributeMaxDynamicSharedMemorySize, paged::CfgB<kD>::kSmem));
-        block<<<p.ctas_b, 320, paged::CfgB<kD>::kSmem, stream>>>(mk, mv, p);
-        C10_CUDA_KERNEL_LAUNCH_CHECK();
-      }
-    }
-    kernel<<<p.ctas_a, 160, paged::Cfg<kD>::kSmem, stream>>>(mk, mv, p);
-    C10_CUDA_KERNEL_LAUNCH_CHECK();
-    paged::combine_kernel<kD><<<(unsigned)((R * p.Hq + 7) / 8), 256, 0, stream>>>(p);
-    C10_CUDA_KERNEL_LAUNCH_CHECK();
+    if constexpr (kD <= 128)
+      if (p.use_b) run(paged::attn_block_kernel<kD>, p.ctas_b, 320, paged::CfgB<kD>::kSmem, false, mq, bk, bv, p);
+    run(paged::attn_rows_kernel<kD>, p.ctas_a, 160, paged::Cfg<kD>::kSmem, p.use_b, mk, mv, p);
+    const int64_t row_blocks = groups > 0 ? std::min<int64_t>((R * p.Hq + 3) / 4, (int64_t)num_sms() * 8) : 0;
+    run(paged::finish_kernel<kD>, p.ctas_a + (p.use_b ? p.ctas_b * paged::kSlices : 0) + row_blocks, 128, 0, true, p);
   };
   if (D == 64) launch(std::integral_constant<int, 64>{});
   else if (D == 128) launch(std::integral_constant<int, 128>{});

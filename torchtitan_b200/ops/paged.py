@@ -92,7 +92,7 @@ def page_plan(cached: torch.Tensor, new: torch.Tensor, block_table: torch.Tensor
 def _vectors(t: torch.Tensor) -> torch.Tensor:
     """``t`` itself when its last dimension is contiguous and every vector starts on 16 bytes, else a copy."""
     e = t.element_size()
-    if t.stride(-1) == 1 and all((s * e) % 16 == 0 for s in t.stride()[:-1]) and t.data_ptr() % 16 == 0:
+    if t.stride(-1) == 1 and all(s > 0 and (s * e) % 16 == 0 for s in t.stride()[:-1]) and t.data_ptr() % 16 == 0:
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
