@@ -26,7 +26,7 @@ std::tuple<at::Tensor, at::Tensor> qk_norm_rope_bwd(const at::Tensor& dq, const 
                                                     const at::Tensor& x, int64_t hq, int64_t hkv, const c10::optional<at::Tensor>& qw,
                                                     const c10::optional<at::Tensor>& kw, const c10::optional<at::Tensor>& table,
                                                     const c10::optional<at::Tensor>& positions, const c10::optional<at::Tensor>& axes,
-                                                    bool interleaved, double eps, double gain, double q_scale);
+                                                    bool interleaved, double eps, double gain, double q_scale, bool fp32_dw);
 std::tuple<at::Tensor, at::Tensor, at::Tensor> page_plan(const at::Tensor& cached, const at::Tensor& new_rows, at::Tensor block_table,
                                                          const at::Tensor& slots, const at::Tensor& pages,
                                                          const c10::optional<at::Tensor>& mapped, int64_t page_size,
@@ -131,7 +131,7 @@ TORCH_LIBRARY(tb200, m) {
   m.def("qk_norm_rope_fwd(Tensor x, int hq, int hkv, Tensor? qw, Tensor? kw, Tensor? table, Tensor? positions, Tensor? axes, "
         "bool interleaved, float eps, float gain, float q_scale) -> (Tensor, Tensor)", &tb200::qk_norm_rope_fwd);
   m.def("qk_norm_rope_bwd(Tensor dq, Tensor dk, Tensor? dv, Tensor x, int hq, int hkv, Tensor? qw, Tensor? kw, Tensor? table, "
-        "Tensor? positions, Tensor? axes, bool interleaved, float eps, float gain, float q_scale) -> (Tensor, Tensor)",
+        "Tensor? positions, Tensor? axes, bool interleaved, float eps, float gain, float q_scale, bool fp32_dw) -> (Tensor, Tensor)",
         &tb200::qk_norm_rope_bwd);
   m.def("page_plan(Tensor cached, Tensor new_rows, Tensor(a!) block_table, Tensor slots, Tensor pages, Tensor? mapped, int page_size, "
         "int total_rows, int num_pages) -> (Tensor, Tensor, Tensor)", &tb200::page_plan);

@@ -414,6 +414,11 @@ struct List {
   __device__ __forceinline__ int64_t stretch(int Hkv) const { return max((int64_t)kMinTiles, ((int64_t)n_tiles * Hkv + ctas - 1) / ctas); }
 };
 
+// What a CTA leaves for the finish kernel: the unit that its stretch begins and does not end, when it shares nothing.
+struct __align__(16) Cut {
+  int parts, row0, pairs, pair0, head;
+};
+
 struct AttnParams {
   const __nv_bfloat16* q;
   int64_t q_row, q_head;
@@ -426,6 +431,7 @@ struct AttnParams {
   float *part_a, *part_a_ml;                     // [ctas_a, 2, kRowsA, D], [ctas_a, 2, kRowsA, 2]: pieces
   float *part_b, *part_b_ml;                     // [ctas_b, 2, kRowsB, D], [ctas_b, 2, kRowsB, 2]
   float *row_o, *row_ml;                         // [2, R, Hq, D], [2, R, Hq, 2]: whole units of groups (own keys, prefix)
+  Cut* cuts;                                     // [ctas_a + ctas_b]
   int* status;
 
   __device__ __forceinline__ List list_a(const WorkLayout& lay) const {
@@ -497,12 +503,13 @@ __device__ __forceinline__ void drain(int it, int stages, F full) {
 struct Walk {
   const int* tiles;
   int Hkv;
-  int64_t at, end;
+  int64_t at, end, per;
   int u, head, first, count;                     // current piece: unit, key head, first tile of the unit, tiles
   int unit_tiles;
 
   __device__ __forceinline__ Walk(const List& l, int Hkv_, int cta) : tiles(l.tiles), Hkv(Hkv_) {
-    const int64_t line = (int64_t)l.n_tiles * Hkv, per = l.stretch(Hkv);
+    const int64_t line = (int64_t)l.n_tiles * Hkv;
+    per = l.stretch(Hkv);
     at = min(line, cta * per);
     end = min(line, at + per);
     u = at < end ? find_segment_warp(tiles, l.n_units, (int)(at / Hkv)) : 0;
@@ -517,6 +524,12 @@ struct Walk {
     count = (int)min((int64_t)(unit_tiles - first), end - at);
     at += count;
     return true;
+  }
+  // After the last piece of the stretch: how many CTAs the unit is spread over if it begins here and goes on, else 0.
+  __device__ __forceinline__ Cut cut(const Unit& unit) const {
+    Cut c{0, unit.row0, unit.pairs, unit.pair0, head};
+    if (first == 0 && count < unit_tiles && unit.direct) c.parts = 2 + (int)((unit_tiles - count - 1) / per);
+    return c;
   }
 };
 
@@ -596,6 +609,7 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
     // a page's box is [64-column block][key][128 bytes]; this warp's 16 keys lie in one box
     const int box = min(p.ps, kTileA);
     const uint32_t block = box * 128, mine = (warp * 16) / box * (box * D * 2) + (warp * 16) % box * 128;
+    if (threadIdx.x == 0) p.cuts[blockIdx.x] = Cut{0, 0, 0, 0, 0};       // each piece writes it again
     bool ok = true;
     while (ok && walk.next()) {
       const Unit u = list.units[walk.u];
@@ -790,6 +804,7 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
       consumer_sync();
       const bool whole = walk.count == walk.unit_tiles;
       const int which = walk.first > 0 ? 0 : 1;
+      if (threadIdx.x == 0) p.cuts[blockIdx.x] = walk.cut(u);
       const int64_t cta = blockIdx.x;
       for (int c = threadIdx.x; c < kRowsA * (D / 4); c += 128) {
         const int row = c / (D / 4), d = (c % (D / 4)) * 4;
@@ -839,19 +854,19 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
 // P = exp2(S - m) written over S as bf16, O += P V with P read from tensor memory.  Behind every P V the issuer puts the S
 // of the tile four later, into the same buffer, and a commit (a bare one at the end), so "the next S of a buffer is there"
 // also says that its P V is done: a warpgroup that has to rescale its accumulator waits for that of its other buffer.
-// Queries come by TMA too (boxes of rows x heads of the key head), the next piece's while the present one runs.
+// Queries come by TMA too (boxes of rows x heads of the key head), the next piece's as soon as the last S is done.
 // Bound by the exponentials (64 x 128 per tile on a 16-per-clock unit are 512 clocks, as many as the MMAs take) when many
 // units share their keys through L2, by HBM when each key range has one unit.
 //   warp 0: TMA producer    warp 1: TMEM, MMA issue    warps 2..5, 6..9: softmax of even / odd tiles, then the output
 // Tensor memory: score buffer b (of warpgroup b % 2) at column 64 b, accumulator of warpgroup g at 256 + 128 g.
 template <int D>
 struct CfgB {
-  static constexpr int kStages = D == 64 ? 8 : 4;                // tiles of keys and of values in flight
+  static constexpr int kStages = D == 64 ? 10 : 5;               // tiles of keys and of values in flight: 160 KB
   static constexpr uint32_t kQBytes = kRowsB * D * 2;
   static constexpr uint32_t kTileBytes = kTileB * D * 2;
-  static constexpr uint32_t kStage = 2 * kQBytes + 2 * kStages * kTileBytes;     // fp32 rows on their way out, 2 KB a warp
+  static constexpr uint32_t kStage = kQBytes + 2 * kStages * kTileBytes;         // fp32 rows on their way out, 2 KB a warp
   static constexpr uint32_t kBars = kStage + 8 * 2048;
-  static constexpr int kNumBars = 4 * kStages + 14;
+  static constexpr int kNumBars = 4 * kStages + 12;
   static constexpr uint32_t kMl = kBars + 8 * kNumBars + 8;      // TMEM address, abort flag
   static constexpr uint32_t kSmem = kMl + 2 * kRowsB * 2 * 4;
 };
@@ -905,9 +920,9 @@ attn_block_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
   constexpr uint32_t kQCol = kRowsB * 128, kCol = kTileB * 128;   // one 64-column block of the queries, of a tile
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t base = smem_u32(smem);
-  auto q_smem = [&](int i) { return base + C::kQBytes * i; };
-  auto k_smem = [&](int s) { return base + 2 * C::kQBytes + C::kTileBytes * (2 * s); };
-  auto v_smem = [&](int s) { return base + 2 * C::kQBytes + C::kTileBytes * (2 * s + 1); };
+  const uint32_t q_smem = base;
+  auto k_smem = [&](int s) { return base + C::kQBytes + C::kTileBytes * (2 * s); };
+  auto v_smem = [&](int s) { return base + C::kQBytes + C::kTileBytes * (2 * s + 1); };
   const uint32_t bars = base + C::kBars;
   auto k_full = [&](int s) { return bars + 8u * s; };
   auto k_empty = [&](int s) { return bars + 8u * (C::kStages + s); };
@@ -915,9 +930,7 @@ attn_block_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
   auto v_empty = [&](int s) { return bars + 8u * (3 * C::kStages + s); };
   auto s_full = [&](int b) { return bars + 8u * (4 * C::kStages + b); };
   auto p_ready = [&](int b) { return bars + 8u * (4 * C::kStages + 4 + b); };
-  auto q_full = [&](int i) { return bars + 8u * (4 * C::kStages + 8 + i); };
-  auto q_empty = [&](int i) { return bars + 8u * (4 * C::kStages + 10 + i); };
-  const uint32_t o_full = bars + 8u * (4 * C::kStages + 12), o_free = o_full + 8u;
+  const uint32_t q_full = bars + 8u * (4 * C::kStages + 8), q_empty = q_full + 8u, o_full = q_full + 16u, o_free = q_full + 24u;
   uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(smem + C::kBars + 8 * C::kNumBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_ptr + 1);
   float* ml = reinterpret_cast<float*>(smem + C::kMl);            // [2][kRowsB][2]
@@ -926,7 +939,10 @@ attn_block_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
   let_next_start();
   const List list = p.list_b(WorkLayout(p.B, p.NG, p.max_a, p.max_b));
   Walk walk(list, p.Hkv, blockIdx.x);
-  if (walk.at >= walk.end) return;                                // the same for the whole block
+  if (walk.at >= walk.end) {                                      // the same for the whole block
+    if (threadIdx.x == 64) p.cuts[p.ctas_a + blockIdx.x] = Cut{0, 0, 0, 0, 0};
+    return;
+  }
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kStages; ++s) {
@@ -939,10 +955,8 @@ attn_block_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       mbar_init(s_full(b), 1);
       mbar_init(p_ready(b), 4);
     }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(q_full(i), 1);
-      mbar_init(q_empty(i), 1);
-    }
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
     mbar_init(o_full, 1);
     mbar_init(o_free, 8);
     *abort_flag = 0;
@@ -977,11 +991,11 @@ attn_block_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
         return li < loads && key < u.key_hi ? row[key >> p.ps_shift] : INT_MIN;
       };
       int page = entry(t0), page1 = walk.count > 1 ? entry(t0 + 1) : INT_MIN;
-      if (!warp_wait(q_empty(piece & 1), ((piece >> 1) & 1) ^ 1, abort_flag)) break;
+      if (!warp_wait(q_empty, (piece & 1) ^ 1, abort_flag)) break;   // the last S of the piece before is done
       if (lane == 0) {
-        mbar_expect_tx(q_full(piece & 1), q_bytes);
+        mbar_expect_tx(q_full, q_bytes);
         for (int c = 0; c < D / 64; ++c)
-          tma_load_3d(q_smem(piece & 1) + c * kQCol, &tmap_q, q_full(piece & 1), c * 64, walk.head * p.G, u.row0 + u.pair0 / p.G);
+          tma_load_3d(q_smem + c * kQCol, &tmap_q, q_full, c * 64, walk.head * p.G, u.row0 + u.pair0 / p.G);
       }
       issued_q = ++piece;
       for (int i = 0; i < walk.count; ++i, ++it) {
@@ -1014,7 +1028,7 @@ attn_block_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     if (*abort_flag) {
       drain(issued_k, C::kStages, k_full);
       drain(issued_v, C::kStages, v_full);
-      drain(issued_q, 2, q_full);
+      drain(issued_q, 1, [&](int) { return q_full; });
     }
   } else if (warp == 1) {
     // ---------------------------------------------------------------------------------------------------- MMA issue
@@ -1025,13 +1039,12 @@ attn_block_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     const uint32_t elected = lane == 0;
     const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
     // an operand's descriptor is its base plus 16-byte units
-    const uint64_t q_desc = make_desc(q_smem(0), 16, 1024), k_desc = make_desc(k_smem(0), 16, 1024), v_desc = make_desc(v_smem(0), kCol, 1024);
+    const uint64_t q_desc = make_desc(q_smem, 16, 1024), k_desc = make_desc(k_smem(0), 16, 1024), v_desc = make_desc(v_smem(0), kCol, 1024);
     int it = 0, piece = 0;
     uint32_t ready = 0;                          // parities of p_ready, one bit per buffer
     bool ok = true;
     while (ok && walk.next()) {
       const int n = __shfl_sync(0xffffffffu, walk.count, 0);
-      const uint64_t qd = q_desc + (piece & 1) * (C::kQBytes >> 4);
       auto issue_s = [&](int j) {
         const int st = (it + j) % C::kStages;
         if (!warp_wait(k_full(st), ((it + j) / C::kStages) & 1, abort_flag)) return false;
@@ -1039,13 +1052,13 @@ attn_block_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
         const uint64_t kd = k_desc + st * (2 * C::kTileBytes >> 4);
 #pragma unroll
         for (int k = 0; k < D / 16; ++k)
-          mma_ss(elected, tm + 64 * (j & 3), qd + (((k >> 2) * kQCol + (k & 3) * 32u) >> 4), kd + (((k >> 2) * kCol + (k & 3) * 32u) >> 4), idesc_s, k != 0);
+          mma_ss(elected, tm + 64 * (j & 3), q_desc + (((k >> 2) * kQCol + (k & 3) * 32u) >> 4), kd + (((k >> 2) * kCol + (k & 3) * 32u) >> 4), idesc_s, k != 0);
         mma_commit(elected, s_full(j & 3));
         mma_commit(elected, k_empty(st));
-        if (j == n - 1) mma_commit(elected, q_empty(piece & 1));
+        if (j == n - 1) mma_commit(elected, q_empty);
         return true;
       };
-      ok = warp_wait(q_full(piece & 1), (piece >> 1) & 1, abort_flag);
+      ok = warp_wait(q_full, piece & 1, abort_flag);
       for (int j = 0; j < min(n, 4) && ok; ++j) ok = issue_s(j);
       // the output of the piece before has been read
       ok = ok && (piece == 0 || warp_wait(o_free, (piece - 1) & 1, abort_flag));
@@ -1075,6 +1088,7 @@ attn_block_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     const uint32_t o_t = lane_base + 256;
     float* stage = reinterpret_cast<float*>(smem + C::kStage + (warp - 2) * 2048);
     int it = 0, piece = 0;
+    if (threadIdx.x == 64) p.cuts[p.ctas_a + blockIdx.x] = Cut{0, 0, 0, 0, 0};   // each piece writes it again
     uint32_t full = 0;                           // parities of s_full, one bit per buffer
     bool ok = true;
     while (ok && walk.next()) {
@@ -1253,6 +1267,7 @@ attn_block_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       if (softmax_any(false)) break;             // ml is read before the next piece writes it
       if (lane == 0) mbar_arrive(o_free);
       ++piece;
+      if (threadIdx.x == 64) p.cuts[p.ctas_a + blockIdx.x] = walk.cut(u);
     }
   }
   tc_fence_before();
@@ -1264,9 +1279,9 @@ attn_block_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
   if (threadIdx.x == 0 && *abort_flag) atomicOr(p.status, kStatusWaitTimedOut);
 }
 
-// Joins what the attention kernels left in parts.  The index work depends on the plan alone and runs before the wait for
-// them.  Blocks [0, cuts): a sequence that shares nothing is in parts where a stretch boundary cuts one of its units; a CTA
-// has at most one cut unit that begins in its stretch and goes on behind it, and the block(s) of that CTA join it.  The other
+// Joins what the attention kernels left in parts.  Blocks [0, cuts): a sequence that shares nothing is in parts where a
+// stretch boundary cuts one of its units; a CTA has at most one cut unit that begins in its stretch and goes on behind it
+// and left its description, and the block(s) of that CTA join it.  The other
 // blocks: a (row, query head) of a group that shares always has two sources; a warp joins the parts of both, those of the
 // prefix first.  All orders are fixed.  Rows behind the last sequence are cleared on the way.
 constexpr int kSlices = 8;                       // blocks that share a cut unit of 128 pairs
@@ -1291,21 +1306,10 @@ __global__ void __launch_bounds__(128, 8) finish_kernel(const AttnParams p) {
     const bool big = (int)blockIdx.x >= p.ctas_a;
     const int c0 = big ? (blockIdx.x - p.ctas_a) / kSlices : blockIdx.x;
     const int row0 = big ? (blockIdx.x - p.ctas_a) % kSlices * (kRowsB / kSlices) : 0;      // this block's rows of the unit
-    const List list = big ? p.list_b(lay) : p.list_a(lay);
     const int rows = big ? kRowsB : kRowsA;
-    const int64_t line = (int64_t)list.n_tiles * p.Hkv, per = list.stretch(p.Hkv);
-    const int64_t end = min(line, (c0 + 1) * per);
-    int parts = 0, head = 0;
-    Unit unit;
-    if (c0 * per < end && end < line) {
-      const int u = find_segment_warp(list.tiles, list.n_units, (int)((end - 1) / p.Hkv));
-      const int nt = list.tiles[u + 1] - list.tiles[u];
-      head = (int)((end - 1 - (int64_t)list.tiles[u] * p.Hkv) / nt);
-      const int64_t t0 = (int64_t)list.tiles[u] * p.Hkv + (int64_t)head * nt, t1 = t0 + nt;
-      unit = list.units[u];
-      if (t0 >= c0 * per && t1 > end && unit.direct) parts = (int)((t1 - 1) / per) - c0 + 1;
-    }
     wait_for_earlier();
+    const Cut unit = p.cuts[big ? p.ctas_a + c0 : c0];
+    const int parts = min(unit.parts, (big ? p.ctas_b : p.ctas_a) - c0), head = unit.head;
     if (p.zero_tail) {
       const int64_t n = (int64_t)(p.R - last_row) * p.Hq * D / 8;
       uint4* tail = reinterpret_cast<uint4*>(p.out + (int64_t)last_row * p.Hq * D);
@@ -1318,21 +1322,33 @@ __global__ void __launch_bounds__(128, 8) finish_kernel(const AttnParams p) {
     const int live = min(big ? min(row0 + kRowsB / kSlices, p.rows_b * p.G) : rows, unit.pairs - unit.pair0);
     for (int c = threadIdx.x; c < (live - row0) * (D / 4); c += 128) {
       const int row = row0 + c / (D / 4), d = (c % (D / 4)) * 4;
+      // eight parts at a time, all their loads in flight together
       float m = -INFINITY, l = 0.f;
-#pragma unroll 8
-      for (int i = 0; i < parts; ++i) m = fmaxf(m, pml[part(i, row) * 2]);
       float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-      for (int i = 0; i < parts; ++i) {
-        const int64_t at = part(i, row);
-        const float2 v = *reinterpret_cast<const float2*>(pml + at * 2);
-        const float w = v.x == -INFINITY ? 0.f : exp2f(v.x - m);
-        const float4 q = *reinterpret_cast<const float4*>(po + at * D + d);
-        l += v.y * w;
-        o.x += w > 0.f ? q.x * w : 0.f;          // a part without a visible key may hold anything
-        o.y += w > 0.f ? q.y * w : 0.f;
-        o.z += w > 0.f ? q.z * w : 0.f;
-        o.w += w > 0.f ? q.w * w : 0.f;
+      for (int i0 = 0; i0 < parts; i0 += 8) {
+        float2 v[8];
+        float4 q[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int64_t at = part(min(i0 + i, parts - 1), row);
+          v[i] = *reinterpret_cast<const float2*>(pml + at * 2);
+          q[i] = *reinterpret_cast<const float4*>(po + at * D + d);
+          if (i0 + i >= parts) v[i].x = -INFINITY;
+        }
+        float mn = m;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) mn = fmaxf(mn, v[i].x);
+        const float a = m == -INFINITY ? 0.f : exp2f(m - mn);
+        m = mn;
+        l *= a;
+        o.x *= a; o.y *= a; o.z *= a; o.w *= a;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (v[i].x == -INFINITY) continue;     // a part without a visible key may hold anything
+          const float w = exp2f(v[i].x - mn);
+          l += v[i].y * w;
+          o.x += q[i].x * w; o.y += q[i].y * w; o.z += q[i].z * w; o.w += q[i].w * w;
+        }
       }
       const int pr = unit.pair0 + row;
       const int64_t rh = (int64_t)(unit.row0 + pr / p.G) * p.Hq + head * p.G + pr % p.G;
@@ -1649,13 +1665,15 @@ void paged_attention(const at::Tensor& q, const at::Tensor& k_pages, const at::T
   const auto f32 = q.options().dtype(at::kFloat);
   const int64_t na = (int64_t)p.ctas_a * 2 * paged::kRowsA, nb = p.use_b ? (int64_t)p.ctas_b * 2 * paged::kRowsB : 0;
   const int64_t nr = groups > 0 ? 2 * R * p.Hq : 0;
-  auto scratch = at::empty({(na + nb + nr) * (D + 2)}, f32);
+  const int64_t n_cuts = p.ctas_a + p.ctas_b;
+  auto scratch = at::empty({(na + nb + nr) * (D + 2) + 4 + n_cuts * (int64_t)(sizeof(paged::Cut) / sizeof(float))}, f32);
   p.part_a = scratch.data_ptr<float>();
   p.part_b = p.part_a + na * D;
   p.row_o = p.part_b + nb * D;
   p.part_a_ml = p.row_o + nr * D;
   p.part_b_ml = p.part_a_ml + na * 2;
   p.row_ml = p.part_b_ml + nb * 2;
+  p.cuts = reinterpret_cast<paged::Cut*>(reinterpret_cast<uintptr_t>(p.row_ml + nr * 2 + 3) & ~(uintptr_t)15);
   const int blocks = (int)(D / 64);
   const CUtensorMap mk = page_map(k_pages, blocks), mv = page_map(v_pages, blocks);
   const CUtensorMap mq = p.use_b ? query_map(q, p.G, p.rows_b) : mk;

@@ -500,8 +500,10 @@ def rope_qk_(qkv: torch.Tensor, table: torch.Tensor, positions: torch.Tensor, in
 # =====================================================================
 def _heads_ok(t: torch.Tensor) -> torch.Tensor:
     """``t[T, H, D]`` with adjacent heads and 16-byte aligned rows, copied only when it is not."""
-    if t.stride(2) == 1 and (t.stride(1) == t.shape[2] or t.shape[1] == 1) and t.stride(0) % 8 == 0 and t.data_ptr() % 16 == 0:
-        return t.as_strided(t.shape, (t.stride(0), t.shape[2], 1))
+    T, H, D = t.shape
+    s0, s1, s2 = t.stride()
+    if s2 == 1 and s1 == D and s0 % 8 == 0 and t.data_ptr() % 16 == 0:
+        return t
     return t.clone(memory_format=torch.contiguous_format)
 
 
@@ -510,31 +512,35 @@ class _QKNormRopeFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, qkv, q_weight, k_weight, table, positions, axes, meta):
-        hq, hkv = meta[0], meta[1]
-        x = qkv
-        if _cuda(qkv):
-            _count()
-            x = _heads_ok(qkv)
-            q, k = ext.require().qk_norm_rope_fwd(x, hq, hkv, q_weight, k_weight, table, positions, axes, *meta[2:])
-        else:
-            q, k = ref.qk_norm_rope_fwd(x, hq, hkv, q_weight, k_weight, table, positions, axes, *meta[2:])
+        x, q, k = _qk_norm_rope_fwd(qkv, q_weight, k_weight, table, positions, axes, meta)
         ctx.save_for_backward(x, q_weight, k_weight, table, positions, axes)
         ctx.meta = meta
-        return q, k, qkv[:, hq + hkv:]
+        return q, k, qkv[:, meta[0] + meta[1]:]
 
     @staticmethod
     def backward(ctx, dq, dk, dv):
         x, q_weight, k_weight, table, positions, axes = ctx.saved_tensors
-        hq, hkv = ctx.meta[:2]
+        args = (x, ctx.meta[0], ctx.meta[1], q_weight, k_weight, table, positions, axes, *ctx.meta[2:])
         if _cuda(x):
-            _count(1 if q_weight is None and k_weight is None else 2)
-            dx, dw = ext.require().qk_norm_rope_bwd(_heads_ok(dq), _heads_ok(dk), _heads_ok(dv), x, hq, hkv, q_weight, k_weight, table,
-                                                    positions, axes, *ctx.meta[2:])
+            weights = [w for w in (q_weight, k_weight) if w is not None]
+            _count(2 if weights else 1)
+            # the gradient is rounded once, to the type that receives it
+            fp32 = any(w.main_grad.dtype == torch.float32 for w in weights if getattr(w, "main_grad", None) is not None)
+            dx, dw = ext.require().qk_norm_rope_bwd(_heads_ok(dq), _heads_ok(dk), _heads_ok(dv), *args, fp32)
         else:
-            dx, dw = ref.qk_norm_rope_bwd(dq, dk, dv, x, hq, hkv, q_weight, k_weight, table, positions, axes, *ctx.meta[2:])
+            dx, dw = ref.qk_norm_rope_bwd(dq, dk, dv, *args)
         dws = [_deliver_wgrad(w, dw[i]) if w is not None and ctx.needs_input_grad[1 + i] else None
                for i, w in enumerate((q_weight, k_weight))]
         return dx, dws[0], dws[1], None, None, None, None
+
+
+def _qk_norm_rope_fwd(qkv, q_weight, k_weight, table, positions, axes, meta):
+    """``(qkv as the kernel reads it, q, k)``."""
+    if not _cuda(qkv):
+        return (qkv, *ref.qk_norm_rope_fwd(qkv, meta[0], meta[1], q_weight, k_weight, table, positions, axes, *meta[2:]))
+    _count()
+    x = _heads_ok(qkv)
+    return (x, *ext.require().qk_norm_rope_fwd(x, meta[0], meta[1], q_weight, k_weight, table, positions, axes, *meta[2:]))
 
 
 def qk_norm_rope(qkv: torch.Tensor, n_heads: int, n_kv_heads: int, q_weight: torch.Tensor | None, k_weight: torch.Tensor | None,
@@ -562,6 +568,9 @@ def qk_norm_rope(qkv: torch.Tensor, n_heads: int, n_kv_heads: int, q_weight: tor
     else:
         positions = axes = None
     meta = (int(n_heads), int(n_kv_heads), bool(interleaved), float(eps), float(gain_center), float(q_scale))
+    if not torch.is_grad_enabled():
+        _, q, k = _qk_norm_rope_fwd(qkv, q_weight, k_weight, table, positions, axes, meta)
+        return q, k, qkv[:, n_heads + n_kv_heads:]
     return _QKNormRopeFn.apply(qkv, q_weight, k_weight, table, positions, axes, meta)
 
 
