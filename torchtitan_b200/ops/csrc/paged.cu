@@ -22,6 +22,7 @@ constexpr int kMaxSlots = 65536;        // rows of the block table: one bit each
 constexpr int kMaxCols = 1 << 20;       // columns of the block table and rows of a step: a block's scan stays inside 32 bits
 constexpr int kMaxRows = 1 << 22;
 constexpr int kMaxLength = 1 << 30;     // tokens of one sequence
+constexpr int kMaxLine = 1 << 30;       // tiles of a step over all key heads
 constexpr int kMinTiles = 2;            // a CTA's stretch is at least this long: shorter ones cost more to join than they save
 
 // Inclusive scan over the block; `part` needs 33 entries.
@@ -242,7 +243,7 @@ struct WorkLayout {
 
 struct WorkParams {
   const int *cached, *row_start, *slots, *group_start, *group_prefix;
-  int B, NG, W, ps, G, window, max_a, max_b, rows_b;   // rows_b: token rows of a unit in list B
+  int B, NG, W, ps, G, Hkv, window, max_a, max_b, rows_b;   // rows_b: token rows of a unit in list B
   int* work;
   int* status;
 };
@@ -382,12 +383,20 @@ __global__ void __launch_bounds__(1024) work_kernel(const WorkParams p) {
           w.key_hi = (int)min((int64_t)prefix[g], room);
         }
         n = w.key_hi > w.key_lo ? (w.key_hi - 1) / tile - w.key_lo / tile + 1 : 0;
+        if (n > kMaxLine / 1024) {               // a block's scan stays inside 32 bits
+          bad = true;
+          n = 0;
+        }
         units[n0 + u] = w;
       }
       int total;
       const int e = block_scan(n, part, total);
       if (u < n_units) tiles[n0 + u] = t0 + n_tiles + e - n;
-      n_tiles += total;
+      n_tiles = min(n_tiles + total, kMaxLine + 1 - t0);
+    }
+    if ((t0 + (int64_t)n_tiles) * p.Hkv > kMaxLine) {      // no real step comes near: lengths that are flagged, no work
+      bad = true;
+      n_units = n_tiles = 0;
     }
     n0 += n_units;
     t0 += n_tiles;
@@ -411,7 +420,7 @@ struct List {
   const Unit* units;
   int n_units, n_tiles, ctas;
   // Tiles of a CTA's stretch.
-  __device__ __forceinline__ int64_t stretch(int Hkv) const { return max((int64_t)kMinTiles, ((int64_t)n_tiles * Hkv + ctas - 1) / ctas); }
+  __device__ __forceinline__ int stretch(int Hkv) const { return max(kMinTiles, (n_tiles * Hkv + ctas - 1) / ctas); }
 };
 
 // What a CTA leaves for the finish kernel: the unit that its stretch begins and does not end, when it shares nothing.
@@ -503,32 +512,36 @@ __device__ __forceinline__ void drain(int it, int stages, F full) {
 struct Walk {
   const int* tiles;
   int Hkv;
-  int64_t at, end, per;
+  int at, end, per;
   int u, head, first, count;                     // current piece: unit, key head, first tile of the unit, tiles
   int unit_tiles;
 
   __device__ __forceinline__ Walk(const List& l, int Hkv_, int cta) : tiles(l.tiles), Hkv(Hkv_) {
-    const int64_t line = (int64_t)l.n_tiles * Hkv;
+    const int line = l.n_tiles * Hkv;
     per = l.stretch(Hkv);
-    at = min(line, cta * per);
+    at = (int)min((int64_t)line, (int64_t)cta * per);
     end = min(line, at + per);
-    u = at < end ? find_segment_warp(tiles, l.n_units, (int)(at / Hkv)) : 0;
+    u = at < end ? find_segment_warp(tiles, l.n_units, at / Hkv) : 0;
   }
   __device__ __forceinline__ bool next() {
     if (at >= end) return false;
-    while ((int64_t)tiles[u + 1] * Hkv <= at) ++u;
-    unit_tiles = tiles[u + 1] - tiles[u];
-    const int64_t in = at - (int64_t)tiles[u] * Hkv;
-    head = (int)(in / unit_tiles);
-    first = (int)(in % unit_tiles);
-    count = (int)min((int64_t)(unit_tiles - first), end - at);
+    int from = tiles[u], to = tiles[u + 1];
+    while (to * Hkv <= at) {
+      from = to;
+      to = tiles[++u + 1];
+    }
+    unit_tiles = to - from;
+    const int in = at - from * Hkv;
+    head = in / unit_tiles;
+    first = in - head * unit_tiles;
+    count = min(unit_tiles - first, end - at);
     at += count;
     return true;
   }
   // After the last piece of the stretch: how many CTAs the unit is spread over if it begins here and goes on, else 0.
   __device__ __forceinline__ Cut cut(const Unit& unit) const {
     Cut c{0, unit.row0, unit.pairs, unit.pair0, head};
-    if (first == 0 && count < unit_tiles && unit.direct) c.parts = 2 + (int)((unit_tiles - count - 1) / per);
+    if (first == 0 && count < unit_tiles && unit.direct) c.parts = 2 + (unit_tiles - count - 1) / per;
     return c;
   }
 };
@@ -1359,68 +1372,66 @@ __global__ void __launch_bounds__(128, 8) finish_kernel(const AttnParams p) {
   }
 
   const int* shared = p.work + lay.shared;
-  const int64_t n_rh = (int64_t)shared[p.NG] * p.Hq;
-  const int64_t stride = (int64_t)(gridDim.x - cuts) * 4;
+  const int n_rows = shared[p.NG], stride = (gridDim.x - cuts) * 4;
   bool waited = false;
-  for (int64_t i = (int64_t)(blockIdx.x - cuts) * 4 + (threadIdx.x >> 5); i < n_rh; i += stride) {
-    const int in = (int)(i / p.Hq), h = (int)(i % p.Hq);
+  for (int64_t i = (blockIdx.x - cuts) * 4 + (threadIdx.x >> 5); i < (int64_t)n_rows * p.Hq; i += stride) {
+    const int in = (unsigned)i / (unsigned)p.Hq, h = (int)i - in * p.Hq;
     const int g = find_segment_warp(shared, p.NG, in);
     const int r = p.work[lay.group_row + g] + in - shared[g];
     const int64_t rh = (int64_t)r * p.Hq + h;
     const int b = find_segment_warp(p.row_start, p.B, r);
-    const float *po[2], *pml[2];
-    int64_t at0[2], at1[2];
-    int step[2], n[2] = {0, 0};
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int s = k == 0 ? p.B + g : b;
-      const int ub = p.use_b ? p.work[lay.src_b + s] : -1;
+    // where the parts of the two sources are: part 0, the others `step` apart
+    struct Parts {
+      const float *o, *ml;
+      int64_t at0, at1;
+      int step, n;
+    };
+    auto locate = [&](bool prefix) {
+      Parts q{p.row_o, p.row_ml, (int64_t)prefix * p.R * p.Hq + rh, 0, 0, 0};
+      const int s = prefix ? p.B + g : b;
+      const int ua = p.work[lay.src_a + s], ub = p.use_b ? p.work[lay.src_b + s] : -1;
       const bool big = ub >= 0;
       const List list = big ? p.list_b(lay) : p.list_a(lay);
-      const int rows = big ? kRowsB : kRowsA;
-      const int u0 = big ? ub : p.work[lay.src_a + s];
-      if (u0 < 0 || u0 >= list.n_units) continue;
-      const int per_unit = big ? p.rows_b * p.G : kRowsA;
+      const int u0 = big ? ub : ua;
+      if (u0 < 0 || u0 >= list.n_units) return q;
+      const int rows = big ? kRowsB : kRowsA, per_unit = big ? p.rows_b * p.G : kRowsA;
       const int pr = (r - list.units[u0].row0) * p.G + h % p.G;
       const int u = u0 + pr / per_unit;
-      if (u >= list.n_units) continue;
-      const int nt = list.tiles[u + 1] - list.tiles[u];
-      if (nt == 0) continue;
-      const int64_t per = list.stretch(p.Hkv);
-      const int64_t t0 = (int64_t)list.tiles[u] * p.Hkv + (int64_t)(h / p.G) * nt;
-      const int c0 = (int)(t0 / per), c1 = (int)((t0 + nt - 1) / per);
-      n[k] = c1 - c0 + 1;
-      if (c0 == c1) {
-        po[k] = p.row_o;
-        pml[k] = p.row_ml;
-        at0[k] = (int64_t)(k == 0) * p.R * p.Hq + rh;
-        at1[k] = step[k] = 0;
-      } else {
-        po[k] = big ? p.part_b : p.part_a;
-        pml[k] = big ? p.part_b_ml : p.part_a_ml;
-        at0[k] = ((int64_t)c0 * 2 + 1) * rows + pr % per_unit;
-        at1[k] = (int64_t)(c0 + 1) * 2 * rows + pr % per_unit;
-        step[k] = 2 * rows;
+      if (u >= list.n_units) return q;
+      const int t = list.tiles[u], nt = list.tiles[u + 1] - t;
+      if (nt == 0) return q;
+      const int per = list.stretch(p.Hkv), t0 = t * p.Hkv + (h / p.G) * nt;
+      const int c0 = t0 / per, c1 = (t0 + nt - 1) / per;
+      q.n = c1 - c0 + 1;
+      if (c0 < c1) {
+        q.o = big ? p.part_b : p.part_a;
+        q.ml = big ? p.part_b_ml : p.part_a_ml;
+        q.at0 = ((int64_t)c0 * 2 + 1) * rows + pr % per_unit;
+        q.at1 = (int64_t)(c0 + 1) * 2 * rows + pr % per_unit;
+        q.step = 2 * rows;
       }
-    }
+      return q;
+    };
+    const Parts own = locate(false), pre = locate(true);
     if (!waited) wait_for_earlier();
     waited = true;
     float o[N];
 #pragma unroll
     for (int e = 0; e < N; ++e) o[e] = 0.f;
     float m = -INFINITY, l = 0.f;
-    const int total = n[0] + n[1];
+    const int total = pre.n + own.n;
     for (int i0 = 0; i0 < total; i0 += 32) {     // the lanes fetch the maxima and sums of 32 parts at once
       const int mine = i0 + lane;
       float pm = -INFINITY, pl = 0.f;
-      const float* src = nullptr;
+      const float* src = p.row_o;
       if (mine < total) {
-        const int k = mine < n[0] ? 0 : 1, j = k == 0 ? mine : mine - n[0];
-        const int64_t at = j == 0 ? at0[k] : at1[k] + (int64_t)(j - 1) * step[k];
-        const float2 v = *reinterpret_cast<const float2*>(pml[k] + at * 2);
+        const bool first = mine < pre.n;
+        const int j = first ? mine : mine - pre.n;
+        const int64_t at = j == 0 ? (first ? pre.at0 : own.at0) : (first ? pre.at1 : own.at1) + (int64_t)(j - 1) * (first ? pre.step : own.step);
+        const float2 v = *reinterpret_cast<const float2*>((first ? pre.ml : own.ml) + at * 2);
         pm = v.x;
         pl = v.y;
-        src = po[k] + at * D;
+        src = (first ? pre.o : own.o) + at * D;
       }
       const float mn = fmaxf(m, warp_max(pm));
       if (mn == -INFINITY) continue;
@@ -1431,15 +1442,22 @@ __global__ void __launch_bounds__(128, 8) finish_kernel(const AttnParams p) {
 #pragma unroll
       for (int e = 0; e < N; ++e) o[e] *= a;
       const int cnt = min(32, total - i0);
-#pragma unroll 4
-      for (int j = 0; j < cnt; ++j) {
-        const float wi = __shfl_sync(0xffffffffu, w, j);
-        const float* q = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, (unsigned long long)src, j)) + lane * N;
-        float v[N];
+      for (int j0 = 0; j0 < cnt; j0 += 4) {      // four parts' outputs in flight
+        float wi[4], v[4][N];
 #pragma unroll
-        for (int e = 0; e < N; ++e) v[e] = wi > 0.f ? q[e] : 0.f;
+        for (int j = 0; j < 4; ++j) {
+          const int k = min(j0 + j, cnt - 1);
+          wi[j] = j0 + j < cnt ? __shfl_sync(0xffffffffu, w, k) : 0.f;
+          const float* q = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, (unsigned long long)src, k)) + lane * N;
 #pragma unroll
-        for (int e = 0; e < N; ++e) o[e] += v[e] * wi;
+          for (int e = 0; e < N; ++e) v[j][e] = q[e];
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (wi[j] > 0.f) {                     // a part without a visible key may hold anything
+#pragma unroll
+            for (int e = 0; e < N; ++e) o[e] += v[j][e] * wi[j];
+          }
       }
     }
     const float f = finish(rh, m, l);
@@ -1571,7 +1589,7 @@ at::Tensor paged_work(const at::Tensor& cached, const at::Tensor& row_start, con
     p.group_start = int_vector(*group_start, NG + 1, dev, "group_start");
   }
   p.B = (int)B; p.NG = (int)NG; p.W = (int)table_cols; p.ps = (int)page_size;
-  p.G = (int)(hq / hkv); p.window = (int)window;
+  p.G = (int)(hq / hkv); p.Hkv = (int)hkv; p.window = (int)window;
   p.max_a = (int)max_units(B, NG, total_rows, p.G, paged::kRowsA);
   p.rows_b = paged::kRowsB / p.G;
   p.max_b = (int)max_units(B, NG, total_rows, p.G, p.rows_b > 0 ? p.rows_b * p.G : paged::kRowsB);
