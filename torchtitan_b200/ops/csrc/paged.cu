@@ -786,24 +786,30 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
           o[n][2 * j + 1] *= f;
         }
       }
+      const int live_rows = min(kRowsA, u.pairs - u.pair0);
+      const bool tall = live_rows > 8;           // a decode step of up to eight heads a key head has nothing in the upper rows
       // an fp32 tile in shared memory: column blocks of eight are spread over the banks by the row
       auto slot = [&](int which, int row, int c) { return exch + which * (kRowsA * D) + row * D + (c ^ ((row & 7) << 3)); };
       auto put = [&](int which) {
 #pragma unroll
-        for (int n = 0; n < D / 8; ++n)
+        for (int j = 0; j < 2; ++j) {
+          if (j == 1 && !tall) break;
 #pragma unroll
-          for (int j = 0; j < 2; ++j)
+          for (int n = 0; n < D / 8; ++n)
             *reinterpret_cast<float2*>(slot(which, r_lo + 8 * j, n * 8 + quad * 2)) = make_float2(o[n][2 * j], o[n][2 * j + 1]);
+        }
       };
       auto add = [&](int which) {
 #pragma unroll
-        for (int n = 0; n < D / 8; ++n)
+        for (int j = 0; j < 2; ++j) {
+          if (j == 1 && !tall) break;
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
+          for (int n = 0; n < D / 8; ++n) {
             const float2 v = *reinterpret_cast<const float2*>(slot(which, r_lo + 8 * j, n * 8 + quad * 2));
             o[n][2 * j] += v.x;
             o[n][2 * j + 1] += v.y;
           }
+        }
       };
       if (warp & 1) put(warp >> 1);
       consumer_sync();
@@ -819,10 +825,9 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
       const int which = walk.first > 0 ? 0 : 1;
       if (threadIdx.x == 0) p.cuts[blockIdx.x] = walk.cut(u);
       const int64_t cta = blockIdx.x;
-      for (int c = threadIdx.x; c < kRowsA * (D / 4); c += 128) {
+      for (int c = threadIdx.x; c < live_rows * (D / 4); c += 128) {
         const int row = c / (D / 4), d = (c % (D / 4)) * 4;
         const int pr = u.pair0 + row;
-        if (pr >= u.pairs) continue;
         const float4 v = *reinterpret_cast<const float4*>(slot(0, row, d));
         float mm = -INFINITY, ll = 0.f;
         for (int w = 0; w < 4; ++w) mm = fmaxf(mm, ml[(w * kRowsA + row) * 2]);
