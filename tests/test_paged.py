@@ -382,6 +382,8 @@ def test_attention_refusals(device):
         paged.attention(s.q, s.kp[:-1], s.vp[:-1], plan, 1.0)
     with pytest.raises(ValueError, match="pools"):
         paged.attention(s.q, s.kp, s.vp[..., :32], plan, 1.0)
+    with pytest.raises(ValueError, match="scale"):
+        paged.attention(s.q, s.kp, s.vp, plan, 0.0)
     with pytest.raises(ValueError, match="queries"):
         paged.attention(s.q[:, :3], s.kp, s.vp, plan, 1.0)
 
@@ -449,3 +451,63 @@ def test_a_side_stream_gives_the_same_result():
             outs.append(paged.attention(s.q, s.kp, s.vp, s.plan(), s.scale))
     torch.cuda.synchronize()
     assert all(torch.equal(o, want) for o in outs)
+
+
+@pytest.mark.gpu
+def test_the_largest_number_of_sequences_and_one_more():
+    B, ps, hq, hkv, D = 4096, 16, 4, 2, 64
+    g = torch.Generator("cuda").manual_seed(0)
+    kp, vp = (torch.randn(B + 1, hkv, ps, D, device="cuda", generator=g).to(torch.bfloat16) for _ in range(2))
+    q = torch.randn(B, hq, D, device="cuda", generator=g).to(torch.bfloat16)
+    ar = torch.arange(B, dtype=torch.int32, device="cuda")
+    lens = ar % ps
+    table = ar.flip(0).view(B, 1).contiguous()
+    plan = paged.page_plan(lens, torch.ones_like(ar), table, ar, _i32([], "cuda"), ps, B, num_pages=B + 1, mapped=torch.ones_like(ar),
+                           group_start=torch.arange(B + 1, dtype=torch.int32, device="cuda"), group_prefix=torch.zeros_like(ar),
+                           n_heads=hq, n_kv_heads=hkv)
+    got = paged.attention(q, kp, vp, plan, 0.125)
+    assert ext.require().status(True) == 0
+    page = table[:, 0].long()
+    k, v = kp[page].double(), vp[page].double()                                     # [B, hkv, ps, D]
+    s = torch.einsum("bhgd,bhjd->bhgj", q.double().view(B, hkv, 2, D), k) * 0.125
+    s = s.masked_fill(torch.arange(ps, device="cuda") > lens[:, None, None, None], float("-inf"))
+    p = torch.softmax(s, -1)
+    want = torch.einsum("bhgj,bhjd->bhgd", p, v).reshape(B, hq, D)
+    size = torch.einsum("bhgj,bhjd->bhgd", p, v.abs()).reshape(B, hq, D)
+    assert ((got.double() - want).abs() <= 2 ** -8 * want.abs() + (2 ** -8 + 2 ** -12) * size).all()
+    more = torch.zeros(B + 1, dtype=torch.int32, device="cuda")
+    with pytest.raises(RuntimeError, match="4096"):
+        paged.page_plan(more, more, table, more, _i32([], "cuda"), ps, 0, num_pages=B)
+
+
+@pytest.mark.gpu
+def test_a_group_whose_first_member_has_no_tokens_yet():
+    """The first step of a group: the member that computes the prefix has it among its new rows, the others start behind it."""
+    s = _Step([(64, [(0, 1), (3, 2), (0, 1)])], hq=8, hkv=2, D=128, ps=32, device="cuda")
+    want = paged.attention(s.q, s.kp, s.vp, s.plan(grouped=False), s.scale)
+    for prefix in (0, 1, 33, 63, 64, 1000, -5):                                     # clipped to the shortest member
+        s.prefix = [prefix]
+        s.check(paged.attention(s.q, s.kp, s.vp, s.plan(), s.scale))
+    assert torch.equal(want, paged.attention(s.q, s.kp, s.vp, s.plan(grouped=False), s.scale))
+
+
+@pytest.mark.gpu
+def test_pages_with_heads_inside_slots_and_an_expanded_query():
+    """Pools laid out [page, slot, head, D] are a permuted view; queries with a stride of zero are copied."""
+    s = _Step([(0, [(90, 1), (17, 1)])], hq=8, hkv=2, D=64, ps=16, device="cuda")
+    want = paged.attention(s.q, s.kp, s.vp, s.plan(), s.scale)
+    kp, vp = (t.transpose(1, 2).contiguous().transpose(1, 2) for t in (s.kp, s.vp))
+    assert torch.equal(paged.attention(s.q, kp, vp, s.plan(), s.scale), want)
+    one = s.q[:1].expand(2, -1, -1)
+    assert torch.equal(paged.attention(one, s.kp, s.vp, s.plan(), s.scale), paged.attention(one.contiguous(), s.kp, s.vp, s.plan(), s.scale))
+
+
+@pytest.mark.gpu
+def test_no_sequences_at_all():
+    e = _i32([], "cuda")
+    table = torch.zeros(2, 3, dtype=torch.int32, device="cuda")
+    plan = paged.page_plan(e, e, table, e, e, 16, 3, num_pages=4, n_heads=4, n_kv_heads=2)
+    kp = torch.zeros(4, 2, 16, 64, device="cuda", dtype=torch.bfloat16)
+    assert not paged.attention(torch.ones(3, 4, 64, device="cuda", dtype=torch.bfloat16), kp, kp, plan, 1.0).any()
+    plan = paged.page_plan(e, e, table, e, e, 16, 0, num_pages=4, n_heads=4, n_kv_heads=2)
+    assert paged.attention(torch.ones(0, 4, 64, device="cuda", dtype=torch.bfloat16), kp, kp, plan, 1.0).shape == (0, 4, 64)

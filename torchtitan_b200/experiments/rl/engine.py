@@ -325,9 +325,11 @@ class GenerationEngine(Configurable):
         if device.type == "cuda":
             from torchtitan_b200.ops import ext
 
-            if int(ext.require().status(False)) & 16:
+            bits = int(ext.require().status(False))
+            if bits & 20:
                 ext.require().status(True)
-                raise RuntimeError("paged cache: a page table entry was out of range")
+                raise RuntimeError("paged cache: " + ("a page table entry was out of range" if bits & 16 else
+                                                      "a bounded wait inside the attention kernels expired"))
 
     def _finish_reason(self, s: _Seq, tok: int) -> str | None:
         sc = s.sampling

@@ -9,6 +9,8 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/library.h>
 
+#include <atomic>
+
 #include "common.cuh"
 
 namespace tb200 {
@@ -564,8 +566,14 @@ at::Tensor swiglu_bwd(const at::Tensor& gu, const at::Tensor& dout) {
 
 // Address of the status word on the current device, for kernels of other translation units.
 int* status_word_ptr() {
-  int* p = nullptr;
-  C10_CUDA_CHECK(cudaGetSymbolAddress(reinterpret_cast<void**>(&p), g_status_word));
+  static std::atomic<int*> per_device[64];       // the address is fixed once the module is loaded on a device
+  int dev = 0;
+  C10_CUDA_CHECK(cudaGetDevice(&dev));
+  int* p = dev < 64 ? per_device[dev].load() : nullptr;
+  if (p == nullptr) {
+    C10_CUDA_CHECK(cudaGetSymbolAddress(reinterpret_cast<void**>(&p), g_status_word));
+    if (dev < 64) per_device[dev].store(p);
+  }
   return p;
 }
 

@@ -9,6 +9,8 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <cuda.h>
 
+#include <atomic>
+
 #include "common.cuh"
 #include "tc.cuh"
 
@@ -889,22 +891,6 @@ struct CfgB {
   static constexpr uint32_t kSmem = kMl + 2 * kRowsB * 2 * 4;
 };
 
-// tcgen05 with the elected lane as a predicate instead of a branch.
-__device__ __forceinline__ void mma_ss(uint32_t elected, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
-               "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-               ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(elected) : "memory");
-}
-__device__ __forceinline__ void mma_ts(uint32_t elected, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
-               "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-               ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(elected) : "memory");
-}
-__device__ __forceinline__ void mma_commit(uint32_t elected, uint32_t bar) {
-  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
-               "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(elected) : "memory");
-}
-
 // Named barrier of the eight softmax warps; true for all when any thread brings true.
 __device__ __forceinline__ bool softmax_any(bool v) {
   uint32_t r;
@@ -1050,54 +1036,62 @@ attn_block_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     }
   } else if (warp == 1) {
     // ---------------------------------------------------------------------------------------------------- MMA issue
-    // The whole warp runs the loop, so that its values stay in uniform registers; one lane's MMAs and commits take effect.
-    // (In a branch of one lane every operand is moved to a uniform register for every MMA: 60 to 75 clocks each.)
-    const uint32_t idesc_s = make_idesc(false, false, kRowsB, kTileB);
-    const uint32_t idesc_pv = make_idesc(false, true, kRowsB, D);         // values are [keys, D]: MN-major
-    const uint32_t elected = lane == 0;
-    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
-    // an operand's descriptor is its base plus 16-byte units
-    const uint64_t q_desc = make_desc(q_smem, 16, 1024), k_desc = make_desc(k_smem(0), 16, 1024), v_desc = make_desc(v_smem(0), kCol, 1024);
-    int it = 0, piece = 0;
-    uint32_t ready = 0;                          // parities of p_ready, one bit per buffer
-    bool ok = true;
-    while (ok && walk.next()) {
-      const int n = __shfl_sync(0xffffffffu, walk.count, 0);
-      auto issue_s = [&](int j) {
-        const int st = (it + j) % C::kStages;
-        if (!warp_wait(k_full(st), ((it + j) / C::kStages) & 1, abort_flag)) return false;
-        tc_fence_after();
-        const uint64_t kd = k_desc + st * (2 * C::kTileBytes >> 4);
+    // This thread's own instructions are on the critical path of every tile: stages and parities are counted up, not
+    // divided out, and a barrier that is there already costs one poll.
+    if (lane == 0) {
+      const uint32_t idesc_s = make_idesc(false, false, kRowsB, kTileB);
+      const uint32_t idesc_pv = make_idesc(false, true, kRowsB, D);       // values are [keys, D]: MN-major
+      // an operand's descriptor is its base plus 16-byte units
+      const uint64_t q_desc = make_desc(q_smem, 16, 1024), k_desc = make_desc(k_smem(0), 16, 1024), v_desc = make_desc(v_smem(0), kCol, 1024);
+      auto wait = [&](uint32_t bar, uint32_t parity) { return mbar_try_wait(bar, parity) || mbar_wait(bar, parity, abort_flag); };
+      int piece = 0, ks = 0, vs = 0;             // next stages of the two rings
+      uint32_t kp = 0, vp = 0, ready = 0;        // their parities, and those of p_ready (one bit per buffer)
+      bool ok = true;
+      while (ok && walk.next()) {
+        const int n = walk.count;
+        auto issue_s = [&](int j) {
+          if (!wait(k_full(ks), kp)) return false;
+          tc_fence_after();
+          const uint64_t kd = k_desc + ks * (2 * C::kTileBytes >> 4);
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k)
-          mma_ss(elected, tm + 64 * (j & 3), q_desc + (((k >> 2) * kQCol + (k & 3) * 32u) >> 4), kd + (((k >> 2) * kCol + (k & 3) * 32u) >> 4), idesc_s, k != 0);
-        mma_commit(elected, s_full(j & 3));
-        mma_commit(elected, k_empty(st));
-        if (j == n - 1) mma_commit(elected, q_empty);
-        return true;
-      };
-      ok = warp_wait(q_full, piece & 1, abort_flag);
-      for (int j = 0; j < min(n, 4) && ok; ++j) ok = issue_s(j);
-      // the output of the piece before has been read
-      ok = ok && (piece == 0 || warp_wait(o_free, (piece - 1) & 1, abort_flag));
-      for (int j = 0; j < n && ok; ++j) {
-        const int b = j & 3, g = j & 1, st = (it + j) % C::kStages;
-        ok = warp_wait(v_full(st), ((it + j) / C::kStages) & 1, abort_flag) && warp_wait(p_ready(b), (ready >> b) & 1, abort_flag);
-        if (!ok) break;
-        ready ^= 1u << b;
-        tc_fence_after();
-        const uint64_t vd = v_desc + st * (2 * C::kTileBytes >> 4);
+          for (int k = 0; k < D / 16; ++k)
+            umma_bf16<1>(tmem + 64 * (j & 3), q_desc + (((k >> 2) * kQCol + (k & 3) * 32u) >> 4), kd + (((k >> 2) * kCol + (k & 3) * 32u) >> 4), idesc_s, k != 0);
+          umma_commit(s_full(j & 3));
+          umma_commit(k_empty(ks));
+          if (j == n - 1) umma_commit(q_empty);
+          if (++ks == C::kStages) {
+            ks = 0;
+            kp ^= 1;
+          }
+          return true;
+        };
+        ok = wait(q_full, piece & 1);
+        for (int j = 0; j < min(n, 4) && ok; ++j) ok = issue_s(j);
+        // the output of the piece before has been read
+        ok = ok && (piece == 0 || wait(o_free, (piece - 1) & 1));
+        for (int j = 0; j < n && ok; ++j) {
+          const int b = j & 3, g = j & 1;
+          ok = wait(v_full(vs), vp) && wait(p_ready(b), (ready >> b) & 1);
+          if (!ok) break;
+          ready ^= 1u << b;
+          tc_fence_after();
+          const uint64_t vd = v_desc + vs * (2 * C::kTileBytes >> 4);
 #pragma unroll
-        for (int k = 0; k < kTileB / 16; ++k)    // 16 keys: 8 packed columns of P, 16 rows of V
-          mma_ts(elected, tm + 256 + 128 * g, tm + 64 * b + k * 8, vd + k * (2048 >> 4), idesc_pv, j >= 2 || k != 0);
-        mma_commit(elected, v_empty(st));
-        if (j + 4 < n) ok = issue_s(j + 4);
-        else mma_commit(elected, s_full(b));
+          for (int k = 0; k < kTileB / 16; ++k)  // 16 keys: 8 packed columns of P, 16 rows of V
+            umma_bf16_ts(tmem + 256 + 128 * g, tmem + 64 * b + k * 8, vd + k * (2048 >> 4), idesc_pv, j >= 2 || k != 0);
+          umma_commit(v_empty(vs));
+          if (++vs == C::kStages) {
+            vs = 0;
+            vp ^= 1;
+          }
+          if (j + 4 < n) ok = issue_s(j + 4);
+          else umma_commit(s_full(b));
+        }
+        if (ok) umma_commit(o_full);
+        ++piece;
       }
-      if (ok) mma_commit(elected, o_full);
-      it += n;
-      ++piece;
     }
+    __syncwarp();
   } else {
     // ---------------------------------------------------------------------------------------------------- softmax
     const int g = (warp - 2) >> 2, quarter = warp & 3;
@@ -1714,11 +1708,18 @@ void paged_attention(const at::Tensor& q, const at::Tensor& k_pages, const at::T
     attr.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = chained ? 1 : 0;
-    if (smem > 0) C10_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, args...));
   };
   auto launch = [&](auto dim) {
     constexpr int kD = decltype(dim)::value;
+    static std::atomic<uint64_t> ready{0};       // the shared memory sizes are set once per head dimension and device
+    const uint64_t bit = 1ull << (dev.index() & 63);
+    if (!(ready.load() & bit)) {
+      C10_CUDA_CHECK(cudaFuncSetAttribute(paged::attn_rows_kernel<kD>, cudaFuncAttributeMaxDynamicSharedMemorySize, paged::Cfg<kD>::kSmem));
+      if constexpr (kD <= 128)
+        C10_CUDA_CHECK(cudaFuncSetAttribute(paged::attn_block_kernel<kD>, cudaFuncAttributeMaxDynamicSharedMemorySize, paged::CfgB<kD>::kSmem));
+      ready.fetch_or(bit);
+    }
     if constexpr (kD <= 128)
       if (p.use_b) run(paged::attn_block_kernel<kD>, p.ctas_b, 320, paged::CfgB<kD>::kSmem, false, mq, bk, bv, p);
     run(paged::attn_rows_kernel<kD>, p.ctas_a, 160, paged::Cfg<kD>::kSmem, p.use_b, mk, mv, p);

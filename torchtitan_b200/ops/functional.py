@@ -529,9 +529,12 @@ class _QKNormRopeFn(torch.autograd.Function):
             dx, dw = ext.require().qk_norm_rope_bwd(_heads_ok(dq), _heads_ok(dk), _heads_ok(dv), *args, fp32)
         else:
             dx, dw = ref.qk_norm_rope_bwd(dq, dk, dv, *args)
-        dws = [_deliver_wgrad(w, dw[i]) if w is not None and ctx.needs_input_grad[1 + i] else None
-               for i, w in enumerate((q_weight, k_weight))]
-        return dx, dws[0], dws[1], None, None, None, None
+        if q_weight is None and k_weight is None:
+            return dx, None, None, None, None, None, None
+        need = ctx.needs_input_grad
+        dqw, dkw = dw.unbind(0)
+        return (dx, _deliver_wgrad(q_weight, dqw) if need[1] else None, _deliver_wgrad(k_weight, dkw) if need[2] else None,
+                None, None, None, None)
 
 
 def _qk_norm_rope_fwd(qkv, q_weight, k_weight, table, positions, axes, meta):
@@ -558,6 +561,8 @@ def qk_norm_rope(qkv: torch.Tensor, n_heads: int, n_kv_heads: int, q_weight: tor
     if qkv.dim() != 3 or qkv.shape[1] != n_heads + 2 * n_kv_heads:
         raise ValueError(f"qk_norm_rope: expected [T, {n_heads} + 2 * {n_kv_heads}, D], got {tuple(qkv.shape)}")
     if table is not None:
+        if positions is None:
+            raise ValueError("qk_norm_rope: a rotation needs positions")
         want = (qkv.shape[0],) if axes is None else (positions.shape[0], qkv.shape[0])
         if tuple(positions.shape) != want:
             raise ValueError(f"qk_norm_rope: positions {tuple(positions.shape)} do not fit {qkv.shape[0]} tokens"
@@ -568,7 +573,7 @@ def qk_norm_rope(qkv: torch.Tensor, n_heads: int, n_kv_heads: int, q_weight: tor
     else:
         positions = axes = None
     meta = (int(n_heads), int(n_kv_heads), bool(interleaved), float(eps), float(gain_center), float(q_scale))
-    if not torch.is_grad_enabled():
+    if not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (qkv, q_weight, k_weight))):
         _, q, k = _qk_norm_rope_fwd(qkv, q_weight, k_weight, table, positions, axes, meta)
         return q, k, qkv[:, n_heads + n_kv_heads:]
     return _QKNormRopeFn.apply(qkv, q_weight, k_weight, table, positions, axes, meta)

@@ -91,8 +91,9 @@ def page_plan(cached: torch.Tensor, new: torch.Tensor, block_table: torch.Tensor
 
 def _vectors(t: torch.Tensor) -> torch.Tensor:
     """``t`` itself when its last dimension is contiguous and every vector starts on 16 bytes, else a copy."""
-    e = t.element_size()
-    if t.stride(-1) == 1 and all(s > 0 and (s * e) % 16 == 0 for s in t.stride()[:-1]) and t.data_ptr() % 16 == 0:
+    s0, s1, s2 = t.stride()
+    n = 16 // t.element_size()
+    if s2 == 1 and s0 > 0 and s1 > 0 and s0 % n == 0 and s1 % n == 0 and t.data_ptr() % 16 == 0:
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
@@ -110,13 +111,18 @@ def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pla
               sinks: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """``q [R, Hq, D]`` -> ``[R, Hq, D]``: row ``r`` at position ``p`` of its sequence attends to the tokens
     ``max(0, p - window + 1) .. p`` (``window = 0``: all up to ``p``).  ``sinks [Hq]``: one logit per head in the softmax
-    denominator.  Rows behind the last sequence are zero, or left as they are when ``out`` is given."""
-    if q.shape[0] != plan.total_rows:
-        raise ValueError(f"paged attention: {q.shape[0]} query rows, the plan has {plan.total_rows}")
-    if tuple(k_pages.shape) != tuple(v_pages.shape) or k_pages.shape[0] != plan.num_pages or k_pages.shape[2] != plan.page_size:
+    denominator.  Rows behind the last sequence are zero, or left as they are when ``out`` is given.  For inference: no
+    gradient flows back."""
+    R, hq, D = q.shape
+    n_pages, hkv, ps, dk = k_pages.shape
+    if not scale > 0:
+        raise ValueError(f"paged attention: the scale must be positive, got {scale}")
+    if R != plan.total_rows:
+        raise ValueError(f"paged attention: {R} query rows, the plan has {plan.total_rows}")
+    if v_pages.shape != k_pages.shape or n_pages != plan.num_pages or ps != plan.page_size:
         raise ValueError(f"paged attention: pools {tuple(k_pages.shape)} / {tuple(v_pages.shape)} do not fit a plan of "
                          f"{plan.num_pages} pages of {plan.page_size}")
-    if q.shape[1] % k_pages.shape[1] or q.shape[2] != k_pages.shape[3]:
+    if hq % hkv or D != dk:
         raise ValueError(f"paged attention: queries {tuple(q.shape)} against pools {tuple(k_pages.shape)}")
     if not supported(q, k_pages):
         if q.is_cuda:
@@ -128,12 +134,14 @@ def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pla
         n = int(plan.row_start[-1])
         out[:n] = o[:n]
         return out
-    if plan.heads != (q.shape[1], k_pages.shape[1]) or int(window) not in plan.work:
-        raise ValueError(f"paged attention: {q.shape[1]} / {k_pages.shape[1]} heads with window {window}, the plan was made for "
-                         f"{plan.heads} and windows {tuple(plan.work)}")
-    _count(2)
-    dst = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
-    ext.require().paged_attention(_vectors(q), k_pages, v_pages, plan.block_table, plan.cached, plan.row_start, plan.work[int(window)],
-                                  plan.groups, plan.max_rows, float(scale), int(window),
-                                  None if sinks is None else sinks.float().contiguous(), dst, out is None)
+    work = plan.work.get(int(window))
+    if plan.heads != (hq, hkv) or work is None:
+        raise ValueError(f"paged attention: {hq} / {hkv} heads with window {window}, the plan was made for {plan.heads} and "
+                         f"windows {tuple(plan.work)}")
+    _count(3 if D <= 128 and plan.max_rows * (hq // hkv) > 16 else 2)
+    if sinks is not None and (sinks.dtype != torch.float32 or not sinks.is_contiguous()):
+        sinks = sinks.float().contiguous()
+    dst = q.new_empty((R, hq, D)) if out is None else out
+    ext.require().paged_attention(_vectors(q), k_pages, v_pages, plan.block_table, plan.cached, plan.row_start, work, plan.groups,
+                                  plan.max_rows, float(scale), int(window), sinks, dst, out is None)
     return dst
