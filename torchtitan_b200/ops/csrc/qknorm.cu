@@ -24,11 +24,11 @@ namespace qkn {
 
 constexpr int kE = 8;          // elements per lane
 constexpr int kThreads = 128;
-// Resident blocks per SM: what the registers allow without spilling (bf16 backward 5 x 4 warps; forward 6 x 4).
+// Resident blocks per SM: what the registers allow without spilling.
 template <typename T>
 constexpr int kFwdBlocks = sizeof(T) == 2 ? 6 : 4;
 template <typename T>
-constexpr int kBwdBlocks = sizeof(T) == 2 ? 5 : 4;
+constexpr int kBwdBlocks = 4;
 
 struct Params {
   const void* x;               // [T, Hq + 2 Hkv, D], row stride xs
@@ -55,7 +55,7 @@ struct Params {
 // Two fp32 values in one register pair: the packed instructions halve the arithmetic, which would else bound the kernels.
 using F2 = uint64_t;
 constexpr int kP = kE / 2;
-constexpr int kStages = 3;     // tokens in flight per warp
+constexpr int kStages = 2;     // tokens in flight per warp: the one at hand and the next (three and four gained nothing)
 __device__ __forceinline__ F2 f2(float lo, float hi) {
   F2 r;
   asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
@@ -508,6 +508,13 @@ __global__ void __launch_bounds__(1024) sum_partials_kernel(const float* __restr
   else if ((D) <= 128) { constexpr int kGroup = 16; __VA_ARGS__(); } \
   else { constexpr int kGroup = 32; __VA_ARGS__(); }
 
+// The tensor itself when its heads are adjacent and its rows start on 16 bytes, else a copy that is so.
+static at::Tensor qkn_rows(const at::Tensor& t) {
+  if (t.dim() == 3 && t.stride(2) == 1 && t.stride(1) == t.size(2) && t.stride(0) % 8 == 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0)
+    return t;
+  return t.clone(at::MemoryFormat::Contiguous);
+}
+
 static void qkn_fill(qkn::Params& p, const at::Tensor& x, int64_t hq, int64_t hkv, const c10::optional<at::Tensor>& qw,
                      const c10::optional<at::Tensor>& kw, const c10::optional<at::Tensor>& table,
                      const c10::optional<at::Tensor>& positions, const c10::optional<at::Tensor>& axes, bool interleaved,
@@ -573,16 +580,17 @@ static int qkn_grid(int64_t T, int64_t per, int per_sm) {
 // Wide warps (several heads a lane) once every resident warp still has a token to itself; a decode step of a few tokens
 // spreads over the SMs instead.
 static bool qkn_wide(const qkn::Params& p, int group) {
-  const int64_t chunk = 4 * (32 / group);
+  const int64_t chunk = 4 * (32 / group);        // of the widest warps
   return p.T * ((p.Hq + chunk - 1) / chunk + (p.Hkv + chunk - 1) / chunk) >= (int64_t)num_sms() * 16;
 }
 
-std::tuple<at::Tensor, at::Tensor> qk_norm_rope_fwd(const at::Tensor& x, int64_t hq, int64_t hkv, const c10::optional<at::Tensor>& qw,
+std::tuple<at::Tensor, at::Tensor> qk_norm_rope_fwd(const at::Tensor& x_in, int64_t hq, int64_t hkv, const c10::optional<at::Tensor>& qw,
                                                     const c10::optional<at::Tensor>& kw, const c10::optional<at::Tensor>& table,
                                                     const c10::optional<at::Tensor>& positions, const c10::optional<at::Tensor>& axes,
                                                     bool interleaved, double eps, double gain, double q_scale) {
-  TORCH_CHECK(x.is_cuda(), "qk_norm_rope: x must be a CUDA tensor");
-  c10::cuda::CUDAGuard guard(x.device());
+  TORCH_CHECK(x_in.is_cuda(), "qk_norm_rope: x must be a CUDA tensor");
+  c10::cuda::CUDAGuard guard(x_in.device());
+  const at::Tensor x = qkn_rows(x_in);
   qkn::Params p{};
   qkn_fill(p, x, hq, hkv, qw, kw, table, positions, axes, interleaved, eps, gain, q_scale);
   auto q = at::empty({p.T, hq, p.D}, x.options());
@@ -609,12 +617,13 @@ std::tuple<at::Tensor, at::Tensor> qk_norm_rope_fwd(const at::Tensor& x, int64_t
 
 // Returns dx of x's shape (contiguous) and the weight gradients [2, D] (empty without weights), fp32 or x's type.
 std::tuple<at::Tensor, at::Tensor> qk_norm_rope_bwd(const at::Tensor& dq, const at::Tensor& dk, const c10::optional<at::Tensor>& dv,
-                                                    const at::Tensor& x, int64_t hq, int64_t hkv, const c10::optional<at::Tensor>& qw,
+                                                    const at::Tensor& x_in, int64_t hq, int64_t hkv, const c10::optional<at::Tensor>& qw,
                                                     const c10::optional<at::Tensor>& kw, const c10::optional<at::Tensor>& table,
                                                     const c10::optional<at::Tensor>& positions, const c10::optional<at::Tensor>& axes,
                                                     bool interleaved, double eps, double gain, double q_scale, bool fp32_dw) {
-  TORCH_CHECK(x.is_cuda(), "qk_norm_rope: x must be a CUDA tensor");
-  c10::cuda::CUDAGuard guard(x.device());
+  TORCH_CHECK(x_in.is_cuda(), "qk_norm_rope: x must be a CUDA tensor");
+  c10::cuda::CUDAGuard guard(x_in.device());
+  const at::Tensor x = qkn_rows(x_in);
   qkn::Params p{};
   qkn_fill(p, x, hq, hkv, qw, kw, table, positions, axes, interleaved, eps, gain, q_scale);
   auto grad = [&](const at::Tensor& g, int64_t heads, int64_t& stride) -> const void* {
@@ -629,9 +638,10 @@ std::tuple<at::Tensor, at::Tensor> qk_norm_rope_bwd(const at::Tensor& dq, const 
   auto dx = at::empty({p.T, hq + 2 * hkv, p.D}, x.options());
   auto dw = at::empty({has_w ? 2 : 0, p.D}, fp32_dw ? x.options().dtype(at::kFloat) : x.options());
   if (p.T == 0) return {dx, dw.zero_()};
-  p.dq = grad(dq, hq, p.dqs);
-  p.dk = grad(dk, hkv, p.dks);
-  if (dv.has_value()) p.dv = grad(*dv, hkv, p.dvs);
+  const at::Tensor dq_ = qkn_rows(dq), dk_ = qkn_rows(dk), dv_ = dv.has_value() ? qkn_rows(*dv) : at::Tensor();
+  p.dq = grad(dq_, hq, p.dqs);
+  p.dk = grad(dk_, hkv, p.dks);
+  if (dv_.defined()) p.dv = grad(dv_, hkv, p.dvs);
   p.dx = dx.data_ptr();
   auto stream = at::cuda::getCurrentCUDAStream();
   at::Tensor partial;
@@ -647,10 +657,13 @@ std::tuple<at::Tensor, at::Tensor> qk_norm_rope_bwd(const at::Tensor& dq, const 
       }
       const int smem = qkn::kThreads / 32 * qkn::kStages * 2 * kHeads * 32 * qkn::kE * (int)x.element_size();
       if (x.scalar_type() == at::kBFloat16) qkn::bwd_kernel<__nv_bfloat16, kGroup, kHeads><<<grid, qkn::kThreads, smem, stream>>>(p);
-      else qkn::bwd_kernel<float, kGroup, kHeads><<<grid, qkn::kThreads, smem, stream>>>(p);
+      else if constexpr (kHeads <= 2) qkn::bwd_kernel<float, kGroup, kHeads><<<grid, qkn::kThreads, smem, stream>>>(p);
     };
-    if (qkn_wide(p, kGroup)) launch(std::integral_constant<int, 2>{});
-    else launch(std::integral_constant<int, 1>{});
+    // four heads a lane read a token's cos / sin half as often as two: 65 -> 61 us (8192 tokens, 32 + 4 heads of 128), 54 -> 43 us
+    // (4097 tokens, 16 + 4 heads of 256, three axes); fp32 vectors are twice as long and keep to two
+    if (!qkn_wide(p, kGroup)) launch(std::integral_constant<int, 1>{});
+    else if (x.scalar_type() == at::kBFloat16) launch(std::integral_constant<int, 4>{});
+    else launch(std::integral_constant<int, 2>{});
   });
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   if (has_w) {

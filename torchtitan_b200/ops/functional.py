@@ -498,22 +498,13 @@ def rope_qk_(qkv: torch.Tensor, table: torch.Tensor, positions: torch.Tensor, in
 # =====================================================================
 # Per-head norms of queries and keys + RoPE
 # =====================================================================
-def _heads_ok(t: torch.Tensor) -> torch.Tensor:
-    """``t[T, H, D]`` with adjacent heads and 16-byte aligned rows, copied only when it is not."""
-    T, H, D = t.shape
-    s0, s1, s2 = t.stride()
-    if s2 == 1 and s1 == D and s0 % 8 == 0 and t.data_ptr() % 16 == 0:
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
-
-
 class _QKNormRopeFn(torch.autograd.Function):
     """Keeps the projection output only: the backward reads it in any case and recomputes each head's rsqrt."""
 
     @staticmethod
     def forward(ctx, qkv, q_weight, k_weight, table, positions, axes, meta):
-        x, q, k = _qk_norm_rope_fwd(qkv, q_weight, k_weight, table, positions, axes, meta)
-        ctx.save_for_backward(x, q_weight, k_weight, table, positions, axes)
+        q, k = _qk_norm_rope_fwd(qkv, q_weight, k_weight, table, positions, axes, meta)
+        ctx.save_for_backward(qkv, q_weight, k_weight, table, positions, axes)
         ctx.meta = meta
         return q, k, qkv[:, meta[0] + meta[1]:]
 
@@ -526,7 +517,7 @@ class _QKNormRopeFn(torch.autograd.Function):
             _count(2 if weights else 1)
             # the gradient is rounded once, to the type that receives it
             fp32 = any(w.main_grad.dtype == torch.float32 for w in weights if getattr(w, "main_grad", None) is not None)
-            dx, dw = ext.require().qk_norm_rope_bwd(_heads_ok(dq), _heads_ok(dk), _heads_ok(dv), *args, fp32)
+            dx, dw = ext.require().qk_norm_rope_bwd(dq, dk, dv, *args, fp32)
         else:
             dx, dw = ref.qk_norm_rope_bwd(dq, dk, dv, *args)
         if q_weight is None and k_weight is None:
@@ -538,12 +529,11 @@ class _QKNormRopeFn(torch.autograd.Function):
 
 
 def _qk_norm_rope_fwd(qkv, q_weight, k_weight, table, positions, axes, meta):
-    """``(qkv as the kernel reads it, q, k)``."""
+    hq, hkv, *rest = meta
     if not _cuda(qkv):
-        return (qkv, *ref.qk_norm_rope_fwd(qkv, meta[0], meta[1], q_weight, k_weight, table, positions, axes, *meta[2:]))
+        return ref.qk_norm_rope_fwd(qkv, hq, hkv, q_weight, k_weight, table, positions, axes, *rest)
     _count()
-    x = _heads_ok(qkv)
-    return (x, *ext.require().qk_norm_rope_fwd(x, meta[0], meta[1], q_weight, k_weight, table, positions, axes, *meta[2:]))
+    return ext.require().qk_norm_rope_fwd(qkv, hq, hkv, q_weight, k_weight, table, positions, axes, *rest)
 
 
 def qk_norm_rope(qkv: torch.Tensor, n_heads: int, n_kv_heads: int, q_weight: torch.Tensor | None, k_weight: torch.Tensor | None,
@@ -574,7 +564,7 @@ def qk_norm_rope(qkv: torch.Tensor, n_heads: int, n_kv_heads: int, q_weight: tor
         positions = axes = None
     meta = (int(n_heads), int(n_kv_heads), bool(interleaved), float(eps), float(gain_center), float(q_scale))
     if not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (qkv, q_weight, k_weight))):
-        _, q, k = _qk_norm_rope_fwd(qkv, q_weight, k_weight, table, positions, axes, meta)
+        q, k = _qk_norm_rope_fwd(qkv, q_weight, k_weight, table, positions, axes, meta)
         return q, k, qkv[:, n_heads + n_kv_heads:]
     return _QKNormRopeFn.apply(qkv, q_weight, k_weight, table, positions, axes, meta)
 
