@@ -354,6 +354,46 @@ def test_attention_with_extreme_scores_and_infinite_keys_outside():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("groups,window", [
+    ([(0, [(70, 1), (9, 1)])], 0),                                                  # one piece a sequence
+    ([(0, [(9000, 1), (20, 1)])], 0),                                               # parts of a long axis
+    ([(1024, [(40, 1), (700, 1), (3, 1)]), (0, [(11, 1)])], 0),                     # two sources
+    ([(4096, [(c, 1) for c in range(40)])], 0),                                     # many rows behind a prefix
+    ([(0, [(2000, 40), (5, 20)])], 0),                                              # rows of a prompt
+    ([(4096, [(c, 1) for c in range(40)])], 300),
+])
+@pytest.mark.parametrize("sinks", [False, True])
+def test_a_nan_in_sight_stays_a_nan(groups, window, sinks):
+    """A query of NaN, and a key of NaN that one row sees: those outputs are NaN, whichever way their keys are cut, and the
+    others are what they were.  A sink of minus infinity is no sink."""
+    s = _Step(groups, hq=8, hkv=2, D=128, ps=32, device="cuda", seed=7)
+    sink = s.sink if sinks else None
+    plan = s.plan((window,))
+    want, size = s.oracle(window, sink)
+
+    def check(touched):                                                             # [R, Hq]: outputs that have to be NaN
+        got = paged.attention(s.q, s.kp, s.vp, plan, s.scale, window=window, sinks=sink).cpu().double()
+        assert got[touched].isnan().all()
+        err, tol = (got - want).abs()[~touched], (2 ** -8 * want.abs() + (2 ** -8 + 2 ** -12) * size)[~touched]
+        assert (err <= tol).all()
+
+    touched = torch.zeros(s.R, s.hq, dtype=torch.bool)
+    check(touched)
+    if sinks:
+        s.check(paged.attention(s.q, s.kp, s.vp, plan, s.scale, window=window, sinks=torch.full_like(s.sink, -math.inf)), window)
+    keep = s.q[1].clone()
+    s.q[1] = math.nan
+    touched[1] = True
+    check(touched)
+    s.q[1] = keep
+    last = s.cached[0] + s.new[0] - 1                                               # only the last row of sequence 0 sees its last token
+    s.kp[s.pages_of[0][last // s.ps], 1, last % s.ps] = math.nan
+    touched[1] = False
+    touched[s.new[0] - 1, 4:] = True
+    check(touched)
+
+
+@pytest.mark.gpu
 def test_attention_past_32_bit_offsets():
     ps, D, hkv = 64, 128, 8
     n_pages = 36000                                                                  # 2.4e9 elements a pool

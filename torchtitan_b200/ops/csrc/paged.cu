@@ -841,7 +841,7 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
         for (int w = 0; w < 4; ++w) mm = fmaxf(mm, ml[(w * kRowsA + row) * 2]);
         for (int w = 0; w < 4; ++w) {
           const float mw = ml[(w * kRowsA + row) * 2];
-          ll += mw == -INFINITY ? 0.f : exp2f(mw - mm) * ml[(w * kRowsA + row) * 2 + 1];
+          ll += (mw == -INFINITY ? 1.f : exp2f(mw - mm)) * ml[(w * kRowsA + row) * 2 + 1];   // without a maximum: 0, or NaN
         }
         const int64_t rh = (int64_t)(u.row0 + pr / p.G) * p.Hq + walk.head * p.G + pr % p.G;
         if (whole && u.direct) {
@@ -850,9 +850,9 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
           if (p.sinks != nullptr) {
             const float sk = p.sinks[rh % p.Hq] * 1.4426950408889634f, top = fmaxf(sk, mm);
             f = mm == -INFINITY ? 0.f : exp2f(mm - top);
-            den = ll * f + exp2f(sk - top);
+            den = ll * f + (sk == -INFINITY ? 0.f : exp2f(sk - top));
           }
-          f = den > 0.f ? f / den : 0.f;
+          f = den == 0.f ? 0.f : f / den;        // a NaN stays one
           *reinterpret_cast<uint2*>(p.out + rh * D + d) = make_uint2(pack2bf(v.x * f, v.y * f), pack2bf(v.z * f, v.w * f));
         } else if (whole) {
           const int64_t at = (int64_t)(u.base < 0) * p.R * p.Hq + rh;
@@ -1237,9 +1237,9 @@ attn_block_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
         if (p.sinks != nullptr) {
           const float sk = p.sinks[rh % p.Hq] * 1.4426950408889634f, top = fmaxf(sk, mm);
           f = mm == -INFINITY ? 0.f : exp2f(mm - top);
-          den = ll * f + exp2f(sk - top);
+          den = ll * f + (sk == -INFINITY ? 0.f : exp2f(sk - top));
         }
-        f = den > 0.f ? f / den : 0.f;
+        f = den == 0.f ? 0.f : f / den;          // a NaN stays one
         f0 *= f;
         f1 *= f;
       }
@@ -1318,9 +1318,9 @@ __global__ void __launch_bounds__(128, 8) finish_kernel(const AttnParams p) {
     if (p.sinks != nullptr) {
       const float sk = p.sinks[rh % p.Hq] * 1.4426950408889634f, top = fmaxf(sk, m);
       f = m == -INFINITY ? 0.f : exp2f(m - top);
-      l = l * f + exp2f(sk - top);
+      l = l * f + (sk == -INFINITY ? 0.f : exp2f(sk - top));
     }
-    return l > 0.f ? f / l : 0.f;
+    return l == 0.f ? 0.f : f / l;               // a NaN stays one
   };
   if ((int)blockIdx.x < cuts) {
     const bool big = (int)blockIdx.x >= p.ctas_a;
@@ -1353,18 +1353,21 @@ __global__ void __launch_bounds__(128, 8) finish_kernel(const AttnParams p) {
           const int64_t at = part(min(i0 + i, parts - 1), row);
           v[i] = *reinterpret_cast<const float2*>(pml + at * 2);
           q[i] = *reinterpret_cast<const float4*>(po + at * D + d);
-          if (i0 + i >= parts) v[i].x = -INFINITY;
+          if (i0 + i >= parts) v[i] = make_float2(-INFINITY, 0.f);
         }
         float mn = m;
 #pragma unroll
         for (int i = 0; i < 8; ++i) mn = fmaxf(mn, v[i].x);
-        const float a = m == -INFINITY ? 0.f : exp2f(m - mn);
+        const float a = m == -INFINITY ? 1.f : exp2f(m - mn);    // there was no output before: o is 0, l is 0 or NaN
         m = mn;
         l *= a;
         o.x *= a; o.y *= a; o.z *= a; o.w *= a;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          if (v[i].x == -INFINITY) continue;     // a part without a visible key may hold anything
+          if (v[i].x == -INFINITY) {             // without a visible key the output may be anything and the sum is 0,
+            l += v[i].y;                         // without a score but NaN it is NaN
+            continue;
+          }
           const float w = exp2f(v[i].x - mn);
           l += v[i].y * w;
           o.x += q[i].x * w; o.y += q[i].y * w; o.z += q[i].z * w; o.w += q[i].w * w;
@@ -1441,8 +1444,11 @@ __global__ void __launch_bounds__(128, 8) finish_kernel(const AttnParams p) {
         src = (first ? pre.o : own.o) + at * D;
       }
       const float mn = fmaxf(m, warp_max(pm));
-      if (mn == -INFINITY) continue;
-      const float a = m == -INFINITY ? 0.f : exp2f(m - mn);
+      if (mn == -INFINITY) {                     // sums of nothing, or NaN where the scores are
+        l += warp_sum(pl);
+        continue;
+      }
+      const float a = m == -INFINITY ? 1.f : exp2f(m - mn);      // there was no output before: l is 0 or NaN
       const float w = pm == -INFINITY ? 0.f : exp2f(pm - mn);
       m = mn;
       l = l * a + warp_sum(pl * w);

@@ -10,7 +10,7 @@
 // walks over tokens: the gains and the weight gradient's sums stay in registers and a token's cos / sin are read once for
 // all its heads.  The next token's vectors are on their way into shared memory meanwhile (cp.async, kStages tokens deep):
 // with loads into registers alone a warp waited out the latency of every token, and the registers that more warps or more
-// loads in flight would // loads in flight would have needed were not there.  A lane reads back what it copied itself, so nothing is synchronised.
+// loads in flight would have needed were not there.  A lane reads back what it copied itself, so nothing is synchronised.
 // 8192 tokens, 32 + 4 heads of 128, bf16: forward 33 us for 155 MB (4.7 TB/s), backward 59 us for 247 MB (4.2 TB/s).
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
