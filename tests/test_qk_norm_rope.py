@@ -211,3 +211,42 @@ def test_captured_forward_and_backward_replay_on_new_inputs():
         graph.replay()
         for a, b in zip(got, step(fresh)):
             assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,rot,weights,dtype", [(300, 128, (True, True), torch.bfloat16), (1, 64, (True, False), torch.bfloat16),
+                                                 (70, 0, (False, True), torch.float32), (70, 32, (False, False), torch.float32)])
+def test_the_python_and_the_cpp_node_agree(T, rot, weights, dtype, monkeypatch):
+    """Gradients into ``main_grad`` and counted launches go through the node in Python, everything else through the one in C++:
+    the same kernels, so the same bits, with any of the three outputs left out, under a checkpoint and next to ``main_grad``."""
+    (x, qw, kw, table, pos, ax), grads = _case(T, 8, 2, 128, rot, dtype, "cuda")
+    qw, kw = (w if on else None for w, on in zip((qw, kw), weights))
+
+    def grads_of(used, counted, saved=False, main=False):
+        monkeypatch.setattr(OF.settings, "count_launches", counted)
+        leaves = [t.detach().clone().requires_grad_(True) if t is not None else None for t in (x, qw, kw)]
+        held = [t for t in leaves if t is not None]
+        for w in held[1:]:
+            if main:
+                w.main_grad = torch.empty_like(w.detach())
+        fn = lambda a, b, c: OF.qk_norm_rope(a, 8, 2, b, c, table, pos, False, axes=ax)
+        outs = torch.utils.checkpoint.checkpoint(fn, *leaves, use_reentrant=False) if saved else fn(*leaves)
+        torch.autograd.backward([outs[i] for i in used], [grads[i] for i in used])
+        return [outs[i].detach() for i in used] + [t.main_grad if getattr(t, "main_grad", None) is not None else t.grad for t in held]
+
+    for used in ((0, 1, 2), (0,), (1,), (2,), (1, 2)):
+        want = grads_of(used, True)
+        for got in (grads_of(used, False), grads_of(used, False, saved=True), grads_of(used, False, main=True)):
+            assert all(torch.equal(a, b) for a, b in zip(got, want, strict=True))
+
+
+@pytest.mark.gpu
+def test_only_a_weight_needs_its_gradient():
+    (x, qw, kw, table, pos, ax), grads = _case(40, 4, 2, 64, 64, torch.bfloat16, "cuda")
+    full = [t.detach().clone().requires_grad_(True) for t in (x, qw, kw)]
+    only = qw.detach().clone().requires_grad_(True)
+    q, k, _ = OF.qk_norm_rope(full[0], 4, 2, full[1], full[2], table, pos, False)
+    torch.autograd.backward([q, k], grads[:2])
+    q, k, v = OF.qk_norm_rope(x, 4, 2, only, kw, table, pos, False)
+    torch.autograd.backward([q, k], grads[:2])
+    assert torch.equal(only.grad, full[1].grad) and x.grad is None and kw.grad is None

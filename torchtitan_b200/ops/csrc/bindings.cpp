@@ -22,6 +22,10 @@ std::tuple<at::Tensor, at::Tensor> qk_norm_rope_fwd(const at::Tensor& x, int64_t
                                                     const c10::optional<at::Tensor>& kw, const c10::optional<at::Tensor>& table,
                                                     const c10::optional<at::Tensor>& positions, const c10::optional<at::Tensor>& axes,
                                                     bool interleaved, double eps, double gain, double q_scale);
+std::tuple<at::Tensor, at::Tensor, at::Tensor> qk_norm_rope(const at::Tensor& x, int64_t hq, int64_t hkv, const c10::optional<at::Tensor>& qw,
+                                                            const c10::optional<at::Tensor>& kw, const c10::optional<at::Tensor>& table,
+                                                            const c10::optional<at::Tensor>& positions, const c10::optional<at::Tensor>& axes,
+                                                            bool interleaved, double eps, double gain, double q_scale);
 std::tuple<at::Tensor, at::Tensor> qk_norm_rope_bwd(const at::Tensor& dq, const at::Tensor& dk, const c10::optional<at::Tensor>& dv,
                                                     const at::Tensor& x, int64_t hq, int64_t hkv, const c10::optional<at::Tensor>& qw,
                                                     const c10::optional<at::Tensor>& kw, const c10::optional<at::Tensor>& table,
@@ -130,6 +134,8 @@ TORCH_LIBRARY(tb200, m) {
   m.def("conv_silu_bwd(Tensor x, Tensor w, Tensor? pos, Tensor dy) -> (Tensor, Tensor)", &tb200::conv_silu_bwd);
   m.def("qk_norm_rope_fwd(Tensor x, int hq, int hkv, Tensor? qw, Tensor? kw, Tensor? table, Tensor? positions, Tensor? axes, "
         "bool interleaved, float eps, float gain, float q_scale) -> (Tensor, Tensor)", &tb200::qk_norm_rope_fwd);
+  m.def("qk_norm_rope(Tensor x, int hq, int hkv, Tensor? qw, Tensor? kw, Tensor? table, Tensor? positions, Tensor? axes, "
+        "bool interleaved, float eps, float gain, float q_scale) -> (Tensor, Tensor, Tensor)", &tb200::qk_norm_rope);
   m.def("qk_norm_rope_bwd(Tensor dq, Tensor dk, Tensor? dv, Tensor x, int hq, int hkv, Tensor? qw, Tensor? kw, Tensor? table, "
         "Tensor? positions, Tensor? axes, bool interleaved, float eps, float gain, float q_scale, bool fp32_dw) -> (Tensor, Tensor)",
         &tb200::qk_norm_rope_bwd);

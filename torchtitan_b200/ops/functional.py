@@ -499,7 +499,8 @@ def rope_qk_(qkv: torch.Tensor, table: torch.Tensor, positions: torch.Tensor, in
 # Per-head norms of queries and keys + RoPE
 # =====================================================================
 class _QKNormRopeFn(torch.autograd.Function):
-    """Keeps the projection output only: the backward reads it in any case and recomputes each head's rsqrt."""
+    """Keeps the projection output only: the backward reads it in any case and recomputes each head's rsqrt.  Runs on the
+    CPU, where the weights' gradients go to ``main_grad``, and where launches are counted; else a node in C++ does the same."""
 
     @staticmethod
     def forward(ctx, qkv, q_weight, k_weight, table, positions, axes, meta):
@@ -566,6 +567,8 @@ def qk_norm_rope(qkv: torch.Tensor, n_heads: int, n_kv_heads: int, q_weight: tor
     if not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (qkv, q_weight, k_weight))):
         q, k = _qk_norm_rope_fwd(qkv, q_weight, k_weight, table, positions, axes, meta)
         return q, k, qkv[:, n_heads + n_kv_heads:]
+    if _cuda(qkv) and not settings.count_launches and all(getattr(w, "main_grad", None) is None for w in (q_weight, k_weight)):
+        return ext.require().qk_norm_rope(qkv, n_heads, n_kv_heads, q_weight, k_weight, table, positions, axes, *meta[2:])
     return _QKNormRopeFn.apply(qkv, q_weight, k_weight, table, positions, axes, meta)
 
 
