@@ -306,6 +306,7 @@ def test_attention(device, shape, sinks):
     ([(3000 // 16 * 16, [(c, 1) for c in range(12)])], 16, 2, 256, 16, 500),
     ([(0, [(1000, 500)])], 8, 2, 128, 64, 0),                                       # a chunk of a prompt
     ([(0, [(6000, 1), (100, 1)])], 32, 1, 64, 128, 1024),
+    ([(0, [(1000, 300)])] + [(0, [(c, 1)]) for c in (5, 3000, 64, 700)], 16, 4, 128, 32, 0),     # a prompt beside single tokens
 ])
 def test_attention_long(groups, hq, hkv, D, ps, window):
     s = _Step(groups, hq=hq, hkv=hkv, D=D, ps=ps, device="cuda", seed=3)

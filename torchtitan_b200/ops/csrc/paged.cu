@@ -449,12 +449,22 @@ struct AttnParams {
   Cut* cuts;                                     // [ctas_a + ctas_b]
   int* status;
 
+  // SMs that work on list B while the others work on list A, where both have work: in proportion to the time that the
+  // lists take.  In units of an SM's time for a 64-key tile of list A (0.5 us: two CTAs, memory latency) a unit there costs 3
+  // more (its queries, its join) and a tile of list B 2 (the issuing thread).  Against one list after the other on all SMs:
+  // 4 prefixes of 8192 with 16 sequences of up to 1000 tokens behind each 69.6 -> 61.4 us, 2 of 32768 with 64 of up to 4000
+  // behind each 297 -> 262, a prompt of 512 rows beside 60 sequences of up to 8000 tokens 227 -> 209 (L2 cold).
+  __device__ __forceinline__ int sms_b() const {
+    const int64_t a = (int64_t)work[1] + 3 * (int64_t)work[0], b = 2 * (int64_t)work[5];
+    return work[1] == 0 || b == 0 ? ctas_b : max(1, min(ctas_b - 1, (int)((ctas_b * b + (a + b) / 2) / (a + b))));
+  }
   __device__ __forceinline__ List list_a(const WorkLayout& lay) const {
     const int h = use_b ? 0 : 2;
-    return {work + lay.tiles_a, reinterpret_cast<const Unit*>(work + lay.units_a), work[h], work[h + 1], ctas_a};
+    const int ctas = use_b && work[1] > 0 && work[5] > 0 ? ctas_a / ctas_b * (ctas_b - sms_b()) : ctas_a;      // some per SM
+    return {work + lay.tiles_a, reinterpret_cast<const Unit*>(work + lay.units_a), work[h], work[h + 1], ctas};
   }
   __device__ __forceinline__ List list_b(const WorkLayout& lay) const {
-    return {work + lay.tiles_b, reinterpret_cast<const Unit*>(work + lay.units_b), work[4], work[5], ctas_b};
+    return {work + lay.tiles_b, reinterpret_cast<const Unit*>(work + lay.units_b), work[4], work[5], sms_b()};
   }
 };
 
@@ -574,6 +584,11 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
   auto empty = [&](int s) { return bars + 16u * s + 8u; };
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   let_next_start();
+  const List list = p.list_a(WorkLayout(p.B, p.NG, p.max_a, p.max_b));
+  if (blockIdx.x > 0 && (int)blockIdx.x >= list.ctas) {           // block 0 waits for the other kernel below in any case
+    if (threadIdx.x == 0) p.cuts[blockIdx.x] = Cut{0, 0, 0, 0, 0};
+    return;
+  }
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kStages; ++s) {
       mbar_init(full(s), 1);
@@ -583,7 +598,6 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
     mbar_fence_init();
   }
   __syncthreads();
-  const List list = p.list_a(WorkLayout(p.B, p.NG, p.max_a, p.max_b));
   Walk walk(list, p.Hkv, blockIdx.x);
   int it = 0;
 
@@ -1383,6 +1397,7 @@ __global__ void __launch_bounds__(128, 8) finish_kernel(const AttnParams p) {
 
   const int* shared = p.work + lay.shared;
   const int n_rows = shared[p.NG], stride = (gridDim.x - cuts) * 4;
+  const List list_a = p.list_a(lay), list_b = p.list_b(lay);
   bool waited = false;
   for (int64_t i = (blockIdx.x - cuts) * 4 + (threadIdx.x >> 5); i < (int64_t)n_rows * p.Hq; i += stride) {
     const int in = (unsigned)i / (unsigned)p.Hq, h = (int)i - in * p.Hq;
@@ -1401,7 +1416,7 @@ __global__ void __launch_bounds__(128, 8) finish_kernel(const AttnParams p) {
       const int s = prefix ? p.B + g : b;
       const int ua = p.work[lay.src_a + s], ub = p.use_b ? p.work[lay.src_b + s] : -1;
       const bool big = ub >= 0;
-      const List list = big ? p.list_b(lay) : p.list_a(lay);
+      const List list = big ? list_b : list_a;
       const int u0 = big ? ub : ua;
       if (u0 < 0 || u0 >= list.n_units) return q;
       const int rows = big ? kRowsB : kRowsA, per_unit = big ? p.rows_b * p.G : kRowsA;
