@@ -250,3 +250,16 @@ def test_only_a_weight_needs_its_gradient():
     q, k, v = OF.qk_norm_rope(x, 4, 2, only, kw, table, pos, False)
     torch.autograd.backward([q, k], grads[:2])
     assert torch.equal(only.grad, full[1].grad) and x.grad is None and kw.grad is None
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("T,hq,hkv,D,rot", [
+    (1, 3, 1, 128, 128), (33, 5, 3, 64, 64),                                     # few tokens: a head a lane
+    (2600, 12, 4, 128, 128), (4800, 3, 1, 64, 32), (2400, 5, 3, 256, 64)])       # several heads a lane
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_without_eps_heads_that_do_not_fill_a_warp_keep_their_weight_gradients(device, T, hq, hkv, D, rot, dtype):
+    """A warp works on a power of two of heads; those past the last one are zeros, whose rsqrt is infinite at ``eps = 0``."""
+    if device == "cpu" and T > 100:
+        T = 100
+    ts, grads = _case(T, hq, hkv, D, rot, dtype, device)
+    _check(ts, grads, hq, hkv, dtype, False, eps=0.0)

@@ -446,7 +446,8 @@ __global__ void __launch_bounds__(kThreads, kBwdBlocks<T>) bwd_kernel(const Para
         }
         const float r = rsqrtf(group_sum<kGroup>(sum2(ss)) * inv_d + p.eps);
         const float m = -group_sum<kGroup>(sum2(dot)) * inv_d * r * r * r;      // dx = r g + m x
-        const float rs = r * scale;
+        // a head that does not exist adds nothing: its zeros would meet an infinite r without eps
+        const float rs = h0 + i * kPar < H ? r * scale : 0.f;
 #pragma unroll
         for (int j = 0; j < kP; ++j) {
           dw[j] = fma2(f2(rs, rs), mul2(dn[j], f[j]), dw[j]);
