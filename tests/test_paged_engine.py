@@ -261,3 +261,36 @@ def test_training_step_with_the_fused_norms(fused):
     assert abs(losses[0] - losses[1]) <= 2e-2 * abs(losses[0])
     for n, g in grads[0].items():
         assert (grads[1][n] - g).norm() <= 0.1 * g.norm() + 1e-6, n
+
+
+# --------------------------------------------------------------------------------------------------- batch-invariant mode
+def test_batch_invariant_mode_refuses_the_paged_cache():
+    from torchtitan_b200.experiments.rl import batch_invariant, config_registry
+
+    model = _model("llama3", "debugmodel")
+    with batch_invariant():
+        with pytest.raises(ValueError, match="batch-invariant"):
+            GenerationEngine(_paged(), model=model)
+        GenerationEngine(GenerationEngine.Config(threaded=False), model=model)
+    GenerationEngine(_paged(), model=model)
+    cfg = config_registry.rl_grpo_qwen3_0_6b_alphabet_sort_batch_invariant()
+    cfg.validate()
+    cfg.generator.kv_cache = "paged"
+    with pytest.raises(ValueError, match="contiguous"):
+        cfg.validate()
+    cfg.trainer.debug.batch_invariant = False
+    cfg.validate()
+
+
+@pytest.mark.gpu
+def test_batch_invariant_mode_refuses_paged_attention():
+    from torchtitan_b200.experiments.rl import batch_invariant
+    from torchtitan_b200.ops import paged
+
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    kp = torch.zeros(2, 2, 16, 64, device="cuda", dtype=torch.bfloat16)
+    q = torch.zeros(1, 4, 64, device="cuda", dtype=torch.bfloat16)
+    plan = paged.page_plan(i32([3]), i32([1]), i32([[0]]), i32([0]), i32([]), 16, 1, num_pages=2, mapped=i32([1]), n_heads=4, n_kv_heads=2)
+    with batch_invariant(), pytest.raises(RuntimeError, match="batch-invariant"):
+        paged.attention(q, kp, kp, plan, 0.1)
+    paged.attention(q, kp, kp, plan, 0.1)

@@ -8,8 +8,9 @@ order per output tile (no split-K, tile shape independent of M), norms and the c
 row, and the NVLink reduce-scatter sums ranks in rank order.  Attention walks the key tiles of a row in order: a
 sequence's result does not depend on the other sequences of a packed batch as long as it starts on a multiple of
 the 128-token tile (pad prompts accordingly); at other offsets the same products are grouped into different
-partial sums.  What is not invariant are the library paths (cuBLAS picks kernels by shape), so this mode makes every
-silent library route an error instead."""
+partial sums.  What is not invariant are the library paths (cuBLAS picks kernels by shape) and attention over a paged
+cache (``ops.paged``: the keys of all sequences of a step are cut into equal stretches, so a sequence's partial sums
+follow the other sequences' lengths).  This mode makes both an error instead."""
 
 from __future__ import annotations
 

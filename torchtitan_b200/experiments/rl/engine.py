@@ -114,7 +114,8 @@ class GenerationEngine(Configurable):
         sampling: SamplingConfig = field(default_factory=SamplingConfig)
         kv_cache: Literal["contiguous", "paged"] = "contiguous"
         """``paged``: keys and values live in pages of one pool per layer, one attention launch serves all sequences, and
-        requests whose prompts begin with the same pages of tokens (the samples of one group) compute and read them once."""
+        requests whose prompts begin with the same pages of tokens (the samples of one group) compute and read them once.
+        Refused in batch-invariant mode: a token's partial sums depend on the other sequences' lengths."""
         kv_cache_tokens: int = 65536
         """Paged cache: tokens of the pool.  A request is admitted when its prompt and all tokens it may still generate fit."""
         kv_page_size: int = 64
@@ -139,7 +140,10 @@ class GenerationEngine(Configurable):
         self._paged = None
         if self.config.kv_cache == "paged":
             from torchtitan_b200.models.common.attention import PagedKVCache
+            from torchtitan_b200.ops import functional as OF
 
+            if OF.settings.strict_native:
+                raise ValueError('kv_cache = "paged" is not batch-invariant (debug.batch_invariant is on): use "contiguous"')
             c = self.config
             self._paged = PagedKVCache.for_model(
                 model, tokens=c.kv_cache_tokens, max_seqs=c.max_num_seqs, max_length=min(self.max_context or c.kv_cache_tokens, c.kv_cache_tokens),

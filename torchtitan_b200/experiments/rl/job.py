@@ -118,6 +118,9 @@ class RLJob(Configurable):
                 # that need their tensor- / expert-parallel peers cannot), with own copies the pull copies full tensors
                 raise ValueError("the RL job trains with data parallelism (FSDP / HSDP); tensor, expert, context and "
                                  "pipeline parallelism are not supported here")
+            if t.debug.batch_invariant and self.generator.kv_cache == "paged":
+                raise ValueError('debug.batch_invariant needs generator.kv_cache = "contiguous": paged attention is not '
+                                 "batch-invariant")
             b = self.controller.async_loop.batcher.batch
             # the batcher's grid decides the training shapes
             t.training.max_context_length = b.seq_len

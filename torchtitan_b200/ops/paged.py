@@ -21,7 +21,7 @@ from dataclasses import dataclass, field
 import torch
 
 from . import ext, reference as ref
-from .functional import _count, _library_fallback
+from .functional import _count, _library_fallback, settings
 
 __all__ = ["PagePlan", "page_plan", "write_kv", "attention", "supported"]
 
@@ -112,7 +112,8 @@ def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pla
     """``q [R, Hq, D]`` -> ``[R, Hq, D]``: row ``r`` at position ``p`` of its sequence attends to the tokens
     ``max(0, p - window + 1) .. p`` (``window = 0``: all up to ``p``).  ``sinks [Hq]``: one logit per head in the softmax
     denominator.  Rows behind the last sequence are zero, or left as they are when ``out`` is given.  For inference: no
-    gradient flows back."""
+    gradient flows back.  Not batch-invariant on CUDA (the other sequences' lengths decide where a sequence's keys are cut
+    into partial sums), so batch-invariant mode refuses it."""
     R, hq, D = q.shape
     n_pages, hkv, ps, dk = k_pages.shape
     if not scale > 0:
@@ -134,6 +135,9 @@ def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pla
         n = int(plan.row_start[-1])
         out[:n] = o[:n]
         return out
+    if settings.strict_native:
+        raise RuntimeError("paged attention cuts a sequence's keys by the lengths of all sequences of the step, which is not "
+                           "batch-invariant (debug.batch_invariant is on)")
     work = plan.work.get(int(window))
     if plan.heads != (hq, hkv) or work is None:
         raise ValueError(f"paged attention: {hq} / {hkv} heads with window {window}, the plan was made for {plan.heads} and "
