@@ -552,3 +552,17 @@ def test_no_sequences_at_all():
     assert not paged.attention(torch.ones(3, 4, 64, device="cuda", dtype=torch.bfloat16), kp, kp, plan, 1.0).any()
     plan = paged.page_plan(e, e, table, e, e, 16, 0, num_pages=4, n_heads=4, n_kv_heads=2)
     assert paged.attention(torch.ones(0, 4, 64, device="cuda", dtype=torch.bfloat16), kp, kp, plan, 1.0).shape == (0, 4, 64)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("start", [[0, 3, 1, 4], [0, 4, 0, 4], [2, 0, 2, 4], [0, 2, 9, 9], [-1, 2, 2, 4], [4, 3, 2, 0]])
+def test_groups_out_of_order_are_flagged_and_share_nothing(start):
+    """Offsets that fall or leave the step: a sequence would belong to two groups.  Results are those without groups."""
+    s = _Step([(64, [(5, 1), (9, 1)]), (64, [(30, 2), (3, 1)])], hq=8, hkv=2, D=128, ps=16, device="cuda", pad=1)
+    want = paged.attention(s.q, s.kp, s.vp, s.plan(grouped=False), s.scale)
+    ops = ext.require()
+    assert ops.status(True) == 0
+    s.start, s.prefix = start, [64, 64, 64]
+    got = paged.attention(s.q, s.kp, s.vp, s.plan(), s.scale)
+    assert ops.status(True) & 16
+    assert torch.equal(got, want)

@@ -286,7 +286,13 @@ __global__ void __launch_bounds__(1024) work_kernel(const WorkParams p) {
     if (use > 0)
       for (int b = a + lane; b < e; b += 32) seq_group[b] = g;
   }
-  __syncthreads();
+  // Offsets out of order are flagged and nothing is shared: a sequence of two groups would be joined twice, and running
+  // row counts would leave 32 bits.
+  if (__syncthreads_or(bad)) {
+    for (int g = threadIdx.x; g < p.NG; g += blockDim.x) prefix[g] = 0;
+    for (int b = threadIdx.x; b < p.B; b += blockDim.x) seq_group[b] = -1;
+    __syncthreads();
+  }
   {
     int* shared = p.work + lay.shared;           // running row counts of the groups that share a prefix
     int rows = 0;
@@ -344,7 +350,7 @@ __global__ void __launch_bounds__(1024) work_kernel(const WorkParams p) {
       n_units += total;
     }
     if (threadIdx.x == 0) start[n_src] = n_units;
-    if (n_units > max_units - n0) {              // overlapping groups: device data that is flagged
+    if (n_units > max_units - n0) {              // no step comes near: a row belongs to at most two sources
       bad = true;
       n_units = max_units - n0;
     }

@@ -66,7 +66,7 @@ def page_plan(cached: torch.Tensor, new: torch.Tensor, block_table: torch.Tensor
     With ``n_heads`` and ``n_kv_heads`` the plan also holds what ``attention`` needs for layers of these heads, for each of
     ``windows`` (0 = no window).  ``group_start [groups + 1]`` and ``group_prefix [groups]`` declare that the sequences
     ``group_start[g] .. group_start[g + 1]`` share their first ``group_prefix[g]`` tokens: their table rows begin with the
-    same pages.  ``max_rows``: an upper bound of the new rows of one sequence or group, if the caller knows one."""
+    same pages.  Offsets that are not in order are flagged and nothing is shared.  ``max_rows``: an upper bound of the new rows of one sequence or group, if the caller knows one."""
     if page_size not in PAGE_SIZES:
         raise ValueError(f"page_plan: page_size must be one of {PAGE_SIZES}, got {page_size}")
     args = (cached, new, block_table, slots, pages, mapped, int(page_size), int(total_rows), int(num_pages))
