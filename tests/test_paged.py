@@ -566,3 +566,45 @@ def test_groups_out_of_order_are_flagged_and_share_nothing(start):
     got = paged.attention(s.q, s.kp, s.vp, s.plan(), s.scale)
     assert ops.status(True) & 16
     assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [
+    dict(groups=[(64, [(5, 1), (9, 3)]), (0, [(30, 2)]), (128, [(3, 1), (0, 2), (70, 1)]), (0, [(7, 1)]), (64, [(1, 4), (2, 1)])], hq=8, hkv=2, D=128, ps=32),
+    dict(groups=[(0, [(300, 40)]), (256, [(c, 2) for c in range(20)]), (128, [(c, 9) for c in range(5)])], hq=16, hkv=2, D=64, ps=64),
+    dict(groups=[(64, [(c, 1) for c in range(4)])] * 3, hq=16, hkv=4, D=256, ps=16),
+])
+@pytest.mark.parametrize("window", [0, 50])
+def test_a_bound_on_the_shared_rows(shape, window):
+    """Groups up to the bound share; those beyond it are attended to without sharing: the same results, whatever is claimed."""
+    s = _Step(device="cuda", pad=2, seed=11, **shape)
+    rows = [sum(s.new[a:b]) for a, b in zip(s.start, s.start[1:])]
+    sizes = [n for n, p in zip(rows, s.prefix) if p]
+    for claim in (None, s.R, sum(sizes), sum(sizes) - 1, sizes[0], sizes[0] - 1, 1, 0, -3, 10 ** 6):
+        plan = s.plan((window,), shared_rows=claim)
+        assert plan.shared_rows == (s.R if claim is None else max(0, min(claim, s.R)))
+        got = paged.attention(s.q, s.kp, s.vp, plan, s.scale, window=window, sinks=s.sink)
+        s.check(got, window, s.sink)
+        assert not got[sum(s.new):].any()
+    assert ext.require().status(True) == 0
+
+
+@pytest.mark.gpu
+def test_a_long_prompt_without_sharing_takes_little_workspace():
+    """4096 rows of 32 heads of 128: partial sums of the rows would be 136 MB."""
+    s = _Step([(0, [(0, 1)])], hq=32, hkv=8, D=128, ps=256, device="cuda")
+    q = torch.zeros(4096, 32, 128, device="cuda", dtype=torch.bfloat16)
+    kp, vp = (torch.zeros(32, 8, 256, 128, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    table = torch.arange(32, device="cuda", dtype=torch.int32).view(2, 16).contiguous()
+    i32 = lambda x: _i32(x, "cuda")
+    plan = paged.page_plan(i32([0, 64]), i32([4094, 2]), table, i32([0, 1]), i32([]), 256, 4096, num_pages=32, mapped=i32([16, 16]),
+                           group_start=i32([0, 2]), group_prefix=i32([0]), n_heads=32, n_kv_heads=8, shared_rows=0)
+    out = torch.empty_like(q)
+    paged.attention(q, kp, vp, plan, s.scale, out=out)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    paged.attention(q, kp, vp, plan, s.scale, out=out)
+    # parts: 296 CTAs x 2 x 16 rows and 148 CTAs x 2 x 128 rows of 130 floats
+    assert torch.cuda.max_memory_allocated() - before <= (296 * 32 + 148 * 256) * 130 * 4 + (1 << 20)
+    assert ext.require().status(True) == 0

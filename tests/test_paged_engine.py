@@ -294,3 +294,38 @@ def test_batch_invariant_mode_refuses_paged_attention():
     with batch_invariant(), pytest.raises(RuntimeError, match="batch-invariant"):
         paged.attention(q, kp, kp, plan, 0.1)
     paged.attention(q, kp, kp, plan, 0.1)
+
+
+# ------------------------------------------------------------------------------------- groups and their workspace in a step
+def _step_plan(cache, slots, rows):
+    cache.begin_step(slots, rows)
+    plan = cache.plan
+    cache.end_step()
+    return plan
+
+
+def test_a_step_that_shares_nothing_has_no_groups():
+    """Workspace for rows of sharing groups is there for those rows only: not in a step whose sequences are alone, not in the step
+    that computes a prefix, and not for a long prompt beside a group."""
+    kw = dict(tokens=2048, max_seqs=8, max_length=1024, page_size=16, device="cpu")
+    prompt = list(range(40))
+    for share in (True, False):
+        cache = PagedKVCache((4, 2), (0,), share_prefixes=share, **kw)
+        a, b = (cache.add(p, 20)[0] for p in (prompt, [7] * 35))
+        plan = _step_plan(cache, [a, b], [40, 35])
+        assert (plan.groups, plan.shared_rows, plan.max_rows) == (0, 0, 40)
+        c, n = cache.add(prompt + [9], 20)
+        assert n == (32 if share else 0)
+        plan = _step_plan(cache, [a, c, b], [1, 41 - n, 1])
+        assert (plan.groups, plan.shared_rows) == ((2, 10) if share else (0, 0)) and plan.max_rows == (10 if share else 41)
+    cache = PagedKVCache((4, 2), (0,), **kw)
+    (a, _), (b, n) = cache.add(prompt, 20), cache.add(prompt, 20)
+    assert _step_plan(cache, [a, b], [40, 40 - n]).groups == 0            # the prefix is among the new rows of this step
+    long, _ = cache.add([5] * 700, 20)
+    plan = _step_plan(cache, [long, a, b], [700, 1, 1])
+    assert (plan.groups, plan.shared_rows, plan.max_rows) == (2, 2, 700)
+    other, _ = cache.add([6] * 50, 20)
+    plan = _step_plan(cache, [a, b, long, other], [1, 1, 1, 50])
+    assert (plan.groups, plan.shared_rows) == (2, 2)                      # the two single sequences are one group without a prefix
+    plan = _step_plan(cache, [a, b, long], [1, 0, 1])                     # one member of the group waits this step out
+    assert (plan.groups, plan.shared_rows) == (0, 0)

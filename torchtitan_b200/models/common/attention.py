@@ -219,8 +219,8 @@ class PagedKVCache:
         from torchtitan_b200.ops import paged
 
         ps = self.page_size
-        cached, mapped, pages, start, prefix, last = [], [], [], [], [], None
-        for i, (s, n) in enumerate(zip(slots, rows)):
+        cached, mapped, pages = [], [], []
+        for s, n in zip(slots, rows):
             c, m = self._length[s], self._mapped[s]
             end = -(-(c + n) // ps)
             if c + n > self.max_length or end > len(self._pages[s]):
@@ -229,21 +229,38 @@ class PagedKVCache:
             mapped.append(m)
             pages += self._pages[s][m:end]
             self._mapped[s] = max(m, end)
-            g = self._group.get(s)
-            if g is None or g != last:
-                start.append(i)
-                prefix.append(0 if g is None else g[1])
-            last = g
+        start, prefix, shared_rows, longest = self._prefix_groups(slots, rows, cached)
         B, NG = len(slots), len(start)
-        flat = torch.tensor(cached + rows + slots + mapped + start + [B] + prefix + pages, dtype=torch.int32)
+        flat = torch.tensor(cached + rows + slots + mapped + pages + start + [B] * (NG > 0) + prefix, dtype=torch.int32)
         if self.device.type == "cuda":
             flat = flat.pin_memory().to(self.device, non_blocking=True)
-        c, r, s, m, st, pr, pg = flat.split([B, B, B, B, NG + 1, NG, len(pages)])
-        group_rows = [sum(rows[a:b]) for a, b in zip(start, start[1:] + [B])]
+        c, r, s, m, pg, st, pr = flat.split([B, B, B, B, len(pages), NG + (NG > 0), NG])
+        groups = dict(group_start=st, group_prefix=pr, shared_rows=shared_rows) if NG else {}
         self.plan = paged.page_plan(c, r, self.block_table, s, pg, ps, sum(rows), num_pages=self.num_pages, mapped=m,
-                                    group_start=st, group_prefix=pr, n_heads=self.heads[0], n_kv_heads=self.heads[1],
-                                    windows=self.windows, max_rows=max(group_rows))
+                                    n_heads=self.heads[0], n_kv_heads=self.heads[1], windows=self.windows, max_rows=longest,
+                                    **groups)
         self._step = (list(slots), list(rows))
+
+    def _prefix_groups(self, slots: list[int], rows: list[int], cached: list[int]) -> tuple[list[int], list[int], int, int]:
+        """``(first sequences, prefixes, rows that share, most rows of one group or sequence)`` of a step.  Only neighbours
+        that have a common prefix in their pages already are a group with one; everything between two of them is one
+        group without a prefix, and a step in which nothing is shared has no groups."""
+        start, prefix, shared_rows, longest, i = [], [], 0, max(rows, default=0), 0
+        while i < len(slots):
+            g, j = self._group.get(slots[i]), i + 1
+            while j < len(slots) and g is not None and self._group.get(slots[j]) == g:
+                j += 1
+            live = [k for k in range(i, j) if rows[k] > 0]
+            if g is not None and len(live) > 1 and min(cached[k] for k in live) > 0:
+                start.append(i)
+                prefix.append(g[1])
+                shared_rows += sum(rows[i:j])
+                longest = max(longest, sum(rows[i:j]))
+            elif not prefix or prefix[-1]:
+                start.append(i)
+                prefix.append(0)
+            i = j
+        return (start, prefix, shared_rows, longest) if shared_rows else ([], [], 0, longest)
 
     def end_step(self) -> None:
         for s, n in zip(*self._step):

@@ -226,7 +226,8 @@ constexpr int kFewPairs = 16;
 
 struct __align__(16) Unit {
   int row0, pairs, pair0, slot;                  // first row and pair count of the source, first pair of the unit, table row
-  int key_lo, key_hi, base, direct;              // keys [lo, hi); position of the source's first row, or -1 for a prefix; alone
+  int key_lo, key_hi, base, shared;              // keys [lo, hi); position of the source's first row, or -1 for a prefix;
+                                                 // number of that row among the rows of sharing groups, -1 = not one
 };
 
 // Layout of the int32 work buffer (one per window), from the sizes that the host knows.
@@ -250,6 +251,7 @@ struct WorkLayout {
 struct WorkParams {
   const int *cached, *row_start, *slots, *group_start, *group_prefix;
   int B, NG, W, ps, G, Hkv, window, max_a, max_b, rows_b;   // rows_b: token rows of a unit in list B
+  int max_shared;                                // rows of sharing groups that the caller has room for
   int* work;
   int* status;
 };
@@ -295,21 +297,29 @@ __global__ void __launch_bounds__(1024) work_kernel(const WorkParams p) {
   }
   {
     int* shared = p.work + lay.shared;           // running row counts of the groups that share a prefix
-    int rows = 0;
+    int rows = 0, kept = 0;
     for (int g0 = 0; g0 < p.NG; g0 += blockDim.x) {
       const int g = g0 + threadIdx.x;
-      int n = 0;
+      int n = 0, a = 0, e = 0;
       if (g < p.NG) {
-        const int r0 = p.row_start[min(max(p.group_start[g], 0), p.B)];
-        if (prefix[g] > 0) n = max(0, p.row_start[min(max(p.group_start[g + 1], 0), p.B)] - r0);
-        p.work[lay.group_row + g] = r0;
+        a = min(max(p.group_start[g], 0), p.B);
+        e = min(max(p.group_start[g + 1], 0), p.B);
+        if (prefix[g] > 0) n = max(0, p.row_start[e] - p.row_start[a]);
+        p.work[lay.group_row + g] = p.row_start[a];
       }
       int total;
-      const int e = block_scan(n, part, total);
-      if (g < p.NG) shared[g] = rows + e - n;
+      const int upto = rows + block_scan(n, part, total);
       rows += total;
+      if (upto > p.max_shared && n > 0) {        // no room: the group is attended to without sharing
+        n = 0;
+        prefix[g] = 0;
+        for (int b = a; b < e; ++b) seq_group[b] = -1;
+      }
+      const int upto_kept = kept + block_scan(n, part, total);
+      if (g < p.NG) shared[g] = upto_kept - n;
+      kept += total;
     }
-    if (threadIdx.x == 0) shared[p.NG] = rows;
+    if (threadIdx.x == 0) shared[p.NG] = kept;
   }
   auto source_rows = [&](int s, int& r0, int& r1) {
     if (s < p.B) {
@@ -373,7 +383,7 @@ __global__ void __launch_bounds__(1024) work_kernel(const WorkParams p) {
           const int g = seq_group[s], c = p.cached[s];
           w.slot = p.slots[s];
           w.base = c;
-          w.direct = g < 0;
+          w.shared = g < 0 ? -1 : p.work[lay.shared + g] + r0 - p.work[lay.group_row + g];
           w.key_lo = g < 0 ? 0 : prefix[g];
           if (p.window > 0) w.key_lo = max(w.key_lo, c + w.pair0 / p.G - p.window + 1);
           w.key_hi = (int)min((int64_t)c + last / p.G + 1, room);
@@ -381,7 +391,7 @@ __global__ void __launch_bounds__(1024) work_kernel(const WorkParams p) {
           const int g = s - p.B;
           w.slot = p.slots[min(leader[g], p.B - 1)];
           w.base = -1;
-          w.direct = 0;
+          w.shared = p.work[lay.shared + g];
           // the smallest position of the group's rows bounds the window of all of them
           int from = 0;
           if (p.window > 0) {
@@ -446,14 +456,20 @@ struct AttnParams {
   __nv_bfloat16* out;                            // [R, Hq, D]
   const float* sinks;                            // [Hq] or null
   const int *table, *cached, *row_start, *work;
-  int B, NG, W, R, Hq, Hkv, G, ps, num_pages, window, max_a, max_b, ctas_a, ctas_b, rows_b, ps_shift;
+  int B, NG, W, R, Hq, Hkv, G, ps, num_pages, window, max_a, max_b, ctas_a, ctas_b, rows_b, ps_shift, max_shared;
   float scale_log2;
   bool zero_tail, use_b;                         // use_b: large sources run on the tcgen05 kernel
   float *part_a, *part_a_ml;                     // [ctas_a, 2, kRowsA, D], [ctas_a, 2, kRowsA, 2]: pieces
   float *part_b, *part_b_ml;                     // [ctas_b, 2, kRowsB, D], [ctas_b, 2, kRowsB, 2]
-  float *row_o, *row_ml;                         // [2, R, Hq, D], [2, R, Hq, 2]: whole units of groups (own keys, prefix)
+  float *row_o, *row_ml;                         // [2, max_shared, Hq, D], [.., 2]: whole units of groups (own keys, prefix)
   Cut* cuts;                                     // [ctas_a + ctas_b]
   int* status;
+
+  // Where a whole unit of a group leaves a (row, query head): `pr` pairs behind the source's first; -1 without room.
+  __device__ __forceinline__ int64_t shared_at(const Unit& u, int pr, int head) const {
+    const int row = u.shared + pr / G;
+    return row < max_shared ? ((int64_t)(u.base < 0) * max_shared + row) * Hq + head * G + pr % G : -1;
+  }
 
   // SMs that work on list B while the others work on list A, where both have work: in proportion to the time that the
   // lists take.  In units of an SM's time for a 64-key tile of list A (0.5 us: two CTAs, memory latency) a unit there costs 3
@@ -563,7 +579,7 @@ struct Walk {
   // After the last piece of the stretch: how many CTAs the unit is spread over if it begins here and goes on, else 0.
   __device__ __forceinline__ Cut cut(const Unit& unit) const {
     Cut c{0, unit.row0, unit.pairs, unit.pair0, head};
-    if (first == 0 && count < unit_tiles && unit.direct) c.parts = 2 + (unit_tiles - count - 1) / per;
+    if (first == 0 && count < unit_tiles && unit.shared < 0) c.parts = 2 + (unit_tiles - count - 1) / per;
     return c;
   }
 };
@@ -864,7 +880,7 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
           ll += (mw == -INFINITY ? 1.f : exp2f(mw - mm)) * ml[(w * kRowsA + row) * 2 + 1];   // without a maximum: 0, or NaN
         }
         const int64_t rh = (int64_t)(u.row0 + pr / p.G) * p.Hq + walk.head * p.G + pr % p.G;
-        if (whole && u.direct) {
+        if (whole && u.shared < 0) {
           float den = ll;
           float f = 1.f;
           if (p.sinks != nullptr) {
@@ -875,7 +891,8 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
           f = den == 0.f ? 0.f : f / den;        // a NaN stays one
           *reinterpret_cast<uint2*>(p.out + rh * D + d) = make_uint2(pack2bf(v.x * f, v.y * f), pack2bf(v.z * f, v.w * f));
         } else if (whole) {
-          const int64_t at = (int64_t)(u.base < 0) * p.R * p.Hq + rh;
+          const int64_t at = p.shared_at(u, pr, walk.head);
+          if (at < 0) continue;
           *reinterpret_cast<float4*>(p.row_o + at * D + d) = v;
           if (d == 0) *reinterpret_cast<float2*>(p.row_ml + at * 2) = make_float2(mm, ll);
         } else {
@@ -1250,7 +1267,7 @@ attn_block_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       float f0 = m0 == -INFINITY ? 0.f : exp2f(m0 - mm), f1 = m1 == -INFINITY ? 0.f : exp2f(m1 - mm);
       const float ll = f0 * ml[r * 2 + 1] + f1 * ml[(kRowsB + r) * 2 + 1];
       const bool whole = walk.count == walk.unit_tiles;
-      const bool last = whole && u.direct;
+      const bool last = whole && u.shared < 0;
       const int64_t rh = live ? (int64_t)(u.row0 + pr / p.G) * p.Hq + walk.head * p.G + pr % p.G : 0;
       if (last) {
         float den = ll, f = 1.f;
@@ -1265,10 +1282,10 @@ attn_block_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
       }
       if (warp_live) {
         // 16 columns of the warp's 32 rows at a time go through shared memory, so that four lanes write the 64 bytes of a row
-        const int64_t at = whole ? (int64_t)(u.base < 0) * p.R * p.Hq + rh : ((int64_t)blockIdx.x * 2 + (walk.first > 0 ? 0 : 1)) * kRowsB + r;
-        if (!last && live && g == 0) *reinterpret_cast<float2*>((whole ? p.row_ml : p.part_b_ml) + at * 2) = make_float2(mm, ll);
+        const int64_t at = last ? 0 : !whole ? ((int64_t)blockIdx.x * 2 + (walk.first > 0 ? 0 : 1)) * kRowsB + r : live ? p.shared_at(u, pr, walk.head) : 0;
+        if (!last && live && g == 0 && at >= 0) *reinterpret_cast<float2*>((whole ? p.row_ml : p.part_b_ml) + at * 2) = make_float2(mm, ll);
         const int sub = lane >> 2, quad = lane & 3;
-        char* mine = !live ? nullptr : last ? reinterpret_cast<char*>(p.out + rh * D) : reinterpret_cast<char*>((whole ? p.row_o : p.part_b) + at * D);
+        char* mine = !live || at < 0 ? nullptr : last ? reinterpret_cast<char*>(p.out + rh * D) : reinterpret_cast<char*>((whole ? p.row_o : p.part_b) + at * D);
         char* dst[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k)
@@ -1402,7 +1419,7 @@ __global__ void __launch_bounds__(128, 8) finish_kernel(const AttnParams p) {
   }
 
   const int* shared = p.work + lay.shared;
-  const int n_rows = shared[p.NG], stride = (gridDim.x - cuts) * 4;
+  const int n_rows = min(shared[p.NG], p.max_shared), stride = (gridDim.x - cuts) * 4;
   const List list_a = p.list_a(lay), list_b = p.list_b(lay);
   bool waited = false;
   for (int64_t i = (blockIdx.x - cuts) * 4 + (threadIdx.x >> 5); i < (int64_t)n_rows * p.Hq; i += stride) {
@@ -1418,7 +1435,7 @@ __global__ void __launch_bounds__(128, 8) finish_kernel(const AttnParams p) {
       int step, n;
     };
     auto locate = [&](bool prefix) {
-      Parts q{p.row_o, p.row_ml, (int64_t)prefix * p.R * p.Hq + rh, 0, 0, 0};
+      Parts q{p.row_o, p.row_ml, ((int64_t)prefix * p.max_shared + in) * p.Hq + h, 0, 0, 0};
       const int s = prefix ? p.B + g : b;
       const int ua = p.work[lay.src_a + s], ub = p.use_b ? p.work[lay.src_b + s] : -1;
       const bool big = ub >= 0;
@@ -1603,7 +1620,7 @@ static int64_t max_units(int64_t B, int64_t NG, int64_t R, int64_t G, int64_t ro
 // The attention work list of a step for one window (see "Work" above).
 at::Tensor paged_work(const at::Tensor& cached, const at::Tensor& row_start, const at::Tensor& slots, const c10::optional<at::Tensor>& group_start,
                       const c10::optional<at::Tensor>& group_prefix, int64_t table_cols, int64_t page_size,
-                      int64_t total_rows, int64_t hq, int64_t hkv, int64_t window) {
+                      int64_t total_rows, int64_t hq, int64_t hkv, int64_t window, int64_t shared_rows) {
   TORCH_CHECK(cached.is_cuda(), "paged_work: CUDA tensors expected");
   const auto dev = cached.device();
   c10::cuda::CUDAGuard guard(dev);
@@ -1611,6 +1628,7 @@ at::Tensor paged_work(const at::Tensor& cached, const at::Tensor& row_start, con
   TORCH_CHECK(hkv > 0 && hq > 0 && hq % hkv == 0, "paged_work: ", hq, " query heads on ", hkv, " key heads");
   TORCH_CHECK(group_start.has_value() == group_prefix.has_value(), "paged_work: group_start and group_prefix come together");
   TORCH_CHECK(window >= 0 && window <= INT32_MAX, "paged_work: bad window");
+  TORCH_CHECK(shared_rows >= 0 && shared_rows <= total_rows, "paged_work: bad count of shared rows");
   paged::WorkParams p{};
   p.cached = int_vector(cached, B, dev, "cached");
   p.row_start = int_vector(row_start, B + 1, dev, "row_start");
@@ -1623,7 +1641,7 @@ at::Tensor paged_work(const at::Tensor& cached, const at::Tensor& row_start, con
     p.group_start = int_vector(*group_start, NG + 1, dev, "group_start");
   }
   p.B = (int)B; p.NG = (int)NG; p.W = (int)table_cols; p.ps = (int)page_size;
-  p.G = (int)(hq / hkv); p.Hkv = (int)hkv; p.window = (int)window;
+  p.G = (int)(hq / hkv); p.Hkv = (int)hkv; p.window = (int)window; p.max_shared = (int)shared_rows;
   p.max_a = (int)max_units(B, NG, total_rows, p.G, paged::kRowsA);
   p.rows_b = paged::kRowsB / p.G;
   p.max_b = (int)max_units(B, NG, total_rows, p.G, p.rows_b > 0 ? p.rows_b * p.G : paged::kRowsB);
@@ -1668,7 +1686,7 @@ static CUtensorMap query_map(const at::Tensor& q, int group, int rows) {
 }
 
 void paged_attention(const at::Tensor& q, const at::Tensor& k_pages, const at::Tensor& v_pages, const at::Tensor& table,
-                     const at::Tensor& cached, const at::Tensor& row_start, const at::Tensor& work, int64_t groups, int64_t max_rows,
+                     const at::Tensor& cached, const at::Tensor& row_start, const at::Tensor& work, int64_t groups, int64_t max_rows, int64_t shared_rows,
                      double scale, int64_t window, const c10::optional<at::Tensor>& sinks, at::Tensor out, bool zero_tail) {
   check_pages(k_pages, v_pages, "paged_attention");
   const auto dev = k_pages.device();
@@ -1687,6 +1705,7 @@ void paged_attention(const at::Tensor& q, const at::Tensor& k_pages, const at::T
     TORCH_CHECK(sinks->device() == dev && sinks->scalar_type() == at::kFloat && sinks->is_contiguous() && sinks->numel() == q.size(1),
                 "paged_attention: sinks must be a contiguous fp32 vector [Hq]");
   TORCH_CHECK(table.device() == dev && table.scalar_type() == at::kInt && table.dim() == 2 && table.is_contiguous());
+  TORCH_CHECK(shared_rows >= 0 && shared_rows <= R, "paged_attention: bad count of shared rows");
   c10::cuda::CUDAGuard guard(dev);
   if (R == 0) return;
   const int64_t B = cached.numel();
@@ -1701,6 +1720,7 @@ void paged_attention(const at::Tensor& q, const at::Tensor& k_pages, const at::T
   p.Hq = (int)q.size(1); p.Hkv = (int)k_pages.size(1); p.G = p.Hq / p.Hkv; p.ps = (int)ps; p.num_pages = (int)k_pages.size(0);
   p.ps_shift = __builtin_ctz((unsigned)ps);
   p.window = (int)window; p.scale_log2 = (float)(scale * 1.4426950408889634); p.zero_tail = zero_tail;
+  p.max_shared = groups > 0 ? (int)shared_rows : 0;
   p.max_a = (int)max_units(B, groups, R, p.G, paged::kRowsA);
   p.rows_b = paged::kRowsB / p.G;
   p.max_b = (int)max_units(B, groups, R, p.G, p.rows_b > 0 ? p.rows_b * p.G : paged::kRowsB);
@@ -1716,7 +1736,7 @@ void paged_attention(const at::Tensor& q, const at::Tensor& k_pages, const at::T
                 "paged_attention: query vectors must be 16-byte aligned");
   const auto f32 = q.options().dtype(at::kFloat);
   const int64_t na = (int64_t)p.ctas_a * 2 * paged::kRowsA, nb = p.use_b ? (int64_t)p.ctas_b * 2 * paged::kRowsB : 0;
-  const int64_t nr = groups > 0 ? 2 * R * p.Hq : 0;
+  const int64_t nr = 2 * (int64_t)p.max_shared * p.Hq;
   const int64_t n_cuts = p.ctas_a + p.ctas_b;
   auto scratch = at::empty({(na + nb + nr) * (D + 2) + 4 + n_cuts * (int64_t)(sizeof(paged::Cut) / sizeof(float))}, f32);
   p.part_a = scratch.data_ptr<float>();
@@ -1758,7 +1778,7 @@ void paged_attention(const at::Tensor& q, const at::Tensor& k_pages, const at::T
     if constexpr (kD <= 128)
       if (p.use_b) run(paged::attn_block_kernel<kD>, p.ctas_b, 320, paged::CfgB<kD>::kSmem, false, mq, bk, bv, p);
     run(paged::attn_rows_kernel<kD>, p.ctas_a, 160, paged::Cfg<kD>::kSmem, p.use_b, mk, mv, p);
-    const int64_t row_blocks = groups > 0 ? std::min<int64_t>((R * p.Hq + 3) / 4, (int64_t)num_sms() * 8) : 0;
+    const int64_t row_blocks = std::min<int64_t>(((int64_t)p.max_shared * p.Hq + 3) / 4, (int64_t)num_sms() * 8);
     run(paged::finish_kernel<kD>, p.ctas_a + (p.use_b ? p.ctas_b * paged::kSlices : 0) + row_blocks, 128, 0, true, p);
   };
   if (D == 64) launch(std::integral_constant<int, 64>{});

@@ -45,6 +45,7 @@ class PagePlan:
     heads: tuple[int, int] | None = None                                 # (query, key heads) of the attention work lists
     groups: int = 0
     max_rows: int = 0                                                    # of one sequence or group
+    shared_rows: int = 0                                                 # of all groups that share a prefix
     work: dict[int, torch.Tensor] = field(default_factory=dict)          # by window
 
 
@@ -56,7 +57,8 @@ def supported(q: torch.Tensor, k_pages: torch.Tensor) -> bool:
 def page_plan(cached: torch.Tensor, new: torch.Tensor, block_table: torch.Tensor, slots: torch.Tensor, pages: torch.Tensor,
               page_size: int, total_rows: int, *, num_pages: int, mapped: torch.Tensor | None = None,
               group_start: torch.Tensor | None = None, group_prefix: torch.Tensor | None = None, n_heads: int | None = None,
-              n_kv_heads: int | None = None, windows: tuple[int, ...] = (0,), max_rows: int | None = None) -> PagePlan:
+              n_kv_heads: int | None = None, windows: tuple[int, ...] = (0,), max_rows: int | None = None,
+              shared_rows: int | None = None) -> PagePlan:
     """Plan of one step over ``B = len(slots)`` sequences (all index tensors int32 on one device).
 
     ``pages`` are the ids handed out, in the order of the sequences: sequence ``b`` takes as many as it needs for
@@ -66,7 +68,10 @@ def page_plan(cached: torch.Tensor, new: torch.Tensor, block_table: torch.Tensor
     With ``n_heads`` and ``n_kv_heads`` the plan also holds what ``attention`` needs for layers of these heads, for each of
     ``windows`` (0 = no window).  ``group_start [groups + 1]`` and ``group_prefix [groups]`` declare that the sequences
     ``group_start[g] .. group_start[g + 1]`` share their first ``group_prefix[g]`` tokens: their table rows begin with the
-    same pages.  Offsets that are not in order are flagged and nothing is shared.  ``max_rows``: an upper bound of the new rows of one sequence or group, if the caller knows one."""
+    same pages.  Offsets that are not in order are flagged and nothing is shared.  ``max_rows``: an upper bound of the new rows of one sequence or group, if the caller knows one.
+    ``shared_rows``: the same of the rows of all groups with a prefix and two or more sequences with rows: attention needs
+    ``2 shared_rows Hq (D + 2)`` floats of workspace for them, and a group beyond the bound is attended to without sharing.
+    Both cost speed only when they are wrong."""
     if page_size not in PAGE_SIZES:
         raise ValueError(f"page_plan: page_size must be one of {PAGE_SIZES}, got {page_size}")
     args = (cached, new, block_table, slots, pages, mapped, int(page_size), int(total_rows), int(num_pages))
@@ -81,11 +86,12 @@ def page_plan(cached: torch.Tensor, new: torch.Tensor, block_table: torch.Tensor
             raise ValueError(f"page_plan: {n_heads} query heads on {n_kv_heads} key heads")
         plan.heads, plan.groups = (int(n_heads), int(n_kv_heads)), 0 if group_prefix is None else group_prefix.numel()
         plan.max_rows = int(total_rows) if max_rows is None else min(int(max_rows), int(total_rows))
+        plan.shared_rows = 0 if not plan.groups else int(total_rows) if shared_rows is None else max(0, min(int(shared_rows), int(total_rows)))
         if block_table.is_cuda:
             for w in dict.fromkeys(int(w or 0) for w in windows):
                 _count()
                 plan.work[w] = ext.require().paged_work(cached, row_start, slots, group_start, group_prefix, block_table.shape[1],
-                                                        int(page_size), int(total_rows), *plan.heads, w)
+                                                        int(page_size), int(total_rows), *plan.heads, w, plan.shared_rows)
     return plan
 
 
@@ -147,5 +153,5 @@ def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pla
         sinks = sinks.float().contiguous()
     dst = q.new_empty((R, hq, D)) if out is None else out
     ext.require().paged_attention(_vectors(q), k_pages, v_pages, plan.block_table, plan.cached, plan.row_start, work, plan.groups,
-                                  plan.max_rows, float(scale), int(window), sinks, dst, out is None)
+                                  plan.max_rows, plan.shared_rows, float(scale), int(window), sinks, dst, out is None)
     return dst
