@@ -329,3 +329,60 @@ def test_a_step_that_shares_nothing_has_no_groups():
     assert (plan.groups, plan.shared_rows) == (2, 2)                      # the two single sequences are one group without a prefix
     plan = _step_plan(cache, [a, b, long], [1, 0, 1])                     # one member of the group waits this step out
     assert (plan.groups, plan.shared_rows) == (0, 0)
+
+
+# -------------------------------------------------------------------------------------------------- flags of a step's kernels
+def test_flags_are_taken_on_the_models_device(monkeypatch):
+    """An engine on another GPU than the current one looks at that GPU's flags, and leaves those of others alone."""
+    from contextlib import contextmanager
+    from types import SimpleNamespace
+
+    from torchtitan_b200.ops import ext
+
+    at, asked, bits = [None], [], [0]
+
+    @contextmanager
+    def device(d):
+        at[0] = d
+        yield
+        at[0] = None
+
+    def take(mask):
+        asked.append((at[0], mask))
+        return bits[0] & mask
+
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(ext, "require", lambda: SimpleNamespace(take_status=take))
+    eng = GenerationEngine(_paged(), model=_model("llama3", "debugmodel"))
+    dev = torch.device("cuda:1")
+    for bits[0], said in ((15, None), (16, "out of range"), (32, "wait"), (63, "out of range")):
+        if said:
+            with pytest.raises(RuntimeError, match=said):
+                eng._check_pages(dev)
+        else:
+            eng._check_pages(dev)
+    assert asked == [(dev, 48)] * 4
+
+
+@pytest.mark.gpu
+def test_flags_are_read_behind_the_stream_of_the_step():
+    """Bad pages of a step on a side stream that is still at work, beside a flag of somebody else."""
+    from torchtitan_b200.experiments.rl.engine import place_model_
+    from torchtitan_b200.ops import ext, paged
+
+    ops = ext.require()
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    args = (i32([0]), i32([1]), i32([[0]]), i32([0]), i32([7]), 16, 1)              # page 7 of a pool of two
+    eng = GenerationEngine(_paged(), model=place_model_(_model("llama3", "debugmodel"), "cuda", torch.bfloat16))
+    dev = torch.device("cuda")
+    ops.status(True)
+    OF.rope(torch.zeros(1, 1, 64, device="cuda"), torch.zeros(4, 64, device="cuda"), torch.tensor([9], device="cuda"), False)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(50_000_000)                                               # some 25 ms
+        paged.page_plan(*args, num_pages=2)
+        with pytest.raises(RuntimeError, match="out of range"):
+            eng._check_pages(dev)
+        eng._check_pages(dev)
+    assert ops.status(False) == 1 and ops.take_status(15) == 1 and ops.status(True) == 0

@@ -325,13 +325,14 @@ class GenerationEngine(Configurable):
         return len(seqs)
 
     def _check_pages(self, device) -> None:
-        """The kernels skip a page or slot that is out of range and flag it; the tokens of such a step are not used."""
+        """The kernels skip a page or slot that is out of range and flag it; the tokens of such a step are not used.  The
+        flags are those of the model's device, read behind the step on its stream, and only the paged kernels' own."""
         if device.type == "cuda":
             from torchtitan_b200.ops import ext
 
-            bits = int(ext.require().status(False))
-            if bits & 20:
-                ext.require().status(True)
+            with torch.cuda.device(device):
+                bits = int(ext.require().take_status(48))
+            if bits:
                 raise RuntimeError("paged cache: " + ("a page table entry was out of range" if bits & 16 else
                                                       "a bounded wait inside the attention kernels expired"))
 

@@ -43,6 +43,7 @@ void paged_attention(const at::Tensor& q, const at::Tensor& k_pages, const at::T
                      const at::Tensor& cached, const at::Tensor& row_start, const at::Tensor& work, int64_t groups, int64_t max_rows, int64_t shared_rows,
                      double scale, int64_t window, const c10::optional<at::Tensor>& sinks, at::Tensor out, bool zero_tail);
 int64_t status(bool clear);
+int64_t take_status(int64_t mask);
 at::Tensor cross_entropy_(at::Tensor logits, const at::Tensor& labels, const at::Tensor& scale);
 void adamw_(at::Tensor master, const at::Tensor& grad, at::Tensor exp_avg, at::Tensor exp_avg_sq,
             const c10::optional<at::Tensor>& lowp, const at::Tensor& grad_scale, double lr, double beta1,
@@ -147,6 +148,7 @@ TORCH_LIBRARY(tb200, m) {
   m.def("paged_attention(Tensor q, Tensor k_pages, Tensor v_pages, Tensor table, Tensor cached, Tensor row_start, Tensor work, "
         "int groups, int max_rows, int shared_rows, float scale, int window, Tensor? sinks, Tensor(a!) out, bool zero_tail) -> ()", &tb200::paged_attention);
   m.def("status(bool clear) -> int", &tb200::status);
+  m.def("take_status(int mask) -> int", &tb200::take_status);
   m.def("cross_entropy_(Tensor(a!) logits, Tensor labels, Tensor scale) -> Tensor", &tb200::cross_entropy_);
   m.def("adamw_(Tensor(a!) master, Tensor grad, Tensor(b!) exp_avg, Tensor(c!) exp_avg_sq, Tensor(d!)? lowp, "
         "Tensor grad_scale, float lr, float beta1, float beta2, float eps, float weight_decay, float bc1, float bc2) -> ()",

@@ -16,6 +16,7 @@ enum StatusBits : int {
   kStatusLabelOutOfRange = 1 << 1,
   kStatusWaitTimedOut = 1 << 2,
   kStatusPagePlanInvalid = 1 << 4,  // a page table, slot or page id outside its range, or too few pages or columns
+  kStatusPagedWaitTimedOut = 1 << 5,  // the waits of paged attention: who generates looks for them, not the trainer
 };
 
 struct __align__(16) bf16x8 {

@@ -587,4 +587,15 @@ int64_t status(bool clear) {
   return v;
 }
 
+__global__ void take_status_kernel(int mask, int* out) { *out = atomicAnd(&g_status_word, ~mask) & mask; }
+
+// The bits of `mask`, which are cleared; the others stay for those who look for them.  Behind the work that the current
+// stream of the current device has queued, which `status` is only where that is the default stream.
+int64_t take_status(int64_t mask) {
+  auto out = at::empty({1}, at::TensorOptions().dtype(at::kInt).device(at::kCUDA));
+  take_status_kernel<<<1, 1, 0, at::cuda::getCurrentCUDAStream()>>>((int)mask, out.data_ptr<int>());
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return out.item<int>();
+}
+
 }  // namespace tb200

@@ -906,7 +906,7 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
   }
   wait_for_earlier();                            // the tcgen05 kernel runs at the same time; what follows needs both
   __syncthreads();
-  if (threadIdx.x == 0 && *abort_flag) atomicOr(p.status, kStatusWaitTimedOut);
+  if (threadIdx.x == 0 && *abort_flag) atomicOr(p.status, kStatusPagedWaitTimedOut);
 }
 
 // Many rows behind one key range (a prefix with the rows of its group, the rows of a prompt chunk): tcgen05.
@@ -1333,7 +1333,7 @@ attn_block_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
-  if (threadIdx.x == 0 && *abort_flag) atomicOr(p.status, kStatusWaitTimedOut);
+  if (threadIdx.x == 0 && *abort_flag) atomicOr(p.status, kStatusPagedWaitTimedOut);
 }
 
 // Joins what the attention kernels left in parts.  Blocks [0, cuts): a sequence that shares nothing is in parts where a

@@ -10,8 +10,9 @@ Sequences that share a prefix (their tables begin with the same pages) may be pa
 is then attended to once for all rows of the group and merged with what follows it.
 
 Lengths and tables live on the device and are checked there: an entry that is out of range is skipped (its row gets slot
--1) and bit 16 of ``torch.ops.tb200.status`` is set.  On CPU tensors the plain forms of ``ops/reference.py`` run, which
-raise instead.
+-1) and 16 is set in ``torch.ops.tb200.status`` (32: a bounded wait inside an attention kernel ran out);
+``torch.ops.tb200.take_status(48)`` reads and clears these two behind the current stream's work.  On CPU tensors the plain
+forms of ``ops/reference.py`` run, which raise instead.
 """
 
 from __future__ import annotations

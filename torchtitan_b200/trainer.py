@@ -482,7 +482,7 @@ class Trainer(Configurable):
 
         if self.device.type == "cuda" and ext.available():
             ops = ext.require()
-            bits = int(ops.status(True)) | int(ops.gemm_status(True)) | int(ops.flash_status(True))
+            bits = int(ops.take_status(15)) | int(ops.gemm_status(True)) | int(ops.flash_status(True))
             if bits & 4:
                 raise RuntimeError(f"a bounded wait inside a kernel pipeline expired (status {bits:#x}): results of this "
                                    "step are incomplete")
