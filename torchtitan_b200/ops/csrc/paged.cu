@@ -539,7 +539,8 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
   return __all_sync(0xffffffffu, tc::mbar_wait(bar, parity, abort_flag));
 }
 
-// After an abort: the copies of the last tiles are waited for (with a limit) before the block may end.
+// After an abort, whichever role it came from and however far the producer had got: the copies of the last tiles are waited
+// for (with a limit) before the block may end.
 template <typename F>
 __device__ __forceinline__ void drain(int it, int stages, F full) {
   volatile int quiet = 0;
@@ -659,7 +660,6 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
         page1 = page2;
       }
     }
-    if (!ok) drain(it, C::kStages, full);
   } else {
     // ---------------------------------------------------------------------------------------------------- consumers
     const int quad = lane & 3, r_lo = lane >> 2;                         // this thread's rows: r_lo and r_lo + 8
@@ -906,7 +906,10 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
   }
   wait_for_earlier();                            // the tcgen05 kernel runs at the same time; what follows needs both
   __syncthreads();
-  if (threadIdx.x == 0 && *abort_flag) atomicOr(p.status, kStatusPagedWaitTimedOut);
+  if (*abort_flag) {
+    if (warp == 4) drain(it, C::kStages, full);
+    if (threadIdx.x == 0) atomicOr(p.status, kStatusPagedWaitTimedOut);
+  }
 }
 
 // Many rows behind one key range (a prefix with the rows of its group, the rows of a prompt chunk): tcgen05.
@@ -931,7 +934,7 @@ struct CfgB {
   static constexpr uint32_t kTileBytes = kTileB * D * 2;
   static constexpr uint32_t kStage = kQBytes + 2 * kStages * kTileBytes;         // fp32 rows on their way out, 2 KB a warp
   static constexpr uint32_t kBars = kStage + 8 * 2048;
-  static constexpr int kNumBars = 4 * kStages + 12;
+  static constexpr int kNumBars = 4 * kStages + 13;
   static constexpr uint32_t kMl = kBars + 8 * kNumBars + 8;      // TMEM address, abort flag
   static constexpr uint32_t kSmem = kMl + 2 * kRowsB * 2 * 4;
 };
@@ -979,7 +982,7 @@ attn_block_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
   auto v_empty = [&](int s) { return bars + 8u * (3 * C::kStages + s); };
   auto s_full = [&](int b) { return bars + 8u * (4 * C::kStages + b); };
   auto p_ready = [&](int b) { return bars + 8u * (4 * C::kStages + 4 + b); };
-  const uint32_t q_full = bars + 8u * (4 * C::kStages + 8), q_empty = q_full + 8u, o_full = q_full + 16u, o_free = q_full + 24u;
+  const uint32_t q_full = bars + 8u * (4 * C::kStages + 8), q_empty = q_full + 8u, o_full = q_full + 16u, o_free = q_full + 24u, quit = q_full + 32u;
   uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(smem + C::kBars + 8 * C::kNumBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_ptr + 1);
   float* ml = reinterpret_cast<float*>(smem + C::kMl);            // [2][kRowsB][2]
@@ -1008,6 +1011,7 @@ attn_block_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     mbar_init(q_empty, 1);
     mbar_init(o_full, 1);
     mbar_init(o_free, 8);
+    mbar_init(quit, 1);
     *abort_flag = 0;
     mbar_fence_init();
   }
@@ -1019,6 +1023,7 @@ attn_block_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_ptr;
+  int issued_k = 0, issued_v = 0, issued_q = 0;  // the producer's copies
 
   if (warp == 0) {
     // ---------------------------------------------------------------------------------------------------- producer
@@ -1030,7 +1035,7 @@ attn_block_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
     const CUtensorMap* map = kv ? &tmap_v : &tmap_k;
     const uint32_t q_bytes = (uint32_t)(p.rows_b * p.G) * D * 2;   // a whole box: rows behind the tensor are filled with zeros
     bool ok = true;
-    int it = 0, piece = 0, issued_k = 0, issued_v = 0, issued_q = 0;
+    int it = 0, piece = 0;
     while (ok && walk.next()) {
       const Unit u = list.units[walk.u];
       const int* row = p.table + (int64_t)u.slot * p.W;
@@ -1073,11 +1078,6 @@ attn_block_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
         page = page1;
         page1 = page2;
       }
-    }
-    if (*abort_flag) {
-      drain(issued_k, C::kStages, k_full);
-      drain(issued_v, C::kStages, v_full);
-      drain(issued_q, 1, [&](int) { return q_full; });
     }
   } else if (warp == 1) {
     // ---------------------------------------------------------------------------------------------------- MMA issue
@@ -1329,11 +1329,23 @@ attn_block_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
   }
   tc_fence_before();
   __syncthreads();
+  if (*abort_flag) {
+    if (warp == 0) {
+      drain(issued_k, C::kStages, k_full);
+      drain(issued_v, C::kStages, v_full);
+      drain(issued_q, 1, [&](int) { return q_full; });
+    } else if (warp == 1 && lane == 0) {         // and the MMAs, before their accumulators are given back
+      volatile int quiet = 0;
+      umma_commit(quit);
+      mbar_wait(quit, 0, &quiet);
+    }
+    if (threadIdx.x == 0) atomicOr(p.status, kStatusPagedWaitTimedOut);
+    __syncwarp();
+  }
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
-  if (threadIdx.x == 0 && *abort_flag) atomicOr(p.status, kStatusPagedWaitTimedOut);
 }
 
 // Joins what the attention kernels left in parts.  Blocks [0, cuts): a sequence that shares nothing is in parts where a
