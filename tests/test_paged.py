@@ -608,3 +608,40 @@ def test_a_long_prompt_without_sharing_takes_little_workspace():
     # parts: 296 CTAs x 2 x 16 rows and 148 CTAs x 2 x 128 rows of 130 floats
     assert torch.cuda.max_memory_allocated() - before <= (296 * 32 + 148 * 256) * 130 * 4 + (1 << 20)
     assert ext.require().status(True) == 0
+
+
+def test_the_plain_forms_raise_on_what_the_kernels_flag():
+    """Entries that were in the table before the step, slots and group offsets: nothing is read from the pool's other end."""
+    for entry in (-1, 4, 2 ** 31 - 1):
+        table = torch.tensor([[0, entry, 2]], dtype=torch.int32)
+        plan = lambda c, n, **kw: paged.page_plan(_i32([c], "cpu"), _i32([n], "cpu"), table, _i32([0], "cpu"), _i32([], "cpu"), 16, 4,
+                                                  num_pages=4, mapped=_i32([kw.pop("mapped", 3)], "cpu"), **kw)
+        with pytest.raises(ValueError, match="outside the pool"):
+            plan(20, 2)                                                 # a row of the step lies in that page
+        plan(20, 0)
+        p = plan(40, 4, n_heads=2, n_kv_heads=1)                        # a page of the past only
+        q, kp = torch.zeros(4, 2, 64), torch.zeros(4, 1, 16, 64)
+        with pytest.raises(ValueError, match="pool"):
+            paged.attention(q, kp, kp, p, 1.0)
+        with pytest.raises(ValueError, match="mapped"):
+            plan(0, 1, mapped=-1)
+        for start in ([0, 2], [1, 0], [-1, 1]):
+            with pytest.raises(ValueError, match="order"):
+                plan(40, 4, n_heads=2, n_kv_heads=1, group_start=_i32(start, "cpu"), group_prefix=_i32([16], "cpu"))
+    kp = torch.zeros(4, 1, 16, 64)
+    for slot in (-2, 64, 2 ** 40):
+        with pytest.raises(ValueError, match="slot"):
+            paged.write_kv(torch.ones(2, 1, 64), torch.ones(2, 1, 64), kp, kp, torch.tensor([5, slot]))
+    assert not kp.any()
+
+
+@pytest.mark.gpu
+def test_the_plain_form_on_the_gpu_looks_at_the_pages_first():
+    """fp32 pools take the plain form: a page outside the pool is an error on the host, before anything is indexed with it."""
+    i32 = lambda x: _i32(x, "cuda")
+    for table in ([[0, 9, 1]], [[0, -1, 1]]):
+        plan = paged.page_plan(i32([40]), i32([1]), i32(table), i32([0]), i32([]), 16, 1, num_pages=4, mapped=i32([3]), n_heads=2, n_kv_heads=1)
+        kp = torch.zeros(4, 1, 16, 64, device="cuda")
+        with pytest.raises(ValueError, match="pool"):
+            paged.attention(torch.zeros(1, 2, 64, device="cuda"), kp, kp, plan, 1.0)
+    assert ext.require().status(True) == 0

@@ -80,6 +80,10 @@ def page_plan(cached: torch.Tensor, new: torch.Tensor, block_table: torch.Tensor
         _count()
         row_start, positions, slot_map = ext.require().page_plan(*args)
     else:
+        if group_start is not None:
+            at = group_start.tolist()
+            if sorted(at) != at or at[0] < 0 or at[-1] > cached.numel():
+                raise ValueError(f"page_plan: the groups' offsets {at} are not in order")
         row_start, positions, slot_map = ref.page_plan(*args)
     plan = PagePlan(row_start, positions, slot_map, cached, slots, block_table, int(page_size), int(num_pages), int(total_rows))
     if n_heads is not None:

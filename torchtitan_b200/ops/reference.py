@@ -182,12 +182,16 @@ def page_plan(cached, new, block_table, slots, pages, mapped, page_size: int, to
         end = -(-(c + n) // page_size)
         if c < 0 or n < 0 or not 0 <= s < S or end > W:
             raise ValueError(f"page_plan: sequence of {c} + {n} tokens in slot {s} does not fit a {S} x {W} block table")
+        if have < 0:
+            raise ValueError(f"page_plan: {have} mapped columns in slot {s}")
         take = pages[at:at + max(0, end - have)]
         if len(take) < end - have or any(not 0 <= i < num_pages for i in take):
             raise ValueError("page_plan: too few pages, or a page outside the pool")
         block_table[s, have:have + len(take)] = torch.tensor(take, dtype=block_table.dtype)
         at += len(take)
         row = block_table[s].tolist()
+        if n and any(not 0 <= i < num_pages for i in row[c // page_size:end]):
+            raise ValueError(f"page_plan: slot {s} holds a page outside the pool")
         for j in range(c, c + n):
             positions.append(j)
             slot_map.append(row[j // page_size] * page_size + j % page_size)
@@ -201,8 +205,10 @@ def page_plan(cached, new, block_table, slots, pages, mapped, page_size: int, to
 
 
 def paged_write(k, v, k_pages, v_pages, slot_map) -> None:
-    live = slot_map >= 0
+    live = slot_map != -1
     ps = k_pages.shape[2]
+    if live.any() and (int(slot_map[live].min()) < 0 or int(slot_map.max()) >= k_pages.shape[0] * ps):
+        raise ValueError("paged_write: a slot outside the pool")
     page, off = slot_map[live] // ps, slot_map[live] % ps
     k_pages[page, :, off] = k[live]
     v_pages[page, :, off] = v[live]
@@ -220,6 +226,8 @@ def paged_attention(q, k_pages, v_pages, block_table, slots, cached, row_start, 
             continue
         L = c + r1 - r0
         ids = block_table[s, :-(-L // ps)].long()
+        if ids.numel() * ps < L or any(not 0 <= i < k_pages.shape[0] for i in ids.tolist()):
+            raise ValueError(f"paged attention: the pages of slot {s} do not hold {L} tokens or lie outside the pool")
         k, v = (p[ids].transpose(0, 1).reshape(Hkv, -1, D)[:, :L].transpose(0, 1) for p in (k_pages, v_pages))
         o, lse = block_attention_fwd(q[r0:r1], k, v, scale, True, c, None, window)
         if sinks is not None:
