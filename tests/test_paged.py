@@ -645,3 +645,19 @@ def test_the_plain_form_on_the_gpu_looks_at_the_pages_first():
         with pytest.raises(ValueError, match="pool"):
             paged.attention(torch.zeros(1, 2, 64, device="cuda"), kp, kp, plan, 1.0)
     assert ext.require().status(True) == 0
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_refusals_of_scales_and_windows(device):
+    """A scale that is zero or infinite in 32 bits turns masked scores into NaN."""
+    s = _Step([(0, [(5, 1)])], hq=4, hkv=2, D=64, ps=16, device=device)
+    plan = s.plan((0, 3))
+    for scale in (0.0, -1.0, 1e-46, 1e-40, 1e39, math.inf, math.nan):
+        with pytest.raises(ValueError, match="scale"):
+            paged.attention(s.q, s.kp, s.vp, plan, scale)
+    for scale in (1e-37, 1e38):
+        assert not paged.attention(s.q, torch.zeros_like(s.kp), s.vp.nan_to_num(), plan, scale).isnan().any()
+    with pytest.raises(ValueError, match="window"):
+        paged.attention(s.q, s.kp, s.vp, plan, 1.0, window=-1)
+    with pytest.raises(ValueError, match="window"):
+        s.plan((0, -2))

@@ -75,6 +75,8 @@ def page_plan(cached: torch.Tensor, new: torch.Tensor, block_table: torch.Tensor
     Both cost speed only when they are wrong."""
     if page_size not in PAGE_SIZES:
         raise ValueError(f"page_plan: page_size must be one of {PAGE_SIZES}, got {page_size}")
+    if any(int(w or 0) < 0 for w in windows):
+        raise ValueError(f"page_plan: windows {tuple(windows)} (0 = none)")
     args = (cached, new, block_table, slots, pages, mapped, int(page_size), int(total_rows), int(num_pages))
     if block_table.is_cuda:
         _count()
@@ -127,8 +129,10 @@ def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pla
     into partial sums), so batch-invariant mode refuses it."""
     R, hq, D = q.shape
     n_pages, hkv, ps, dk = k_pages.shape
-    if not scale > 0:
-        raise ValueError(f"paged attention: the scale must be positive, got {scale}")
+    if not 1.2e-38 <= scale <= 2.3e38:               # times log2(e) a normal fp32 number: masked scores stay minus infinity
+        raise ValueError(f"paged attention: the scale must be positive and finite in 32 bits, got {scale}")
+    if window < 0:
+        raise ValueError(f"paged attention: window {window} (0 = none)")
     if R != plan.total_rows:
         raise ValueError(f"paged attention: {R} query rows, the plan has {plan.total_rows}")
     if v_pages.shape != k_pages.shape or n_pages != plan.num_pages or ps != plan.page_size:
