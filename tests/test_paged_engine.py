@@ -386,3 +386,11 @@ def test_flags_are_read_behind_the_stream_of_the_step():
             eng._check_pages(dev)
         eng._check_pages(dev)
     assert ops.status(False) == 1 and ops.take_status(15) == 1 and ops.status(True) == 0
+
+
+def test_more_sequences_than_a_step_takes_are_refused_at_once():
+    """Not by the step that first has them all in flight."""
+    kw = dict(tokens=64, max_length=64, device="cpu")
+    PagedKVCache((4, 2), (0,), max_seqs=4096, **kw)
+    with pytest.raises(ValueError, match="4096"):
+        PagedKVCache((4, 2), (0,), max_seqs=4097, **kw)

@@ -104,10 +104,12 @@ class PagedKVCache:
 
     def __init__(self, heads: tuple[int, int], windows: tuple[int, ...], *, tokens: int, max_seqs: int, max_length: int,
                  page_size: int = 64, device, share_prefixes: bool = True):
-        from torchtitan_b200.ops.paged import PAGE_SIZES
+        from torchtitan_b200.ops.paged import MAX_SEQS, PAGE_SIZES
 
         if page_size not in PAGE_SIZES:
             raise ValueError(f"page size {page_size} (have {PAGE_SIZES})")
+        if max_seqs > MAX_SEQS:
+            raise ValueError(f"a paged cache for {max_seqs} sequences: a step takes at most {MAX_SEQS}")
         if tokens <= 0 or max_seqs <= 0 or max_length <= 0:
             raise ValueError("a paged cache needs tokens, sequences and a maximum length")
         self.heads, self.windows, self.page_size, self.device = heads, windows, page_size, torch.device(device)

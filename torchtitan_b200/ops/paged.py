@@ -28,6 +28,7 @@ __all__ = ["PagePlan", "page_plan", "write_kv", "attention", "supported"]
 
 PAGE_SIZES = (16, 32, 64, 128, 256)
 HEAD_DIMS = (64, 128, 256)
+MAX_SEQS = 4096                  # of one step on CUDA
 
 
 @dataclass(eq=False)
