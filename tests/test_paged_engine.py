@@ -394,3 +394,25 @@ def test_more_sequences_than_a_step_takes_are_refused_at_once():
     PagedKVCache((4, 2), (0,), max_seqs=4096, **kw)
     with pytest.raises(ValueError, match="4096"):
         PagedKVCache((4, 2), (0,), max_seqs=4097, **kw)
+
+
+def test_a_failed_pull_ends_the_sharing_too():
+    """The weights may be half replaced: later requests compute their prompts themselves."""
+    prompt = list(range(1, 40))
+
+    def source(engine):
+        raise RuntimeError("half the weights")
+
+    async def go():
+        eng = GenerationEngine(_paged(), model=_model("llama3", "debugmodel"), weight_source=source)
+        first = asyncio.create_task(eng.generate(prompt, request_id="a", sampling_config=SamplingConfig(temperature=0.0, max_tokens=9)))
+        await asyncio.sleep(0)
+        await asyncio.sleep(0)
+        assert eng._paged.shared_tokens(prompt) == 32
+        with pytest.raises(RuntimeError, match="half"):
+            await eng.pull_model_state_dict(1)
+        assert eng._paged.shared_tokens(prompt) == 0
+        await first
+        await eng.close()
+
+    _run(go())

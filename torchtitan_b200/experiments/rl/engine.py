@@ -242,10 +242,10 @@ class GenerationEngine(Configurable):
             pulls, self._pending_pull = self._pending_pull, []
         for version, fut, loop in pulls:
             try:
+                if self._paged is not None:          # new requests compute their prompts under the new weights, or what a
+                    self._paged.forget_prefixes()    # failed pull leaves of them
                 if self.weight_source is not None:
                     self.weight_source(self)
-                if self._paged is not None:
-                    self._paged.forget_prefixes()    # new requests compute their prompts under the new weights
                 self.policy_version = version
                 loop.call_soon_threadsafe(lambda f=fut: f.done() or f.set_result(None))
             except Exception as e:              # the caller of the pull sees the failure
