@@ -416,3 +416,21 @@ def test_a_failed_pull_ends_the_sharing_too():
         await eng.close()
 
     _run(go())
+
+
+def test_training_after_an_evaluation_in_inference_mode(fused):
+    """The map of position axes is made once per module; made under inference_mode it could not be saved for a backward."""
+    model = _model("qwen3_5", "debugmodel_vl", 4)
+    tokens, pos = torch.arange(12), torch.arange(12)
+
+    def run():
+        ctx = AttentionContext()
+        ctx.rope_positions = torch.stack([pos, pos % 5, pos % 3])
+        return type(model).__mro__[1].forward(model, tokens, pos, ctx)
+
+    with torch.inference_mode():
+        want = run().clone()
+    got = run()
+    got.float().square().mean().backward()
+    assert torch.equal(got.detach(), want)
+    assert all(p.grad is not None for n, p in model.named_parameters() if "q_norm" in n)

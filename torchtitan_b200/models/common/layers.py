@@ -263,7 +263,8 @@ class RoPE(Module):
                 axes = [f % 3 if f % 3 and f < 3 * secs[f % 3] else 0 for f in range(half)]
             else:
                 axes = [a for a, n in enumerate(secs) for _ in range(n)]
-            self._axes = torch.tensor(axes, dtype=torch.int32, device=positions.device)
+            with torch.inference_mode(False):            # a later backward saves it
+                self._axes = torch.tensor(axes, dtype=torch.int32, device=positions.device)
         return self._axes
 
     def forward(self, x: torch.Tensor, positions: torch.Tensor) -> torch.Tensor:
