@@ -6,7 +6,7 @@ prompts and one row for each sequence already decoding into ONE flat token strea
 it: projections, feed-forward / expert layers and the output projection see all rows together (weights are read
 once per step for all sequences), the attention core runs per sequence against that sequence's key/value cache
 (``models.common.attention.BatchedKVCache``), or with ``kv_cache = "paged"`` in one launch over all sequences' pages
-(``PagedKVCache``), where requests with the same leading tokens share them.  Only the last row of each sequence
+(``PagedKVCache``), where requests of the same prompt share its pages.  Only the last row of each sequence
 reaches the output projection.  Sampling (temperature, top-k, top-p, per-request seed) happens per sequence; a
 sequence ends on EOS, a stop token, a stop sequence (``finish_reason = "stop"``), its token limit (``"length"``) or engine shutdown (``"abort"``).
 
@@ -114,7 +114,7 @@ class GenerationEngine(Configurable):
         sampling: SamplingConfig = field(default_factory=SamplingConfig)
         kv_cache: Literal["contiguous", "paged"] = "contiguous"
         """``paged``: keys and values live in pages of one pool per layer, one attention launch serves all sequences, and
-        requests whose prompts begin with the same pages of tokens (the samples of one group) compute and read them once.
+        requests whose prompts have the same whole pages of tokens (the samples of one group) compute and read them once.
         Refused in batch-invariant mode: a token's partial sums depend on the other sequences' lengths."""
         kv_cache_tokens: int = 65536
         """Paged cache: tokens of the pool.  A request is admitted when its prompt and all tokens it may still generate fit."""

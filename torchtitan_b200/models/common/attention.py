@@ -98,9 +98,9 @@ class PagedKVCache:
     over some rows of some sequences (one H2D copy of their lengths and new page ids, the tables are built on the device),
     ``attend`` is what a layer calls, ``end_step`` advances the lengths, ``release`` ends a sequence.
 
-    Sequences admitted with the same leading tokens share the pages of the whole pages among them (all but the last token
-    at most): the later ones start behind them, and attention reads them once for all rows of the group.  Whole requests are
-    reserved at ``add`` (prompt and the tokens to come), so a sequence in flight never runs out of pages."""
+    Sequences whose prompts have the same whole pages (all but the last token at most) share those pages: the later ones start
+    behind them, and attention reads them once for all rows of the group.  The whole pages have to be equal in number, too:
+    a prompt that only begins with another's pages computes all of its own.  Whole requests are reserved at ``add`` (prompt and the tokens to come), so a sequence in flight never runs out of pages."""
 
     def __init__(self, heads: tuple[int, int], windows: tuple[int, ...], *, tokens: int, max_seqs: int, max_length: int,
                  page_size: int = 64, device, share_prefixes: bool = True):
@@ -153,7 +153,7 @@ class PagedKVCache:
         return tuple(prompt[:(len(prompt) - 1) // self.page_size * self.page_size]) if self.share_prefixes else ()
 
     def shared_tokens(self, prompt) -> int:
-        """Leading tokens of ``prompt`` that a sequence in flight has in its pages."""
+        """Leading tokens of ``prompt`` that ``add`` would take from a sequence in flight: its whole pages or nothing."""
         key = self._prefix_key(prompt)
         return len(key) if key in self._index else 0
 

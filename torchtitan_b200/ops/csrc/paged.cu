@@ -90,6 +90,7 @@ struct PlanParams {
 // the rows and of the newly handed out table entries.  A page that is needed for a row of this step is taken from the
 // hand-out list, not from the table, which another block may still be writing.  Latency bound: a launch, one scan and
 // one round of dependent loads: 6 us for 9 sequences, 8 us for 500 sequences with 50 thousand rows, launch included.
+// The work list (work_kernel) is a launch of its own per step and window.
 __global__ void __launch_bounds__(256) plan_kernel(const PlanParams p) {
   extern __shared__ int sm[];
   int* row_start = sm;                 // [B + 1]
@@ -256,6 +257,9 @@ struct WorkParams {
   int* status;
 };
 
+// One block, because a unit's place follows from a scan over all sources and then all units; latency bound.  Device time of a
+// replayed graph beside the tables' kernel: 4 us for 9 or 61 single rows, 10 us for 4 prefixes of 16 sequences, 24 us for a
+// prompt of 32768 rows (8200 units of 16 pairs), 39 us for 500 sequences of up to 200 rows.
 __global__ void __launch_bounds__(1024) work_kernel(const WorkParams p) {
   extern __shared__ int sm[];
   const int n_src = p.B + p.NG;
@@ -475,7 +479,8 @@ struct AttnParams {
   // lists take.  In units of an SM's time for a 64-key tile of list A (0.5 us: two CTAs, memory latency) a unit there costs 3
   // more (its queries, its join) and a tile of list B 2 (the issuing thread).  Against one list after the other on all SMs:
   // 4 prefixes of 8192 with 16 sequences of up to 1000 tokens behind each 69.6 -> 61.4 us, 2 of 32768 with 64 of up to 4000
-  // behind each 297 -> 262, a prompt of 512 rows beside 60 sequences of up to 8000 tokens 227 -> 209 (L2 cold).
+  // behind each 297 -> 262, a prompt of 512 rows beside 60 sequences of up to 8000 tokens 227 -> 209 (L2 cold).  It can lose: 4
+  // prefixes of 65536 with 32 sequences behind each 233.5 -> 241.7.  The weights were found with heads of 128.
   __device__ __forceinline__ int sms_b() const {
     const int64_t a = (int64_t)work[1] + 3 * (int64_t)work[0], b = 2 * (int64_t)work[5];
     return work[1] == 0 || b == 0 ? ctas_b : max(1, min(ctas_b - 1, (int)((ctas_b * b + (a + b) / 2) / (a + b))));
@@ -923,8 +928,12 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
 // Queries come by TMA too (boxes of rows x heads of the key head), the next piece's as soon as the last S is done.
 // The exponentials (64 x 128 per tile on a 16-per-clock unit) and the MMAs take 512 clocks a tile each; the issuing thread's
 // own work (two waits, twelve MMAs of 60 to 75 clocks, three commits) takes some 1700 and bounds the kernel: 4 groups of
-// 16 sequences behind 65536 tokens, 4 key heads: 139 us for 537 MB (3.9 TB/s); one group of 64: 586 TFLOP/s; a prompt of
-// 4096 rows: 640 TFLOP/s.
+// 16 sequences behind 65536 tokens, 4 key heads: 139 us for 537 MB (3.9 TB/s); one group of 64: 586 TFLOP/s; 512 rows behind
+// 8192 tokens, 32 + 8 heads of 128: 129 us (550 TFLOP/s).  A prompt is slower: 4096 rows alone take 418 us, 329 TFLOP/s counted
+// over the keys that a row sees, some 3500 clocks a tile, which the issuing thread does not explain; what does has not been
+// measured (its units are short, 32 tiles in the mean, with one buffer for the queries and an output to drain each).  The flash
+// forward, which keeps two query tiles per tile of keys, takes 161 us.
+// P is rounded to bf16 before it meets V, as in the flash kernels: the tensor cores take the values' type.
 //   warp 0: TMA producer    warp 1: TMEM, MMA issue    warps 2..5, 6..9: softmax of even / odd tiles, then the output
 // Tensor memory: score buffer b (of warpgroup b % 2) at column 64 b, accumulator of warpgroup g at 256 + 128 g.
 template <int D>

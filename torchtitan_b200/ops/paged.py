@@ -113,7 +113,8 @@ def _vectors(t: torch.Tensor) -> torch.Tensor:
 
 
 def write_kv(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, slot_map: torch.Tensor) -> None:
-    """Store ``k, v [R, Hkv, D]`` at their slots of the pools; rows with slot -1 are left out."""
+    """Store ``k, v [R, Hkv, D]`` at their slots of the pools; rows with slot -1 are left out.  The slots of a call differ:
+    of two rows for one slot, parts of either may be left."""
     if k_pages.is_cuda:
         _count()
         ext.require().paged_write(_vectors(k), _vectors(v), k_pages, v_pages, slot_map)
@@ -125,7 +126,10 @@ def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pla
               sinks: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """``q [R, Hq, D]`` -> ``[R, Hq, D]``: row ``r`` at position ``p`` of its sequence attends to the tokens
     ``max(0, p - window + 1) .. p`` (``window = 0``: all up to ``p``).  ``sinks [Hq]``: one logit per head in the softmax
-    denominator.  Rows behind the last sequence are zero, or left as they are when ``out`` is given.  For inference: no
+    denominator.  A row that sees no key, or only scores of minus infinity, is zero; a NaN among them makes it NaN, and a *value*
+    that is not finite may make NaN of every row of its sequence in this step (of its group, when it lies in a shared
+    prefix), as 0 * inf does in any product of probabilities and values.  Probabilities are rounded to the values' bf16 before
+    the product, scores, sums and partial outputs are fp32.  Rows behind the last sequence are zero, or left as they are when ``out`` is given.  For inference: no
     gradient flows back.  Not batch-invariant on CUDA (the other sequences' lengths decide where a sequence's keys are cut
     into partial sums), so batch-invariant mode refuses it."""
     R, hq, D = q.shape
