@@ -661,3 +661,14 @@ def test_refusals_of_scales_and_windows(device):
         paged.attention(s.q, s.kp, s.vp, plan, 1.0, window=-1)
     with pytest.raises(ValueError, match="window"):
         s.plan((0, -2))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_group_arguments_come_together(device):
+    s = _Step([(0, [(5, 1)])], hq=4, hkv=2, D=64, ps=16, device=device)
+    call = lambda **kw: paged.page_plan(_i32(s.cached, device), _i32(s.new, device), s.table, _i32(s.slots, device), _i32([], device), s.ps, s.R,
+                                        num_pages=s.n_pages, mapped=_i32([1], device), n_heads=4, n_kv_heads=2, **kw)
+    for start, prefix in ((None, [0]), ([0, 1], None), ([0], [0]), ([0, 1], [0, 0]), ([], [])):
+        with pytest.raises(ValueError, match="together"):
+            call(group_start=None if start is None else _i32(start, device), group_prefix=None if prefix is None else _i32(prefix, device))
+    assert call(group_start=_i32([0], device), group_prefix=_i32([], device)).groups == 0

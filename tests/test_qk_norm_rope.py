@@ -263,3 +263,21 @@ def test_without_eps_heads_that_do_not_fill_a_warp_keep_their_weight_gradients(d
         T = 100
     ts, grads = _case(T, hq, hkv, D, rot, dtype, device)
     _check(ts, grads, hq, hkv, dtype, False, eps=0.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("hq,hkv,D,rot", [(32, 8, 128, 128), (5, 3, 64, 32), (16, 4, 256, 64)])
+def test_a_token_does_not_depend_on_the_others(dtype, hq, hkv, D, rot):
+    """Batch-invariant mode allows the operator: few tokens (a head a lane) and many (several) give a token the same bits."""
+    ts, grads = _case(5000, hq, hkv, D, rot, dtype, "cuda")
+    x, qw, kw, table, pos, _ = ts
+
+    def run(sl):
+        leaf = x[sl].detach().clone().requires_grad_(True)
+        out = OF.qk_norm_rope(leaf, hq, hkv, qw, kw, table, pos[sl].contiguous(), False)
+        return [t.detach() for t in out] + list(torch.autograd.grad(out, leaf, [g[sl] for g in grads]))
+
+    whole = run(slice(0, 5000))
+    for sl in (slice(0, 1), slice(37, 50), slice(4000, 5000)):
+        assert all(torch.equal(a, b[sl]) for a, b in zip(run(sl), whole))

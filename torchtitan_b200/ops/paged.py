@@ -76,6 +76,8 @@ def page_plan(cached: torch.Tensor, new: torch.Tensor, block_table: torch.Tensor
     Both cost speed only when they are wrong."""
     if page_size not in PAGE_SIZES:
         raise ValueError(f"page_plan: page_size must be one of {PAGE_SIZES}, got {page_size}")
+    if (group_start is None) != (group_prefix is None) or (group_start is not None and group_start.numel() != group_prefix.numel() + 1):
+        raise ValueError("page_plan: group_start [groups + 1] and group_prefix [groups] come together")
     if any(int(w or 0) < 0 for w in windows):
         raise ValueError(f"page_plan: windows {tuple(windows)} (0 = none)")
     args = (cached, new, block_table, slots, pages, mapped, int(page_size), int(total_rows), int(num_pages))
