@@ -672,3 +672,14 @@ def test_group_arguments_come_together(device):
         with pytest.raises(ValueError, match="together"):
             call(group_start=None if start is None else _i32(start, device), group_prefix=None if prefix is None else _i32(prefix, device))
     assert call(group_start=_i32([0], device), group_prefix=_i32([], device)).groups == 0
+
+
+@pytest.mark.gpu
+def test_a_negative_count_of_mapped_columns_is_flagged():
+    """The plain form raises; the kernel takes it for none."""
+    ops = ext.require()
+    ops.status(True)
+    table = torch.full((1, 3), -5, dtype=torch.int32, device="cuda")
+    p = paged.page_plan(_i32([0], "cuda"), _i32([1], "cuda"), table, _i32([0], "cuda"), _i32([2], "cuda"), 16, 1, num_pages=4, mapped=_i32([-3], "cuda"))
+    assert ops.status(True) & 16
+    assert table.tolist() == [[2, -5, -5]] and p.slot_map.tolist() == [32]

@@ -114,7 +114,7 @@ __global__ void __launch_bounds__(256) plan_kernel(const PlanParams p) {
       } else {
         const int64_t end = ((int64_t)c + n + p.ps - 1) / p.ps;
         const int have = p.mapped != nullptr ? max(0, p.mapped[b]) : (int)(((int64_t)c + p.ps - 1) / p.ps);
-        bad |= end > p.W;
+        bad |= end > p.W || (p.mapped != nullptr && p.mapped[b] < 0);
         need = (int)max((int64_t)0, min(end, (int64_t)p.W) - have);
         if (blockIdx.x == 0) bad |= (atomicOr(&seen[slot >> 5], 1u << (slot & 31)) >> (slot & 31)) & 1u;   // the same slot twice
       }
