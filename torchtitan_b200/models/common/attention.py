@@ -100,7 +100,8 @@ class PagedKVCache:
 
     Sequences whose prompts have the same whole pages (all but the last token at most) share those pages: the later ones start
     behind them, and attention reads them once for all rows of the group.  The whole pages have to be equal in number, too:
-    a prompt that only begins with another's pages computes all of its own.  Whole requests are reserved at ``add`` (prompt and the tokens to come), so a sequence in flight never runs out of pages."""
+    a prompt that only begins with another's pages computes all of its own.  Whole requests are reserved at ``add`` (prompt
+    and the tokens to come), so a sequence in flight never runs out of pages."""
 
     def __init__(self, heads: tuple[int, int], windows: tuple[int, ...], *, tokens: int, max_seqs: int, max_length: int,
                  page_size: int = 64, device, share_prefixes: bool = True):

@@ -3,7 +3,8 @@
 // The same forward and backward as a Python function of two operator calls, without the interpreter between them.  A forward
 // and backward of 8 tokens takes 126 us of host time through the Python function and 103 us through this node (55 us of it
 // for any operator and its gradient), more than the kernels of a short sequence (17 us for 1023 tokens, 16 + 8 heads of
-// 64).  Weights with a `main_grad` (the sharded engine's) take the Python function.  Only the projection output is kept; the backward recomputes each head's rsqrt from it.
+// 64).  Weights with a `main_grad` (the sharded engine's) take the Python function.  Only the projection output is kept;
+// the backward recomputes each head's rsqrt from it.
 #include <torch/csrc/autograd/custom_function.h>
 
 #include <ATen/ATen.h>

@@ -70,10 +70,10 @@ def page_plan(cached: torch.Tensor, new: torch.Tensor, block_table: torch.Tensor
     With ``n_heads`` and ``n_kv_heads`` the plan also holds what ``attention`` needs for layers of these heads, for each of
     ``windows`` (0 = no window).  ``group_start [groups + 1]`` and ``group_prefix [groups]`` declare that the sequences
     ``group_start[g] .. group_start[g + 1]`` share their first ``group_prefix[g]`` tokens: their table rows begin with the
-    same pages.  Offsets that are not in order are flagged and nothing is shared.  ``max_rows``: an upper bound of the new rows of one sequence or group, if the caller knows one.
-    ``shared_rows``: the same of the rows of all groups with a prefix and two or more sequences with rows: attention needs
-    ``2 shared_rows Hq (D + 2)`` floats of workspace for them, and a group beyond the bound is attended to without sharing.
-    Both cost speed only when they are wrong."""
+    same pages.  Offsets that are not in order are flagged and nothing is shared.  ``max_rows``: an upper bound of the new
+    rows of one sequence or group, if the caller knows one.  ``shared_rows``: the same of the rows of all groups with a prefix
+    and two or more sequences with rows: attention needs ``2 shared_rows Hq (D + 2)`` floats of workspace for them, and a
+    group beyond the bound is attended to without sharing.  Both cost speed only when they are wrong."""
     if page_size not in PAGE_SIZES:
         raise ValueError(f"page_plan: page_size must be one of {PAGE_SIZES}, got {page_size}")
     if (group_start is None) != (group_prefix is None) or (group_start is not None and group_start.numel() != group_prefix.numel() + 1):
@@ -131,9 +131,9 @@ def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pla
     denominator.  A row that sees no key, or only scores of minus infinity, is zero; a NaN among them makes it NaN, and a *value*
     that is not finite may make NaN of every row of its sequence in this step (of its group, when it lies in a shared
     prefix), as 0 * inf does in any product of probabilities and values.  Probabilities are rounded to the values' bf16 before
-    the product, scores, sums and partial outputs are fp32.  Rows behind the last sequence are zero, or left as they are when ``out`` is given.  For inference: no
-    gradient flows back.  Not batch-invariant on CUDA (the other sequences' lengths decide where a sequence's keys are cut
-    into partial sums), so batch-invariant mode refuses it."""
+    the product, scores, sums and partial outputs are fp32.  Rows behind the last sequence are zero, or left as they are when
+    ``out`` is given.  For inference: no gradient flows back.  Not batch-invariant on CUDA (the other sequences' lengths
+    decide where a sequence's keys are cut into partial sums), so batch-invariant mode refuses it."""
     R, hq, D = q.shape
     n_pages, hkv, ps, dk = k_pages.shape
     if not 1.2e-38 <= scale <= 2.3e38:               # times log2(e) a normal fp32 number: masked scores stay minus infinity
