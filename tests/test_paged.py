@@ -683,3 +683,49 @@ def test_a_negative_count_of_mapped_columns_is_flagged():
     p = paged.page_plan(_i32([0], "cuda"), _i32([1], "cuda"), table, _i32([0], "cuda"), _i32([2], "cuda"), 16, 1, num_pages=4, mapped=_i32([-3], "cuda"))
     assert ops.status(True) & 16
     assert table.tolist() == [[2, -5, -5]] and p.slot_map.tolist() == [32]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("groups,hq,hkv,D,ps,window", [
+    ([(0, [(0, 5), (20, 1)])], 4, 2, 64, 16, 0),                                     # rows of a prompt in one unit
+    ([(0, [(37, 3), (0, 2)]), (64, [(9, 2), (70, 1), (0, 1)])], 8, 2, 128, 32, 20),   # windows, a prefix that ends outside them
+    ([(0, [(30, 6)])], 4, 1, 256, 16, 8),
+    ([(0, [(100, 70), (3, 33)])], 16, 4, 128, 64, 0),                                # units of many rows
+    ([(0, [(0, 90)]), (128, [(c, 9) for c in range(0, 70, 5)])], 8, 1, 64, 32, 100),
+    ([(256, [(c, 3) for c in range(0, 150, 7)])], 14, 2, 128, 64, 64),
+])
+def test_values_that_a_row_does_not_see_do_not_reach_it(device, groups, hq, hkv, D, ps, window):
+    """Infinite and NaN values in keys of the step: a row that sees them gets what IEEE sums give in those columns, its other
+    columns and all other rows are what they were."""
+    s = _Step(groups, hq=hq, hkv=hkv, D=D, ps=ps, device=device, seed=5)
+    plan = s.plan((window,))
+    want, size = s.oracle(window)
+    rows, r0 = [], 0                                                                # (sequence, first row, position of each row)
+    for b, n in enumerate(s.new):
+        rows += [(b, s.cached[b] + i) for i in range(n)]
+    g = torch.Generator().manual_seed(1)
+    page_of = lambda b, pos: (s.pages_of[b][pos // ps], pos % ps)
+    planted = {}                                                                    # (page, slot, head, column) -> value
+    for _ in range(12):
+        b, pos = rows[int(torch.randint(0, len(rows), (1,), generator=g))]
+        pos = max(0, pos - int(torch.randint(0, window or 6, (1,), generator=g)))
+        where = (*page_of(b, pos), int(torch.randint(0, hkv, (1,), generator=g)), int(torch.randint(0, D, (1,), generator=g)))
+        planted[where] = [math.inf, -math.inf, math.nan][len(planted) % 3]
+    for (page, slot, h, c), v in planted.items():
+        s.vp[page, h, slot, c] = v
+    G = hq // hkv
+    hit = torch.zeros(s.R, hq, D, dtype=torch.float64)
+    by_key = {}
+    for (page, slot, h, c), v in planted.items():
+        by_key.setdefault((page, slot), []).append((h, c, v))
+    for r, (b, pos) in enumerate(rows):
+        for j in range(max(0, pos - window + 1) if window else 0, pos + 1):
+            for h, c, v in by_key.get(page_of(b, j), ()):
+                hit[r, h * G:(h + 1) * G, c] += v                                   # inf - inf is NaN
+    for _ in range(2):
+        got = paged.attention(s.q, s.kp, s.vp, plan, s.scale, window=window).cpu().double()
+        clean = hit == 0
+        assert torch.equal(got[~clean].nan_to_num(7.0, 8.0, 9.0), hit[~clean].nan_to_num(7.0, 8.0, 9.0))
+        err = (got - want).abs()[clean]
+        assert (err <= (2 ** -8 * want.abs() + (2 ** -8 + 2 ** -12) * size)[clean]).all()
+    assert clean.any() and not clean.all()

@@ -40,7 +40,7 @@ at::Tensor paged_work(const at::Tensor& cached, const at::Tensor& row_start, con
                       const c10::optional<at::Tensor>& group_prefix, int64_t table_cols, int64_t page_size,
                       int64_t total_rows, int64_t hq, int64_t hkv, int64_t window, int64_t shared_rows);
 void paged_attention(const at::Tensor& q, const at::Tensor& k_pages, const at::Tensor& v_pages, const at::Tensor& table,
-                     const at::Tensor& cached, const at::Tensor& row_start, const at::Tensor& work, int64_t groups, int64_t max_rows, int64_t shared_rows,
+                     const at::Tensor& slots, const at::Tensor& cached, const at::Tensor& row_start, const at::Tensor& work, int64_t groups, int64_t max_rows, int64_t shared_rows,
                      double scale, int64_t window, const c10::optional<at::Tensor>& sinks, at::Tensor out, bool zero_tail);
 int64_t status(bool clear);
 int64_t take_status(int64_t mask);
@@ -145,8 +145,8 @@ TORCH_LIBRARY(tb200, m) {
   m.def("paged_write(Tensor k, Tensor v, Tensor(a!) k_pages, Tensor(b!) v_pages, Tensor slot_map) -> ()", &tb200::paged_write);
   m.def("paged_work(Tensor cached, Tensor row_start, Tensor slots, Tensor? group_start, Tensor? group_prefix, int table_cols, "
         "int page_size, int total_rows, int hq, int hkv, int window, int shared_rows) -> Tensor", &tb200::paged_work);
-  m.def("paged_attention(Tensor q, Tensor k_pages, Tensor v_pages, Tensor table, Tensor cached, Tensor row_start, Tensor work, "
-        "int groups, int max_rows, int shared_rows, float scale, int window, Tensor? sinks, Tensor(a!) out, bool zero_tail) -> ()", &tb200::paged_attention);
+  m.def("paged_attention(Tensor q, Tensor k_pages, Tensor v_pages, Tensor table, Tensor slots, Tensor cached, Tensor row_start, "
+        "Tensor work, int groups, int max_rows, int shared_rows, float scale, int window, Tensor? sinks, Tensor(a!) out, bool zero_tail) -> ()", &tb200::paged_attention);
   m.def("status(bool clear) -> int", &tb200::status);
   m.def("take_status(int mask) -> int", &tb200::take_status);
   m.def("cross_entropy_(Tensor(a!) logits, Tensor labels, Tensor scale) -> Tensor", &tb200::cross_entropy_);

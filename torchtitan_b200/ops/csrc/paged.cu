@@ -234,7 +234,8 @@ struct __align__(16) Unit {
 // Layout of the int32 work buffer (one per window), from the sizes that the host knows.
 struct WorkLayout {
   int64_t seq_group, shared, group_row, src_a, src_b, tiles_a, tiles_b, units_a, units_b, size;
-  // header: [0, 1] units and tiles (of one key head) of the small sources in list A, [2, 3] of all, [4, 5] of list B
+  // header: [0, 1] units and tiles (of one key head) of the small sources in list A, [2, 3] of all, [4, 5] of list B, [6] whether
+  // a sequence that shares nothing has several rows
   __host__ __device__ WorkLayout(int64_t B, int64_t NG, int64_t max_a, int64_t max_b) {
     seq_group = 8;
     shared = seq_group + B;                      // rows of the groups that share, as running counts
@@ -325,6 +326,10 @@ __global__ void __launch_bounds__(1024) work_kernel(const WorkParams p) {
     }
     if (threadIdx.x == 0) shared[p.NG] = kept;
   }
+  bool several = false;
+  for (int b = threadIdx.x; b < p.B; b += blockDim.x) several |= p.row_start[b + 1] - p.row_start[b] > 1 && seq_group[b] < 0;
+  several = __syncthreads_or(several);
+  if (threadIdx.x == 0) p.work[6] = several;
   auto source_rows = [&](int s, int& r0, int& r1) {
     if (s < p.B) {
       r0 = p.row_start[s];
@@ -459,7 +464,9 @@ struct AttnParams {
   int64_t q_row, q_head;
   __nv_bfloat16* out;                            // [R, Hq, D]
   const float* sinks;                            // [Hq] or null
-  const int *table, *cached, *row_start, *work;
+  const int *table, *slots, *cached, *row_start, *work;
+  const __nv_bfloat16 *kp, *vp;                  // pages; strides in elements
+  int64_t kp_page, kp_head, kp_slot, vp_page, vp_head, vp_slot;
   int B, NG, W, R, Hq, Hkv, G, ps, num_pages, window, max_a, max_b, ctas_a, ctas_b, rows_b, ps_shift, max_shared;
   float scale_log2;
   bool zero_tail, use_b;                         // use_b: large sources run on the tcgen05 kernel
@@ -519,6 +526,7 @@ __device__ __forceinline__ uint32_t pack2bf(float lo, float hi) {
   __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<uint32_t*>(&h);
 }
+__device__ __forceinline__ bool any_nan(const float4& v) { return v.x != v.x || v.y != v.y || v.z != v.z || v.w != v.w; }
 __device__ __forceinline__ void consumer_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 // The same, true for all when any thread brings true.
 __device__ __forceinline__ bool consumer_any(bool v) {
@@ -1357,6 +1365,137 @@ attn_block_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
   }
 }
 
+// One row and query head, key by key, by a warp: for rows that have a NaN in their output.  Where the scores are numbers, that comes
+// from values that are not finite: one that the row sees, or one that only other rows of its unit see, since 0 * inf is a NaN
+// in the products above.  Looking for such values in every tile that some rows see and others do not cost a prompt of
+// 4096 rows 15 % (418 -> 483 us), and a test in the attention kernels' store loops 6 to 20 %, because it changed how their loops
+// over the tiles were compiled.  Looking at the outputs here costs 2 % of a prompt of 4096 rows (428 -> 436 us) and nothing of a
+// step of single rows.  A value that is not finite counts whatever its probability rounds to.
+template <int D>
+__device__ __noinline__ void attend_row(const AttnParams& p, int row, int h) {
+  constexpr int N = D / 32;
+  const int lane = threadIdx.x & 31;
+  const int b = find_segment_warp(p.row_start, p.B, row);
+  const int pos = p.cached[b] + row - p.row_start[b];
+  const int first = p.window > 0 ? max(0, pos - p.window + 1) : 0;
+  const int last = (int)min((int64_t)pos, (int64_t)p.W * p.ps - 1);
+  const int* table = p.table + (int64_t)p.slots[b] * p.W;
+  const __nv_bfloat16* k0 = p.kp + (h / p.G) * p.kp_head;
+  const __nv_bfloat16* v0 = p.vp + (h / p.G) * p.vp_head + lane * N;
+  const uint32_t* q0 = reinterpret_cast<const uint32_t*>(p.q + (int64_t)row * p.q_row + (int64_t)h * p.q_head);
+  float o[N];
+#pragma unroll
+  for (int e = 0; e < N; ++e) o[e] = 0.f;
+  float m = -INFINITY, l = 0.f;
+  for (int base = first; base <= last; base += 32) {             // a key a lane
+    const int key = base + lane, slot = key & (p.ps - 1);
+    const int page = key <= last ? table[key >> p.ps_shift] : -1;
+    const bool there = page >= 0 && page < p.num_pages;          // else zeros, as in the kernels above
+    const uint4* k = reinterpret_cast<const uint4*>(k0 + page * p.kp_page + slot * p.kp_slot);
+    float s = 0.f;
+#pragma unroll 4
+    for (int c = 0; c < D / 8; ++c) {
+      const uint4 v = there ? k[c] : make_uint4(0, 0, 0, 0);
+      const uint32_t kw[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t qw = q0[4 * c + i];
+        s = fmaf(__uint_as_float(qw << 16), __uint_as_float(kw[i] << 16), s);
+        s = fmaf(__uint_as_float(qw & 0xffff0000u), __uint_as_float(kw[i] & 0xffff0000u), s);
+      }
+    }
+    s = key <= last ? s * p.scale_log2 : -INFINITY;
+    if (__any_sync(0xffffffffu, s != s)) {       // so is the sum, and every output
+      l = s = __uint_as_float(0x7fffffffu);
+      break;
+    }
+    const float top = fmaxf(m, warp_max(s));
+    if (top == -INFINITY) continue;
+    const float a = m == -INFINITY ? 0.f : exp2f(m - top), w = exp2f(s - top);
+    m = top;
+    l = l * a + warp_sum(w);
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      if (fabsf(o[e]) < INFINITY) o[e] *= a;
+    const int64_t at = there ? page * p.vp_page + slot * p.vp_slot : -1;
+    unsigned seen = __ballot_sync(0xffffffffu, s > -INFINITY && there);
+    while (seen != 0u) {
+      float wj[4], v[4][N];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {              // four values in flight
+        const int k = seen != 0u ? __ffs(seen) - 1 : -1;
+        seen &= seen - 1;
+        wj[j] = k < 0 ? 0.f : __shfl_sync(0xffffffffu, w, k);
+        const int64_t row_at = k < 0 ? -1 : __shfl_sync(0xffffffffu, at, k);
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[j][e] = k < 0 ? 0.f : __bfloat162float(v0[row_at + e]);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int e = 0; e < N; ++e) o[e] = fabsf(v[j][e]) < INFINITY ? fmaf(wj[j], v[j][e], o[e]) : o[e] + v[j][e];
+    }
+  }
+  float f = 1.f;
+  if (p.sinks != nullptr) {
+    const float sk = p.sinks[h] * 1.4426950408889634f, top = fmaxf(sk, m);
+    f = m == -INFINITY ? 0.f : exp2f(m - top);
+    l = l * f + (sk == -INFINITY ? 0.f : exp2f(sk - top));
+  }
+  f = l == 0.f ? 0.f : f / l;
+  __nv_bfloat16* out = p.out + ((int64_t)row * p.Hq + h) * D + lane * N;
+#pragma unroll
+  for (int e = 0; e < N; ++e)
+    if (f != f || !(fabsf(o[e]) >= INFINITY)) o[e] *= f;         // an infinity stays one unless the sum is a NaN
+#pragma unroll
+  for (int e = 0; e < N; e += 2) *reinterpret_cast<uint32_t*>(out + e) = pack2bf(o[e], o[e + 1]);
+}
+// The same for the rows of 32 adjacent vectors of the output, from vector `c0`, where a lane saw a NaN: those that the attention
+// kernels finished.  A row that this kernel joins may not be there yet; it is looked at where it is joined.
+template <int D>
+__device__ __noinline__ void attend_again(const AttnParams& p, int64_t c0, bool nan) {
+  constexpr int kV = D / 8;
+  const int lane = threadIdx.x & 31;
+  const int* seq_group = p.work + WorkLayout(p.B, p.NG, p.max_a, p.max_b).seq_group;
+  for (unsigned left = __ballot_sync(0xffffffffu, nan); left != 0u;) {
+    const int k = (__ffs(left) - 1) / kV * kV;   // first lane of the row
+    left &= ~((kV == 32 ? 0xffffffffu : (1u << (kV & 31)) - 1u) << k);
+    const int64_t rh = (c0 + k) / kV;
+    const int row = (int)(rh / p.Hq), h = (int)(rh % p.Hq);
+    const int b = find_segment_warp(p.row_start, p.B, row);
+    const int pr = (row - p.row_start[b]) * p.G + h % p.G;
+    bool joined = seq_group[b] >= 0;
+    for (int i = lane; i < p.ctas_a + (p.use_b ? p.ctas_b : 0); i += 32) {
+      const Cut u = p.cuts[i];
+      joined |= u.parts > 0 && u.row0 == p.row_start[b] && u.head == h / p.G && pr >= u.pair0 && pr < u.pair0 + (i < p.ctas_a ? kRowsA : p.rows_b * p.G);
+    }
+    if (!__any_sync(0xffffffffu, joined)) attend_row<D>(p, row, h);
+  }
+}
+__device__ __forceinline__ bool any_nan(const uint4& v) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  bool nan = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) nan |= (w[i] & 0x7fffu) > 0x7f80u || (w[i] & 0x7fff0000u) > 0x7f800000u;
+  return nan;
+}
+// Block `block` of `blocks` looks at its share of the output.  Only where a sequence has several rows: the pairs of one row see
+// the same keys, and values outside those are cleared above.
+template <int D>
+__device__ __forceinline__ void look_for_nan(const AttnParams& p, int last_row, int block, int blocks) {
+  const int64_t n = (int64_t)last_row * p.Hq * (D / 8), step = (int64_t)blocks * 128;
+  const uint4* out = reinterpret_cast<const uint4*>(p.out);
+  const int lane = threadIdx.x & 31;
+  for (int64_t c = (int64_t)block * 128 + threadIdx.x - lane; c < n; c += 4 * step) {
+    uint4 v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = c + i * step + lane < n ? out[c + i * step + lane] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (__any_sync(0xffffffffu, any_nan(v[i]))) attend_again<D>(p, c + i * step, any_nan(v[i]));
+  }
+}
+
 // Joins what the attention kernels left in parts.  Blocks [0, cuts): a sequence that shares nothing is in parts where a
 // stretch boundary cuts one of its units; a CTA has at most one cut unit that begins in its stretch and goes on behind it
 // and left its description, and the block(s) of that CTA join it.  The other blocks: a (row, query head) of a group that
@@ -1365,12 +1504,13 @@ attn_block_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
 constexpr int kSlices = 8;                       // blocks that share a cut unit of 128 pairs
 
 template <int D>
-__global__ void __launch_bounds__(128, 8) finish_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(128, 8) finish_kernel(const __grid_constant__ AttnParams p) {
   constexpr int N = D / 32;
   const int lane = threadIdx.x & 31;
   const WorkLayout lay(p.B, p.NG, p.max_a, p.max_b);
   const int cuts = p.ctas_a + (p.use_b ? p.ctas_b * kSlices : 0);
   const int last_row = p.row_start[p.B];
+  const bool several = p.work[6] != 0;
   auto finish = [&](int64_t rh, float m, float l) {              // 1 / denominator, with the head's sink
     float f = 1.f;
     if (p.sinks != nullptr) {
@@ -1386,6 +1526,7 @@ __global__ void __launch_bounds__(128, 8) finish_kernel(const AttnParams p) {
     const int row0 = big ? (blockIdx.x - p.ctas_a) % kSlices * (kRowsB / kSlices) : 0;      // this block's rows of the unit
     const int rows = big ? kRowsB : kRowsA;
     wait_for_earlier();
+    if (several) look_for_nan<D>(p, last_row, blockIdx.x, cuts);
     const Cut unit = p.cuts[big ? p.ctas_a + c0 : c0];
     const int parts = min(unit.parts, (big ? p.ctas_b : p.ctas_a) - c0), head = unit.head;
     if (p.zero_tail) {
@@ -1398,6 +1539,7 @@ __global__ void __launch_bounds__(128, 8) finish_kernel(const AttnParams p) {
     const float* pml = big ? p.part_b_ml : p.part_a_ml;
     auto part = [&](int i, int row) { return i == 0 ? ((int64_t)c0 * 2 + 1) * rows + row : (int64_t)(c0 + i) * 2 * rows + row; };
     const int live = min(big ? min(row0 + kRowsB / kSlices, p.rows_b * p.G) : rows, unit.pairs - unit.pair0);
+    bool again = false;
     for (int c = threadIdx.x; c < (live - row0) * (D / 4); c += 128) {
       const int row = row0 + c / (D / 4), d = (c % (D / 4)) * 4;
       // eight parts at a time, all their loads in flight together
@@ -1434,8 +1576,13 @@ __global__ void __launch_bounds__(128, 8) finish_kernel(const AttnParams p) {
       const int pr = unit.pair0 + row;
       const int64_t rh = (int64_t)(unit.row0 + pr / p.G) * p.Hq + head * p.G + pr % p.G;
       const float f = finish(rh, m, l);
-      *reinterpret_cast<uint2*>(p.out + rh * D + d) = make_uint2(pack2bf(o.x * f, o.y * f), pack2bf(o.z * f, o.w * f));
+      const float4 y = make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
+      again |= any_nan(y) && l == l;
+      *reinterpret_cast<uint2*>(p.out + rh * D + d) = make_uint2(pack2bf(y.x, y.y), pack2bf(y.z, y.w));
     }
+    if (__syncthreads_or(again))                 // all of the block's rows, which are few
+      for (int pr = unit.pair0 + row0 + (threadIdx.x >> 5); pr < unit.pair0 + live; pr += 4)
+        attend_row<D>(p, unit.row0 + pr / p.G, head * p.G + pr % p.G);
     return;
   }
 
@@ -1534,8 +1681,14 @@ __global__ void __launch_bounds__(128, 8) finish_kernel(const AttnParams p) {
     }
     const float f = finish(rh, m, l);
     __nv_bfloat16* out = p.out + rh * D + lane * N;
+    bool again = false;
 #pragma unroll
-    for (int e = 0; e < N; e += 2) *reinterpret_cast<uint32_t*>(out + e) = pack2bf(o[e] * f, o[e + 1] * f);
+    for (int e = 0; e < N; e += 2) {
+      const float a = o[e] * f, c = o[e + 1] * f;
+      again |= a != a || c != c;
+      *reinterpret_cast<uint32_t*>(out + e) = pack2bf(a, c);
+    }
+    if (__any_sync(0xffffffffu, again && l == l)) attend_row<D>(p, r, h);
   }
   if (!waited) wait_for_earlier();               // a block without a row still ends behind the earlier kernels
 }
@@ -1707,7 +1860,7 @@ static CUtensorMap query_map(const at::Tensor& q, int group, int rows) {
 }
 
 void paged_attention(const at::Tensor& q, const at::Tensor& k_pages, const at::Tensor& v_pages, const at::Tensor& table,
-                     const at::Tensor& cached, const at::Tensor& row_start, const at::Tensor& work, int64_t groups, int64_t max_rows, int64_t shared_rows,
+                     const at::Tensor& slots, const at::Tensor& cached, const at::Tensor& row_start, const at::Tensor& work, int64_t groups, int64_t max_rows, int64_t shared_rows,
                      double scale, int64_t window, const c10::optional<at::Tensor>& sinks, at::Tensor out, bool zero_tail) {
   check_pages(k_pages, v_pages, "paged_attention");
   const auto dev = k_pages.device();
@@ -1735,6 +1888,10 @@ void paged_attention(const at::Tensor& q, const at::Tensor& k_pages, const at::T
   p.out = (__nv_bfloat16*)out.data_ptr();
   p.sinks = sinks.has_value() ? sinks->data_ptr<float>() : nullptr;
   p.table = table.data_ptr<int>();
+  p.slots = int_vector(slots, B, dev, "slots");
+  p.kp = (const __nv_bfloat16*)k_pages.data_ptr(); p.vp = (const __nv_bfloat16*)v_pages.data_ptr();
+  p.kp_page = k_pages.stride(0); p.kp_head = k_pages.stride(1); p.kp_slot = k_pages.stride(2);
+  p.vp_page = v_pages.stride(0); p.vp_head = v_pages.stride(1); p.vp_slot = v_pages.stride(2);
   p.cached = int_vector(cached, B, dev, "cached");
   p.row_start = int_vector(row_start, B + 1, dev, "row_start");
   p.B = (int)B; p.NG = (int)groups; p.W = (int)table.size(1); p.R = (int)R;

@@ -128,11 +128,10 @@ def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pla
               sinks: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """``q [R, Hq, D]`` -> ``[R, Hq, D]``: row ``r`` at position ``p`` of its sequence attends to the tokens
     ``max(0, p - window + 1) .. p`` (``window = 0``: all up to ``p``).  ``sinks [Hq]``: one logit per head in the softmax
-    denominator.  A row that sees no key, or only scores of minus infinity, is zero; a NaN among them makes it NaN, and a *value*
-    that is not finite may make NaN of every row of its sequence in this step (of its group, when it lies in a shared
-    prefix), as 0 * inf does in any product of probabilities and values.  Probabilities are rounded to the values' bf16 before
-    the product, scores, sums and partial outputs are fp32.  Rows behind the last sequence are zero, or left as they are when
-    ``out`` is given.  For inference: no gradient flows back.  Not batch-invariant on CUDA (the other sequences' lengths
+    denominator.  A row that sees no key, or only scores of minus infinity, is zero; a NaN among its scores makes it NaN.  Values
+    that are not finite reach the rows that see them, in their own columns, and no others (rows that have a NaN are computed
+    again, key by key, which takes longer).  Probabilities are rounded to the values' bf16 before the product, scores, sums
+    and partial outputs are fp32.  Rows behind the last sequence are zero, or left as they are when ``out`` is given.  For inference: no gradient flows back.  Not batch-invariant on CUDA (the other sequences' lengths
     decide where a sequence's keys are cut into partial sums), so batch-invariant mode refuses it."""
     R, hq, D = q.shape
     n_pages, hkv, ps, dk = k_pages.shape
@@ -168,6 +167,6 @@ def attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pla
     if sinks is not None and (sinks.dtype != torch.float32 or not sinks.is_contiguous()):
         sinks = sinks.float().contiguous()
     dst = q.new_empty((R, hq, D)) if out is None else out
-    ext.require().paged_attention(_vectors(q), k_pages, v_pages, plan.block_table, plan.cached, plan.row_start, work, plan.groups,
+    ext.require().paged_attention(_vectors(q), k_pages, v_pages, plan.block_table, plan.slots, plan.cached, plan.row_start, work, plan.groups,
                                   plan.max_rows, plan.shared_rows, float(scale), int(window), sinks, dst, out is None)
     return dst

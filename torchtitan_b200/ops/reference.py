@@ -229,7 +229,14 @@ def paged_attention(q, k_pages, v_pages, block_table, slots, cached, row_start, 
         if ids.numel() * ps < L or any(not 0 <= i < k_pages.shape[0] for i in ids.tolist()):
             raise ValueError(f"paged attention: the pages of slot {s} do not hold {L} tokens or lie outside the pool")
         k, v = (p[ids].transpose(0, 1).reshape(Hkv, -1, D)[:, :L].transpose(0, 1) for p in (k_pages, v_pages))
-        o, lse = block_attention_fwd(q[r0:r1], k, v, scale, True, c, None, window)
+        if bool(torch.isfinite(v).all()):
+            o, lse = block_attention_fwd(q[r0:r1], k, v, scale, True, c, None, window)
+        else:                                    # row by row: 0 * inf of a key that a row does not see is no part of it
+            parts = []
+            for i in range(c, L):
+                seen = slice(max(0, i - window + 1) if window else 0, i + 1)
+                parts.append(block_attention_fwd(q[r0 + i - c:r0 + i - c + 1], k[seen], v[seen], scale, False))
+            o, lse = torch.cat([p[0] for p in parts]), torch.cat([p[1] for p in parts], 1)
         if sinks is not None:
             o = (o.float() * torch.sigmoid(lse - sinks.float()[:, None]).t()[..., None]).to(q.dtype)
         out[r0:r1] = o
