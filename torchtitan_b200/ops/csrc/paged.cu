@@ -937,10 +937,10 @@ attn_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_consta
 // The exponentials (64 x 128 per tile on a 16-per-clock unit) and the MMAs take 512 clocks a tile each; the issuing thread's
 // own work (two waits, twelve MMAs of 60 to 75 clocks, three commits) takes some 1700 and bounds the kernel: 4 groups of
 // 16 sequences behind 65536 tokens, 4 key heads: 139 us for 537 MB (3.9 TB/s); one group of 64: 586 TFLOP/s; 512 rows behind
-// 8192 tokens, 32 + 8 heads of 128: 129 us (550 TFLOP/s).  A prompt is slower: 4096 rows alone take 418 us, 329 TFLOP/s counted
+// 8192 tokens, 32 + 8 heads of 128: 128 us (555 TFLOP/s).  A prompt is slower: 4096 rows alone take 437 us, 315 TFLOP/s counted
 // over the keys that a row sees, some 3500 clocks a tile, which the issuing thread does not explain; what does has not been
 // measured (its units are short, 32 tiles in the mean, with one buffer for the queries and an output to drain each).  The flash
-// forward, which keeps two query tiles per tile of keys, takes 161 us.
+// forward, which keeps two query tiles per tile of keys, takes 157 us.
 // P is rounded to bf16 before it meets V, as in the flash kernels: the tensor cores take the values' type.
 //   warp 0: TMA producer    warp 1: TMEM, MMA issue    warps 2..5, 6..9: softmax of even / odd tiles, then the output
 // Tensor memory: score buffer b (of warpgroup b % 2) at column 64 b, accumulator of warpgroup g at 256 + 128 g.
@@ -1369,7 +1369,7 @@ attn_block_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_const
 // from values that are not finite: one that the row sees, or one that only other rows of its unit see, since 0 * inf is a NaN
 // in the products above.  Looking for such values in every tile that some rows see and others do not cost a prompt of
 // 4096 rows 15 % (418 -> 483 us), and a test in the attention kernels' store loops 6 to 20 %, because it changed how their loops
-// over the tiles were compiled.  Looking at the outputs here costs 2 % of a prompt of 4096 rows (428 -> 436 us) and nothing of a
+// over the tiles were compiled.  Looking at the outputs here costs 2 % of a prompt of 4096 rows (427 -> 437 us) and nothing of a
 // step of single rows.  A value that is not finite counts whatever its probability rounds to.
 template <int D>
 __device__ __noinline__ void attend_row(const AttnParams& p, int row, int h) {
